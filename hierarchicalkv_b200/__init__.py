@@ -18,14 +18,34 @@ from .table import (  # noqa: F401
     library_path,
     load_library,
 )
+from .rows import (  # noqa: F401,E402
+    ExpertOrder,
+    expert_combine,
+    expert_combine_backward,
+    expert_dispatch,
+    expert_dispatch_backward,
+    expert_sort,
+    layer_norm,
+    layer_norm_backward,
+    layer_norm_ptr,
+)
 
 __all__ = [
     "CudaException",
     "EvictStrategy",
+    "ExpertOrder",
     "HashTable",
     "HashTableOptions",
     "MerlinException",
     "Predicate",
+    "expert_combine",
+    "expert_combine_backward",
+    "expert_dispatch",
+    "expert_dispatch_backward",
+    "expert_sort",
+    "layer_norm",
+    "layer_norm_backward",
+    "layer_norm_ptr",
     "library_path",
     "load_library",
 ]

@@ -2,7 +2,7 @@
 
     python -m hierarchicalkv_b200.build
 
-nvcc cross-compiles without a GPU; the four translation units compile in
+nvcc cross-compiles without a GPU; the translation units compile in
 parallel and are linked into one shared object beside this file.
 """
 from __future__ import annotations
@@ -18,8 +18,8 @@ ROOT = os.path.dirname(HERE)
 LIB_PATH = os.path.join(HERE, "libhkv_b200.so")
 
 SOURCES = ["hkv_api.cu", "hkv_find.cu", "hkv_upsert.cu", "hkv_scan.cu", "hkv_noalloc.cu", "hkv_shard.cu",
-           "hkv_sharded.cu"]
-HEADERS = ["hkv_device.cuh", "hkv_internal.h"]
+           "hkv_sharded.cu", "hkv_expert.cu", "hkv_norm.cu"]
+HEADERS = ["hkv_device.cuh", "hkv_internal.h", "hkv_rows.cuh", "hkv_norm.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -21,6 +21,7 @@
 #include "../../include/hkv_b200.h"
 #include "hkv_device.cuh"
 #include "hkv_internal.h"
+#include "hkv_norm.h"
 
 namespace {
 
@@ -1246,6 +1247,55 @@ int hkv_find_ptr(hkv_table* t, uint64_t n, const uint64_t* keys, void** values, 
     hkv::launch_find_ptr(t->view, n, keys, values, founds, scores_w.get(), s);
     ls.done();
     check_launch();
+  });
+}
+
+int hkv_find_layer_norm(hkv_table* t, uint64_t n, const uint64_t* keys, const void* weight,
+                        const void* bias, uint32_t param_kind, float eps, void* values,
+                        bool* founds, float* mean, float* rstd, hkv_stream stream) {
+  return guarded([&] {
+    refuse_in_memory_mode(t, "find_layer_norm");
+    uint32_t kind = t->view.value_kind;
+    if (kind == hkv::kValueOpaque && t->opt.value_size == 4) kind = hkv::kValueF32;
+    HKV_CHECK(kind == hkv::kValueF32 || kind == hkv::kValueF16 || kind == hkv::kValueBF16,
+              "find_layer_norm: the table's values must be float, half or bfloat16.");
+    if ((param_kind != kind && param_kind != hkv::kValueF32) || !(eps >= 0.f && eps <= 3.4e38f)) {
+      throw HkvError{HKV_ERR_INVALID_ARG,
+                     "find_layer_norm: weight and bias have the rows' type or float, eps is finite "
+                     "and not negative"};
+    }
+    if (n == 0) return;
+    if (n >= (1ull << 31) || keys == nullptr || values == nullptr || founds == nullptr) {
+      throw HkvError{HKV_ERR_INVALID_ARG,
+                     "find_layer_norm: keys, values and founds must not be null, n below 2^31"};
+    }
+    DeviceGuard dg(t->device);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    WorkspaceLease work(t, 0, n * sizeof(void*), s);   // the rows' addresses
+    if (work.get() == nullptr) {
+      throw HkvError{HKV_ERR_CUDA, "find_layer_norm: out of device memory for the row addresses"};
+    }
+    hkv::NormArgs a{};
+    a.n = n;
+    a.dim = t->opt.dim;
+    a.row_ptrs = static_cast<const void* const*>(work.get());
+    a.weight = weight;
+    a.bias = bias;
+    a.params_f32 = param_kind == hkv::kValueF32;
+    a.eps = eps;
+    a.inv_dim = 1.f / float(a.dim);
+    a.y = values;
+    a.y_stride = t->view.row_bytes;
+    a.mean = mean;
+    a.rstd = rstd;
+    // one reader lock over both launches: no update comes between the lookup
+    // and the reading of the rows
+    LockScope ls(t, kReader, s);
+    hkv::launch_find_ptr(t->view, n, keys, static_cast<void**>(work.get()), founds, nullptr, s);
+    const int rc = hkv::launch_norm(a, kind, s);
+    ls.done();
+    check_launch();
+    if (rc != HKV_OK) throw HkvError{rc, hkv_rows_last_error()};
   });
 }
 

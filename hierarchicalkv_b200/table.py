@@ -136,6 +136,8 @@ def library_path() -> str:
 _P = ctypes.c_void_p
 _U64 = ctypes.c_uint64
 _INT = ctypes.c_int
+_U32 = ctypes.c_uint32
+_F32 = ctypes.c_float
 
 # name -> argtypes (restype is int unless listed in _RESTYPES)
 _SIGNATURES = {
@@ -196,6 +198,19 @@ _SIGNATURES = {
     "hkv_sharded_upsert": [_P, _INT, _U64, _P, _INT, ctypes.c_uint32, _P],
     "hkv_sharded_status": [_P, ctypes.c_uint32, _P, ctypes.POINTER(ctypes.c_uint32)],
     "hkv_sharded_last_error": [],
+    "hkv_expert_sort_workspace_bytes": [_U64, _U32, _U32],
+    "hkv_expert_sort": [_U64, _U32, _P, _U32, _U32, _P, _P, _P, _P, _U64, _P],
+    "hkv_expert_dispatch": [_U64, _U32, _U64, _P, _U64, _U32, _P, _P, _P, _U64, _INT, _P],
+    "hkv_expert_combine": [_U64, _U32, _U64, _U32, _P, _U64, _P, _U32, _P, _P, _U64, _P],
+    "hkv_expert_combine_backward": [_U64, _U32, _U64, _U32, _P, _U64, _P, _U64, _P, _U32, _U32, _P,
+                                    _P, _P, _U64, _INT, _P, _P],
+    "hkv_layer_norm": [_U64, _U64, _U32, _P, _U64, _P, _P, _U32, _F32, _P, _U64, _P, _P, _P],
+    "hkv_layer_norm_ptr": [_U64, _U64, _U32, _P, _P, _P, _U32, _F32, _P, _U64, _P, _P, _P],
+    "hkv_find_layer_norm": [_P, _U64, _P, _P, _P, _U32, _F32, _P, _P, _P, _P, _P],
+    "hkv_layer_norm_backward_workspace_bytes": [_U64, _U64, _U32],
+    "hkv_layer_norm_backward": [_U64, _U64, _U32, _P, _U64, _P, _U64, _P, _U32, _P, _P, _P, _U64, _P,
+                                _P, _P, _U64, _P],
+    "hkv_rows_last_error": [],
     "hkv_accum_or_assign_unique": [_P, _U64, _P, _P, _P, _P, _P, _INT],
     "hkv_size_no_alloc": [_P, _P, ctypes.POINTER(_U64)],
     "hkv_size_no_alloc_last_error": [],
@@ -225,6 +240,9 @@ _RESTYPES = {
     "hkv_last_error": ctypes.c_char_p,
     "hkv_size_no_alloc_last_error": ctypes.c_char_p,
     "hkv_shard_last_error": ctypes.c_char_p,
+    "hkv_expert_sort_workspace_bytes": _U64,
+    "hkv_layer_norm_backward_workspace_bytes": _U64,
+    "hkv_rows_last_error": ctypes.c_char_p,
 }
 
 
@@ -432,6 +450,36 @@ class HashTable:
     def find(self, n, keys, values, founds, scores=None, stream=None) -> None:
         self._call("hkv_find", n, _ptr(keys), _ptr(values), _ptr(founds), _ptr(scores),
                    _stream(stream))
+
+    def find_layer_norm(self, n, keys, values, founds, weight=None, bias=None, eps=1e-5,
+                        mean=None, rstd=None, stream=None) -> None:
+        """find whose rows pass through layer norm on their way into ``values``:
+        the rows are normalised straight from the table, without a copy of them
+        in between.  Rows of misses are left as they are, as find leaves them.
+        ``weight`` / ``bias`` (dim elements of the value type or float32, both of
+        one type; None: ones / zeros), ``mean`` / ``rstd`` (float32, optional):
+        what layer_norm_backward needs.  Values must be float32, float16 or
+        bfloat16."""
+        dim = self._opts.dim if self._opts is not None else 0
+        kind = None
+        for name, p in (("weight", weight), ("bias", bias)):
+            if p is None:
+                continue
+            if p.dtype not in (self.value_dtype, torch.float32) or kind not in (None, p.dtype):
+                raise ValueError(f"{name} must have the value type or float32, weight and bias one type")
+            if p.numel() != dim:
+                raise ValueError(f"{name} must have dim = {dim} elements")
+            kind = p.dtype
+        if values.dtype != self.value_dtype or values.numel() < n * dim:
+            raise ValueError("values must hold n rows of the table's value type")
+        if keys.numel() < n or founds.numel() < n:
+            raise ValueError("keys and founds must hold n elements")
+        for name, s in (("mean", mean), ("rstd", rstd)):
+            if s is not None and (s.dtype != torch.float32 or s.numel() < n):
+                raise ValueError(f"{name} must hold n float32 elements")
+        self._call("hkv_find_layer_norm", n, _ptr(keys), _ptr(weight), _ptr(bias),
+                   _VALUE_KINDS.get(kind or self.value_dtype, 0), eps, _ptr(values), _ptr(founds),
+                   _ptr(mean), _ptr(rstd), _stream(stream))
 
     def find_host(self, n, keys, values, founds, scores=None, stream=None) -> None:
         """find for a batch in host memory (CPU tensors, pinned for asynchronous

@@ -522,6 +522,102 @@ HKV_API int hkv_accum_or_assign_unique(hkv_table* table, uint64_t n, const uint6
                                        const uint64_t* scores, hkv_stream stream,
                                        int ignore_evict_strategy);
 
+/* ---- row operators of a model ------------------------------------------------
+ * What a model does with the rows of a table next: layer norm, and the routing
+ * of token rows to experts and back.  No counterpart in the reference.  Buffers
+ * must be GPU-accessible and start at a multiple of their element size, as
+ * everywhere (include/merlin_hashtable.cuh:216-221); strides are in bytes;
+ * rows may lie apart, a row itself is contiguous; outputs must not overlap inputs.
+ * value_kind (HKV_VALUE_F32 / F16 / BF16) names the rows' element type; weights,
+ * biases and their gradients have that type or float (weight_kind / param_kind).
+ * Sums are in 32-bit floats, results are rounded once and do not depend on the
+ * order in which blocks run.  The calls enqueue on `stream` (of the current
+ * device), allocate nothing and keep nothing: they may be captured, and calls
+ * that run at the same time need workspaces of their own. */
+
+/* Sorts the tokens * top_k assignments of tokens to experts by expert (buffers as
+ * in include/merlin_hashtable.cuh:216-221).  expert_ids[tokens][top_k], int32 or
+ * int64 (id_bytes); ids outside [0, experts) drop the assignment.  The sort is stable:
+ * within an expert the rows keep the order of assignment t * top_k + j.
+ * offsets[experts + 1]: expert e's rows are [offsets[e], offsets[e + 1]);
+ * position[tokens][top_k]: the row of each assignment, -1 if dropped;
+ * source[tokens * top_k]: the assignment of each row, -1 behind the last row.
+ * At most 1024 experts, top_k 64, 2^31 - 1 assignments.  `work`: scratch of
+ * hkv_expert_sort_workspace_bytes (0 for all but large batches). */
+HKV_API uint64_t hkv_expert_sort_workspace_bytes(uint64_t tokens, uint32_t top_k, uint32_t experts);
+HKV_API int hkv_expert_sort(uint64_t tokens, uint32_t top_k, const void* expert_ids,
+                            uint32_t id_bytes, uint32_t experts, int32_t* offsets,
+                            int32_t* position, int32_t* source, void* work, uint64_t work_bytes,
+                            hkv_stream stream);
+/* rows[position[t][j]] = x[t], bytes as in hkv_shard_gather_rows (any element
+ * type; GPU-accessible as in include/merlin_hashtable.cuh:216-221).  The rows from
+ * offsets[experts] on are zeroed with zero_rows_behind, else left as they are. */
+HKV_API int hkv_expert_dispatch(uint64_t tokens, uint32_t top_k, uint64_t row_bytes, const void* x,
+                                uint64_t x_stride, uint32_t experts, const int32_t* offsets,
+                                const int32_t* position, void* rows, uint64_t rows_stride,
+                                int zero_rows_behind, hkv_stream stream);
+/* out[t] = sum over j of weights[t][j] * rows[position[t][j]]; a token none of
+ * whose assignments was kept gets zeros.  weights null: ones, which is the
+ * gradient of hkv_expert_dispatch (include/merlin_hashtable.cuh:216-221 for the
+ * buffers). */
+HKV_API int hkv_expert_combine(uint64_t tokens, uint32_t top_k, uint64_t dim, uint32_t value_kind,
+                               const void* rows, uint64_t rows_stride, const void* weights,
+                               uint32_t weight_kind, const int32_t* position, void* out,
+                               uint64_t out_stride, hkv_stream stream);
+/* Gradients of hkv_expert_combine: d_rows[position[t][j]] = weights[t][j] * d_out[t],
+ * d_weights[t][j] = <d_out[t], rows[position[t][j]]>, 0 for dropped assignments
+ * (include/merlin_hashtable.cuh:216-221 for the buffers).  The rows from
+ * offsets[experts] on are zeroed with zero_rows_behind, else left as they are. */
+HKV_API int hkv_expert_combine_backward(uint64_t tokens, uint32_t top_k, uint64_t dim,
+                                        uint32_t value_kind, const void* d_out,
+                                        uint64_t d_out_stride, const void* rows,
+                                        uint64_t rows_stride, const void* weights,
+                                        uint32_t weight_kind, uint32_t experts,
+                                        const int32_t* offsets, const int32_t* position,
+                                        void* d_rows, uint64_t d_rows_stride,
+                                        int zero_rows_behind, void* d_weights, hkv_stream stream);
+
+/* y = (x - mean) * rstd * weight + bias over rows of dim elements (those find
+ * returns, include/merlin_hashtable.cuh:2464-2577), rstd = 1 / sqrt(var + eps) with the
+ * variance over dim.  weight / bias null: ones / zeros.  mean and rstd (n floats
+ * each, may be null) are what the gradient needs. */
+HKV_API int hkv_layer_norm(uint64_t n, uint64_t dim, uint32_t value_kind, const void* x,
+                           uint64_t x_stride, const void* weight, const void* bias,
+                           uint32_t param_kind, float eps, void* y, uint64_t y_stride, float* mean,
+                           float* rstd, hkv_stream stream);
+/* The same on rows by address, as find* returns them
+ * (include/merlin_hashtable.cuh:2729-2787): the rows are read where the table keeps
+ * them and must stay valid and unchanged until the call has run.  Each address
+ * is null or a multiple of the widest of 16, 8, 4, 2 bytes that divides the row's
+ * length.  Null addresses (misses) leave y, mean and rstd of their row as they are. */
+HKV_API int hkv_layer_norm_ptr(uint64_t n, uint64_t dim, uint32_t value_kind,
+                               const void* const* row_ptrs, const void* weight, const void* bias,
+                               uint32_t param_kind, float eps, void* y, uint64_t y_stride,
+                               float* mean, float* rstd, hkv_stream stream);
+/* HashTable::find (include/merlin_hashtable.cuh:2464-2577) whose rows go through
+ * layer norm on their way out: find* and hkv_layer_norm_ptr under one reader lock.
+ * values[n][dim] has the table's element type (float, half or bfloat16); rows of
+ * misses are left as they are, founds[n] tells which. */
+HKV_API int hkv_find_layer_norm(hkv_table* table, uint64_t n, const uint64_t* keys,
+                                const void* weight, const void* bias, uint32_t param_kind,
+                                float eps, void* values, bool* founds, float* mean, float* rstd,
+                                hkv_stream stream);
+/* Gradients of hkv_layer_norm from dy, x and the mean and rstd it kept; dx goes
+ * back into the table as accum_or_assign's deltas
+ * (include/merlin_hashtable.cuh:1589-1692).  d_weight and d_bias (dim elements of
+ * param_kind, each may be null) are summed over the n rows.  `work`: scratch of
+ * hkv_layer_norm_backward_workspace_bytes. */
+HKV_API uint64_t hkv_layer_norm_backward_workspace_bytes(uint64_t n, uint64_t dim,
+                                                         uint32_t value_kind);
+HKV_API int hkv_layer_norm_backward(uint64_t n, uint64_t dim, uint32_t value_kind, const void* dy,
+                                    uint64_t dy_stride, const void* x, uint64_t x_stride,
+                                    const void* weight, uint32_t param_kind, const float* mean,
+                                    const float* rstd, void* dx, uint64_t dx_stride, void* d_weight,
+                                    void* d_bias, void* work, uint64_t work_bytes,
+                                    hkv_stream stream);
+/* Message of the last failed row operator (not hkv_find_layer_norm) of this thread. */
+HKV_API const char* hkv_rows_last_error(void);
+
 /* Device status word: bit 0 a bounded slot wait ran out, bit 1 eviction
  * retries ran out.  Reading it synchronises the stream; it is cleared by the
  * read.  (The reference spins without bound in these places:
