@@ -411,96 +411,87 @@ int launch_sort(uint64_t n, const ID* ids, uint32_t experts, int32_t* offsets, i
 //
 // Bound by HBM: T rows read, N written.  Token by token: a thread loads one
 // chunk of a token's row and stores it to the row's k places, so every row is
-// read once whatever k is.
+// read from memory once whatever k is.  Unaligned rows: the thread owns chunk i
+// of each place instead (places have alignments of their own) and cuts it out of
+// the token's row, which is in L1 after the first place.
 
 constexpr int kMoveBlock = 256;
 
-struct RowGrid {
-  uint32_t chunks;     // accesses per row
-  uint64_t total;      // rows * chunks
-};
+// Zeroes the rows behind the last expert's, if the caller asked for it.
+template <int G>
+__device__ __forceinline__ void zero_behind(const int32_t* kept, uint64_t n, uint8_t* rows,
+                                            uint64_t rows_stride, uint64_t row_bytes) {
+  if (kept == nullptr) return;
+  for (uint64_t r = uint64_t(max(*kept, 0)) + blockIdx.x; r < n; r += gridDim.x) {
+    uint8_t* row = rows + r * rows_stride;
+    const uint32_t ahead = uint32_t(reinterpret_cast<uintptr_t>(row)) & 15u;
+    for (uint64_t at = threadIdx.x * 16ull; at < row_bytes + ahead; at += blockDim.x * 16ull) {
+      store_chunk<G>(row - ahead + at, make_uint4(0, 0, 0, 0), row, row + row_bytes);
+    }
+  }
+}
 
-template <int VB>
+// G == 0: all rows are whole aligned chunks; else pieces of G bytes at their ends.
+template <int G>
 __global__ void __launch_bounds__(kMoveBlock)
     dispatch_kernel(const uint64_t tokens, const uint32_t top_k, const uint32_t chunks,
-                    const uint8_t* __restrict__ x, const uint64_t x_stride,
-                    const int32_t* __restrict__ position, uint8_t* __restrict__ rows,
-                    const uint64_t rows_stride) {
-  using Raw = typename VecType<VB>::type;
+                    const uint64_t row_bytes, const RowsIn x, const int32_t* __restrict__ position,
+                    uint8_t* __restrict__ rows, const uint64_t rows_stride,
+                    const int32_t* __restrict__ kept) {
+  const uint64_t n = tokens * top_k;
+  zero_behind<(G ? G : 16)>(kept, n, rows, rows_stride, row_bytes);
   const uint64_t c = uint64_t(blockIdx.x) * kMoveBlock + threadIdx.x;
   const uint64_t token = c / chunks;
   if (token >= tokens) return;
-  const uint32_t off = uint32_t(c - token * chunks) * VB;
-  const Raw v = *reinterpret_cast<const Raw*>(x + token * x_stride + off);
-  const uint64_t n = tokens * top_k;
+  const uint64_t off = (c - token * chunks) * 16;
   const int32_t* at = position + token * top_k;
-  for (uint32_t j = 0; j < top_k; ++j) {
-    const uint32_t place = uint32_t(at[j]);   // -1 is above every place
-    if (place < n) *reinterpret_cast<Raw*>(rows + place * rows_stride + off) = v;
+  const uint8_t* from = x.first + token * x.stride;
+  if (G == 0) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(from + off));
+    for (uint32_t j = 0; j < top_k; ++j) {
+      const uint32_t place = uint32_t(at[j]);   // -1 is above every place
+      if (place < n) *reinterpret_cast<uint4*>(rows + place * rows_stride + off) = v;
+    }
+  } else {
+    for (uint32_t j = 0; j < top_k; ++j) {
+      const uint32_t place = uint32_t(at[j]);
+      if (place >= n) continue;
+      uint8_t* row = rows + place * rows_stride;
+      uint8_t* q = row - (uint32_t(reinterpret_cast<uintptr_t>(row)) & 15u) + off;
+      if (q >= row + row_bytes) continue;
+      const uint8_t* p = from + (q - row);
+      store_chunk<(G ? G : 16)>(
+          q, load_chunk<(G ? G : 16)>(p, p < from ? from : p, from + row_bytes, x.first, x.last),
+          row, row + row_bytes);
+    }
   }
-}
-
-// Zeroes the rows behind the last expert's.
-template <int VB>
-__global__ void __launch_bounds__(kMoveBlock)
-    zero_behind_kernel(const uint64_t n, const uint32_t chunks, const int32_t* __restrict__ kept,
-                       uint8_t* __restrict__ rows, const uint64_t rows_stride) {
-  using Raw = typename VecType<VB>::type;
-  const uint64_t first = uint64_t(max(*kept, 0));
-  if (first >= n) return;
-  const uint64_t total = (n - first) * chunks;
-  for (uint64_t c = uint64_t(blockIdx.x) * kMoveBlock + threadIdx.x; c < total;
-       c += uint64_t(gridDim.x) * kMoveBlock) {
-    const uint64_t row = c / chunks;
-    *reinterpret_cast<Raw*>(rows + (first + row) * rows_stride + (c - row * chunks) * VB) = Raw{};
-  }
-}
-
-#define HKV_FOR_ACCESS(vb, CALL) \
-  switch (vb) {                  \
-    case 16: CALL(16); break;    \
-    case 8: CALL(8); break;      \
-    case 4: CALL(4); break;      \
-    case 2: CALL(2); break;      \
-    default: CALL(1); break;     \
-  }
-
-void zero_behind(uint64_t n, uint64_t row_bytes, const int32_t* kept, void* rows,
-                 uint64_t rows_stride, cudaStream_t stream) {
-  const uint32_t vb = access_bytes(row_bytes | address_bits(rows) | rows_stride);
-  const uint32_t chunks = uint32_t(row_bytes / vb);
-  const uint64_t want = (n * chunks + kMoveBlock - 1) / kMoveBlock;
-  const uint64_t cap = uint64_t(sm_count()) * 8;
-  const unsigned grid = unsigned(want < cap ? want : cap);
-#define HKV_CALL(VB) \
-  zero_behind_kernel<VB><<<grid, kMoveBlock, 0, stream>>>(n, chunks, kept, static_cast<uint8_t*>(rows), rows_stride)
-  HKV_FOR_ACCESS(vb, HKV_CALL)
-#undef HKV_CALL
 }
 
 // ---- combine ------------------------------------------------------------------
 //
 // Bound by HBM: N rows read, T written.  A thread owns one chunk of a token's
-// row and sums the k rows' chunks in registers, in the order of j.
+// output row and sums the k rows' chunks in registers, in the order of j.
 
-template <typename T, int VB>
+template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(kMoveBlock)
     combine_kernel(const uint64_t tokens, const uint32_t top_k, const uint32_t chunks,
-                   const uint8_t* __restrict__ rows, const uint64_t rows_stride,
-                   const void* __restrict__ weights, const bool weights_f32,
-                   const int32_t* __restrict__ position, uint8_t* __restrict__ out,
-                   const uint64_t out_stride) {
-  using P = Pack<T, VB>;
+                   const uint64_t row_bytes, const RowsIn rows, const void* __restrict__ weights,
+                   const bool weights_f32, const int32_t* __restrict__ position,
+                   uint8_t* __restrict__ out, const uint64_t out_stride) {
+  using C = Chunk<T>;
   const uint64_t c = uint64_t(blockIdx.x) * kMoveBlock + threadIdx.x;
   const uint64_t token = c / chunks;
   if (token >= tokens) return;
-  const uint32_t off = uint32_t(c - token * chunks) * VB;
   const uint64_t n = tokens * top_k;
-  float sum[P::kElems];
+  uint8_t* to = out + token * out_stride;
+  int64_t off = int64_t(c - token * chunks) * 16;
+  if (!WHOLE) off -= uint32_t(reinterpret_cast<uintptr_t>(to)) & 15u;
+  if (!WHOLE && off >= int64_t(row_bytes)) return;
+  float sum[C::kElems];
 #pragma unroll
-  for (int e = 0; e < P::kElems; ++e) sum[e] = 0.f;
+  for (int e = 0; e < C::kElems; ++e) sum[e] = 0.f;
   for (uint32_t j0 = 0; j0 < top_k; j0 += 4) {
-    P row[4];
+    C row[4];
     float w[4];
     bool ok[4];
 #pragma unroll
@@ -511,7 +502,14 @@ __global__ void __launch_bounds__(kMoveBlock)
       ok[u] = place < n;
       w[u] = 1.f;
       if (ok[u]) {
-        row[u].raw = *reinterpret_cast<const typename P::Raw*>(rows + place * rows_stride + off);
+        const uint8_t* from = rows.first + place * rows.stride;
+        if (WHOLE) {
+          row[u].raw = __ldg(reinterpret_cast<const uint4*>(from + off));
+        } else {
+          const uint8_t* p = from + off;
+          row[u].raw = load_chunk<sizeof(T)>(p, off < 0 ? from : p, from + row_bytes, rows.first,
+                                             rows.last);
+        }
         if (weights != nullptr) {
           w[u] = weights_f32 ? static_cast<const float*>(weights)[i]
                              : to_float(static_cast<const T*>(weights)[i]);
@@ -522,37 +520,40 @@ __global__ void __launch_bounds__(kMoveBlock)
     for (int u = 0; u < 4; ++u) {
       if (!ok[u]) continue;
 #pragma unroll
-      for (int e = 0; e < P::kElems; ++e) sum[e] = fmaf(w[u], row[u].get(e), sum[e]);
+      for (int e = 0; e < C::kElems; ++e) sum[e] = fmaf(w[u], row[u].get(e), sum[e]);
     }
   }
-  P result;
+  C result;
 #pragma unroll
-  for (int e = 0; e < P::kElems; ++e) result.set(e, sum[e]);
-  *reinterpret_cast<typename P::Raw*>(out + token * out_stride + off) = result.raw;
+  for (int e = 0; e < C::kElems; ++e) result.set(e, sum[e]);
+  if (WHOLE) *reinterpret_cast<uint4*>(to + off) = result.raw;
+  else store_chunk<sizeof(T)>(to + off, result.raw, to, to + row_bytes);
 }
 
 // ---- combine, backward ----------------------------------------------------------
 //
 // Bound by HBM: T + N rows read, N written.  A group of threads takes a token;
-// a lane keeps its chunk of d_out in registers, and for four assignments at a
-// time loads the rows' chunks, stores w * d_out and adds to its four partial
-// dot products, which the group sums at the end.
+// for four assignments at a time a lane loads its chunks of the rows, stores
+// w * d_out and adds to its four partial dot products, which the group sums at
+// the end.  d_out's chunk is loaded once for the four; with unaligned rows each
+// place has its own cut of it, out of L1.
 
-template <typename T, int VB>
+template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(256)
     combine_backward_kernel(const uint64_t tokens, const uint32_t top_k, const uint32_t chunks,
-                            const uint32_t group, const uint8_t* __restrict__ d_out,
-                            const uint64_t d_out_stride, const uint8_t* __restrict__ rows,
-                            const uint64_t rows_stride, const void* __restrict__ weights,
+                            const uint32_t group, const uint64_t row_bytes, const RowsIn d_out,
+                            const RowsIn rows, const void* __restrict__ weights,
                             const bool weights_f32, const int32_t* __restrict__ position,
                             uint8_t* __restrict__ d_rows, const uint64_t d_rows_stride,
-                            void* __restrict__ d_weights) {
-  using P = Pack<T, VB>;
+                            void* __restrict__ d_weights, const int32_t* __restrict__ kept) {
+  using C = Chunk<T>;
   __shared__ float partial[8][4];
+  const uint64_t n = tokens * top_k;
+  zero_behind<sizeof(T)>(kept, n, d_rows, d_rows_stride, row_bytes);
   const uint32_t lane = threadIdx.x & (group - 1u);
   const uint64_t token = (uint64_t(blockIdx.x) * blockDim.x + threadIdx.x) / group;
   const bool live = token < tokens;
-  const uint64_t n = tokens * top_k;
+  const uint8_t* d_from = d_out.first + token * d_out.stride;
   for (uint32_t j0 = 0; j0 < top_k; j0 += 4) {
     uint32_t place[4];
     float w[4], dot[4];
@@ -569,27 +570,45 @@ __global__ void __launch_bounds__(256)
     }
     if (live) {
       for (uint32_t c = lane; c < chunks; c += group) {
-        P d, row[4];
-        d.raw = *reinterpret_cast<const typename P::Raw*>(d_out + token * d_out_stride +
-                                                          uint64_t(c) * VB);
+        C d[WHOLE ? 1 : 4], row[4];
+        int64_t off[4];
+        if (WHOLE) d[0].raw = __ldg(reinterpret_cast<const uint4*>(d_from + uint64_t(c) * 16));
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          if (place[u] < n) {
-            row[u].raw = *reinterpret_cast<const typename P::Raw*>(rows + place[u] * rows_stride +
-                                                                   uint64_t(c) * VB);
+          if (place[u] >= n) continue;
+          const uint8_t* from = rows.first + place[u] * rows.stride;
+          if (WHOLE) {
+            row[u].raw = __ldg(reinterpret_cast<const uint4*>(from + uint64_t(c) * 16));
+          } else {
+            const uint8_t* to = d_rows + place[u] * d_rows_stride;
+            off[u] = int64_t(c) * 16 - (uint32_t(reinterpret_cast<uintptr_t>(to)) & 15u);
+            row[u].raw = d[u % (WHOLE ? 1 : 4)].raw = make_uint4(0, 0, 0, 0);
+            if (off[u] < int64_t(row_bytes)) {
+              const uint8_t* p = from + off[u];
+              row[u].raw = load_chunk<sizeof(T)>(p, off[u] < 0 ? from : p, from + row_bytes,
+                                                 rows.first, rows.last);
+              p = d_from + off[u];
+              d[u % (WHOLE ? 1 : 4)].raw = load_chunk<sizeof(T)>(
+                  p, off[u] < 0 ? d_from : p, d_from + row_bytes, d_out.first, d_out.last);
+            }
           }
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           if (place[u] >= n) continue;
-          P g;
+          const C& du = d[WHOLE ? 0 : u];
+          uint8_t* to = d_rows + place[u] * d_rows_stride;
+          C g;
 #pragma unroll
-          for (int e = 0; e < P::kElems; ++e) {
-            dot[u] = fmaf(d.get(e), row[u].get(e), dot[u]);
-            g.set(e, w[u] * d.get(e));
+          for (int e = 0; e < C::kElems; ++e) {
+            const int64_t b = WHOLE ? 0 : off[u] + e * int(sizeof(T));
+            if (WHOLE || (b >= 0 && b < int64_t(row_bytes))) {
+              dot[u] = fmaf(du.get(e), row[u].get(e), dot[u]);
+            }
+            g.set(e, w[u] * du.get(e));
           }
-          *reinterpret_cast<typename P::Raw*>(d_rows + place[u] * d_rows_stride + uint64_t(c) * VB) =
-              g.raw;
+          if (WHOLE) *reinterpret_cast<uint4*>(to + uint64_t(c) * 16) = g.raw;
+          else store_chunk<sizeof(T)>(to + off[u], g.raw, to, to + row_bytes);
         }
       }
     }
@@ -598,7 +617,7 @@ __global__ void __launch_bounds__(256)
     for (int u = 0; u < 4; ++u) {
       for (uint32_t d = width >> 1; d > 0; d >>= 1) dot[u] += __shfl_xor_sync(kFull, dot[u], d);
     }
-    if (group > 32u) {   // the whole block is on one token then or on a few: all of it arrives
+    if (group > 32u) {   // uniform over the block: all of it arrives
       __syncthreads();
       const uint32_t warp = threadIdx.x >> 5;
       if ((threadIdx.x & 31u) == 0) {
@@ -631,33 +650,18 @@ uint32_t pow2_at_least(uint64_t v) {
   return p;
 }
 
-// Access width of typed rows: whole elements.
-uint32_t typed_access(uint64_t bits, uint32_t size) {
-  const uint32_t v = access_bytes(bits);
-  return v < size ? 0u : v;   // 0: an address is no multiple of the element
+// Chunks per row: unaligned rows touch up to one more at either end.
+uint32_t chunks_of(uint64_t row_bytes, bool whole) {
+  return uint32_t(whole ? row_bytes / 16 : (row_bytes + 30) / 16);
 }
 
-#define HKV_FOR_TYPED_ACCESS(kind, vb, CALL)                        \
-  if ((kind) == hkv::kValueF32) {                                   \
-    switch (vb) {                                                   \
-      case 16: CALL(float, 16); break;                              \
-      case 8: CALL(float, 8); break;                                \
-      default: CALL(float, 4); break;                               \
-    }                                                               \
-  } else if ((kind) == hkv::kValueF16) {                            \
-    switch (vb) {                                                   \
-      case 16: CALL(__half, 16); break;                             \
-      case 8: CALL(__half, 8); break;                               \
-      case 4: CALL(__half, 4); break;                               \
-      default: CALL(__half, 2); break;                              \
-    }                                                               \
-  } else {                                                          \
-    switch (vb) {                                                   \
-      case 16: CALL(__nv_bfloat16, 16); break;                      \
-      case 8: CALL(__nv_bfloat16, 8); break;                        \
-      case 4: CALL(__nv_bfloat16, 4); break;                        \
-      default: CALL(__nv_bfloat16, 2); break;                       \
-    }                                                               \
+#define HKV_FOR_TYPE(kind, whole, CALL)                         \
+  if ((kind) == hkv::kValueF32) {                               \
+    if (whole) { CALL(float, true); } else { CALL(float, false); } \
+  } else if ((kind) == hkv::kValueF16) {                        \
+    if (whole) { CALL(__half, true); } else { CALL(__half, false); } \
+  } else {                                                      \
+    if (whole) { CALL(__nv_bfloat16, true); } else { CALL(__nv_bfloat16, false); } \
   }
 
 int check_order(uint64_t tokens, uint32_t top_k, uint32_t experts) {
@@ -724,19 +728,26 @@ int hkv_expert_dispatch(uint64_t tokens, uint32_t top_k, uint64_t row_bytes, con
   if (tokens == 0) return HKV_OK;
   HKV_ROWS_CHECK(x != nullptr && position != nullptr && rows != nullptr && offsets != nullptr,
                  "x, offsets, position and rows must not be null");
-  const uint32_t vb =
-      access_bytes(row_bytes | address_bits(x) | x_stride | address_bits(rows) | rows_stride);
-  const uint32_t chunks = uint32_t(row_bytes / vb);
+  const uint64_t bits =
+      row_bytes | address_bits(x) | x_stride | address_bits(rows) | rows_stride;
+  const bool whole = whole_chunks(bits);
+  const uint32_t chunks = chunks_of(row_bytes, whole);
   unsigned grid = 0;
   rc = grid_of(tokens * chunks, kMoveBlock, &grid);
   if (rc != HKV_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (zero_rows_behind) zero_behind(tokens * top_k, row_bytes, offsets + experts, rows, rows_stride, s);
-#define HKV_CALL(VB)                                                                              \
-  dispatch_kernel<VB><<<grid, kMoveBlock, 0, s>>>(tokens, top_k, chunks,                          \
-                                                  static_cast<const uint8_t*>(x), x_stride, position, \
-                                                  static_cast<uint8_t*>(rows), rows_stride)
-  HKV_FOR_ACCESS(vb, HKV_CALL)
+  const RowsIn in = rows_in(x, tokens, x_stride, row_bytes);
+  const int32_t* kept = zero_rows_behind ? offsets + experts : nullptr;
+#define HKV_CALL(G)                                                                              \
+  dispatch_kernel<G><<<grid, kMoveBlock, 0, s>>>(tokens, top_k, chunks, row_bytes, in, position, \
+                                                 static_cast<uint8_t*>(rows), rows_stride, kept)
+  switch (whole ? 0u : piece_bytes(bits)) {
+    case 0: HKV_CALL(0); break;
+    case 8: HKV_CALL(8); break;
+    case 4: HKV_CALL(4); break;
+    case 2: HKV_CALL(2); break;
+    default: HKV_CALL(1); break;
+  }
 #undef HKV_CALL
   return rows_launched();
 }
@@ -756,19 +767,22 @@ int hkv_expert_combine(uint64_t tokens, uint32_t top_k, uint64_t dim, uint32_t v
   if (tokens == 0) return HKV_OK;
   HKV_ROWS_CHECK(rows != nullptr && position != nullptr && out != nullptr,
                  "rows, position and out must not be null");
-  const uint32_t vb = typed_access(
-      dim * size | address_bits(rows) | rows_stride | address_bits(out) | out_stride, size);
-  HKV_ROWS_CHECK(vb != 0, "a row does not start at a multiple of its element size");
-  const uint32_t chunks = uint32_t(dim * size / vb);
+  const uint64_t row_bytes = dim * size;
+  const uint64_t bits =
+      row_bytes | address_bits(rows) | rows_stride | address_bits(out) | out_stride;
+  HKV_ROWS_CHECK(bits % size == 0, "a row does not start at a multiple of its element size");
+  const bool whole = whole_chunks(bits);
+  const uint32_t chunks = chunks_of(row_bytes, whole);
   unsigned grid = 0;
   rc = grid_of(tokens * chunks, kMoveBlock, &grid);
   if (rc != HKV_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-#define HKV_CALL(T, VB)                                                                            \
-  combine_kernel<T, VB><<<grid, kMoveBlock, 0, s>>>(                                               \
-      tokens, top_k, chunks, static_cast<const uint8_t*>(rows), rows_stride, weights,              \
-      weight_kind == kValueF32, position, static_cast<uint8_t*>(out), out_stride)
-  HKV_FOR_TYPED_ACCESS(value_kind, vb, HKV_CALL)
+  const RowsIn in = rows_in(rows, tokens * top_k, rows_stride, row_bytes);
+#define HKV_CALL(T, WHOLE)                                                                \
+  combine_kernel<T, WHOLE><<<grid, kMoveBlock, 0, s>>>(                                   \
+      tokens, top_k, chunks, row_bytes, in, weights, weight_kind == kValueF32, position,  \
+      static_cast<uint8_t*>(out), out_stride)
+  HKV_FOR_TYPE(value_kind, whole, HKV_CALL)
 #undef HKV_CALL
   return rows_launched();
 }
@@ -791,25 +805,26 @@ int hkv_expert_combine_backward(uint64_t tokens, uint32_t top_k, uint64_t dim, u
   HKV_ROWS_CHECK(d_out != nullptr && rows != nullptr && weights != nullptr && offsets != nullptr &&
                      position != nullptr && d_rows != nullptr && d_weights != nullptr,
                  "no argument may be null");
-  const uint32_t vb = typed_access(dim * size | address_bits(d_out) | d_out_stride |
-                                       address_bits(rows) | rows_stride | address_bits(d_rows) |
-                                       d_rows_stride,
-                                   size);
-  HKV_ROWS_CHECK(vb != 0, "a row does not start at a multiple of its element size");
-  const uint32_t chunks = uint32_t(dim * size / vb);
+  const uint64_t row_bytes = dim * size;
+  const uint64_t bits = row_bytes | address_bits(d_out) | d_out_stride | address_bits(rows) |
+                        rows_stride | address_bits(d_rows) | d_rows_stride;
+  HKV_ROWS_CHECK(bits % size == 0, "a row does not start at a multiple of its element size");
+  const bool whole = whole_chunks(bits);
+  const uint32_t chunks = chunks_of(row_bytes, whole);
   uint32_t group = pow2_at_least(chunks);
   group = group > 256u ? 256u : group;
   unsigned grid = 0;
   rc = grid_of(tokens * group, 256, &grid);
   if (rc != HKV_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (zero_rows_behind) zero_behind(tokens * top_k, dim * size, offsets + experts, d_rows, d_rows_stride, s);
-#define HKV_CALL(T, VB)                                                                            \
-  combine_backward_kernel<T, VB><<<grid, 256, 0, s>>>(                                             \
-      tokens, top_k, chunks, group, static_cast<const uint8_t*>(d_out), d_out_stride,              \
-      static_cast<const uint8_t*>(rows), rows_stride, weights, weight_kind == kValueF32, position, \
-      static_cast<uint8_t*>(d_rows), d_rows_stride, d_weights)
-  HKV_FOR_TYPED_ACCESS(value_kind, vb, HKV_CALL)
+  const RowsIn d_in = rows_in(d_out, tokens, d_out_stride, row_bytes);
+  const RowsIn in = rows_in(rows, tokens * top_k, rows_stride, row_bytes);
+  const int32_t* kept = zero_rows_behind ? offsets + experts : nullptr;
+#define HKV_CALL(T, WHOLE)                                                                       \
+  combine_backward_kernel<T, WHOLE><<<grid, 256, 0, s>>>(                                        \
+      tokens, top_k, chunks, group, row_bytes, d_in, in, weights, weight_kind == kValueF32,      \
+      position, static_cast<uint8_t*>(d_rows), d_rows_stride, d_weights, kept)
+  HKV_FOR_TYPE(value_kind, whole, HKV_CALL)
 #undef HKV_CALL
   return rows_launched();
 }

@@ -28,101 +28,227 @@ namespace hkv {
 namespace {
 
 constexpr uint32_t kFull = 0xFFFFFFFFu;
-constexpr int kNormBlock = 256;
+constexpr int kNormBlock = 256;       // forward; more where a row needs more
+constexpr int kBackwardBlock = 512;
 
 // Sum over the `group` threads of a row (a power of two: part of a warp, or
-// whole warps of this block); every thread gets it.  `scratch`: one float per
-// warp of the block.  With groups above a warp every thread of the block calls.
+// whole warps of this block); every thread gets it.  scratch: two floats of each
+// value per warp, used in turn, so that one barrier of the group's own (named
+// 1 + its number in the block) is enough.
 template <int N>
-__device__ __forceinline__ void group_sum(float (&v)[N], uint32_t group, float (*scratch)[N]) {
-  const uint32_t width = group < 32u ? group : 32u;
-  for (uint32_t d = width >> 1; d > 0; d >>= 1) {
+struct GroupSum {
+  uint32_t group, warp, first_warp, barrier;
+  float (*scratch)[2][N];   // [warps of the block]
+  uint32_t turn = 0;
+
+  __device__ __forceinline__ GroupSum(uint32_t group_, float (*scratch_)[2][N])
+      : group(group_),
+        warp(threadIdx.x >> 5),
+        first_warp((threadIdx.x >> 5) & ~((group_ >> 5) - (group_ >> 5 ? 1u : 0u))),
+        barrier(1u + threadIdx.x / group_),
+        scratch(scratch_) {}
+
+  __device__ __forceinline__ void operator()(float (&v)[N]) {
+    const uint32_t width = group < 32u ? group : 32u;
+    for (uint32_t d = width >> 1; d > 0; d >>= 1) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(kFull, v[i], d);
-  }
-  if (group > 32u) {
-    const uint32_t warp = threadIdx.x >> 5;
-    __syncthreads();   // the previous sum has been read
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(kFull, v[i], d);
+    }
+    if (group <= 32u) return;
     if ((threadIdx.x & 31u) == 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) scratch[warp][i] = v[i];
+      for (int i = 0; i < N; ++i) scratch[warp][turn][i] = v[i];
     }
-    __syncthreads();
-    const uint32_t first = warp & ~((group >> 5) - 1u);
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(group) : "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = 0.f;
-    for (uint32_t w = 0; w < group >> 5; ++w) {
+    for (uint32_t w = first_warp; w < first_warp + (group >> 5); ++w) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] += scratch[first + w][i];
+      for (int i = 0; i < N; ++i) v[i] += scratch[w][turn][i];
+    }
+    turn ^= 1u;
+  }
+};
+
+// Where a thread's chunks lie in its row: chunk c of the thread is
+// first + c * width.  A warp of a group above 32 owns consecutive chunks, so that
+// neighbouring chunks are in neighbouring lanes whatever the group.
+struct ChunkMap {
+  uint32_t first, width, lane;   // lane: within the width
+
+  __device__ __forceinline__ ChunkMap(uint32_t group, int per_thread) {
+    width = group < 32u ? group : 32u;
+    lane = threadIdx.x & (width - 1u);
+    const uint32_t warp_in_group = (threadIdx.x & (group - 1u)) >> 5;
+    first = warp_in_group * 32u * uint32_t(per_thread) + lane;
+  }
+  __device__ __forceinline__ uint32_t operator()(int c) const { return first + uint32_t(c) * width; }
+};
+
+// The thread's chunks of a row; what is behind the row's end is zero.
+template <typename T, int CHUNKS, bool WHOLE>
+__device__ __forceinline__ void load_row(const uint8_t* row, uint64_t row_bytes, uint32_t chunks,
+                                         const ChunkMap& map, const uint8_t* first,
+                                         const uint8_t* last, Chunk<T> (&x)[CHUNKS]) {
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const uint32_t at = map(c);
+    x[c].raw = make_uint4(0, 0, 0, 0);
+    if (row == nullptr || at >= chunks) continue;
+    const uint8_t* p = row + uint64_t(at) * 16;
+    if (WHOLE) {
+      x[c].raw = __ldg(reinterpret_cast<const uint4*>(p));
+    } else {
+      x[c].raw = load_chunk<sizeof(T)>(p, p, row + row_bytes, first, last);
+      if (p + 16 > row + row_bytes) {
+        const int have = int(row + row_bytes - p) / int(sizeof(T));
+#pragma unroll
+        for (int e = 0; e < Chunk<T>::kElems; ++e) {
+          if (e >= have) x[c].set(e, 0.f);
+        }
+      }
     }
   }
 }
 
-// CHUNKS accesses of VB bytes per thread; `group` threads per row.
-template <typename T, int VB, int CHUNKS>
-__global__ void __launch_bounds__(1024)
-    norm_kernel(const NormArgs a, const uint32_t group, const uint32_t chunks) {
-  using P = Pack<T, VB>;
-  __shared__ float scratch[32][1];
-  const uint32_t lane = threadIdx.x & (group - 1u);
-  const uint64_t r = (uint64_t(blockIdx.x) * blockDim.x + threadIdx.x) / group;
-  const uint8_t* row = nullptr;
-  if (r < a.n) {
-    row = a.row_ptrs != nullptr ? static_cast<const uint8_t*>(a.row_ptrs[r])
-                                : static_cast<const uint8_t*>(a.x) + r * a.x_stride;
+// Stores the thread's chunks of a row.  At an unaligned address every aligned 16
+// bytes belong to two neighbouring chunks: a lane gets its left neighbour's and
+// stores the joint; only the ends of the row, and of a warp's run of it, are
+// stored element by element.  The whole warp calls; row == nullptr: nothing.
+template <typename T, int CHUNKS, bool WHOLE>
+__device__ __forceinline__ void store_row(uint8_t* row, uint64_t row_bytes, uint32_t chunks,
+                                          const ChunkMap& map, const Chunk<T> (&y)[CHUNKS]) {
+  if (WHOLE) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const uint32_t at = map(c);
+      if (row != nullptr && at < chunks) *reinterpret_cast<uint4*>(row + uint64_t(at) * 16) = y[c].raw;
+    }
+    return;
   }
-  P x[CHUNKS];
+  const uint32_t s = uint32_t(reinterpret_cast<uintptr_t>(row)) & 15u;
+  const uint8_t* end = row + row_bytes;
+  const uint32_t left = (threadIdx.x & 31u & ~(map.width - 1u)) | ((map.lane - 1u) & (map.width - 1u));
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-    const uint32_t at = lane + c * group;
-    if (row != nullptr && at < chunks) {
-      x[c].raw = *reinterpret_cast<const typename P::Raw*>(row + uint64_t(at) * VB);
-    } else {
-      x[c].raw = typename P::Raw{};
+    const uint32_t at = map(c);
+    const bool to_next = map.lane == map.width - 1u;   // its right neighbour is in the next round
+    const uint4 mine = y[c].raw;
+    const uint4 give = to_next && c > 0 ? y[c > 0 ? c - 1 : 0].raw : mine;
+    uint4 prev;
+    prev.x = __shfl_sync(kFull, give.x, left);
+    prev.y = __shfl_sync(kFull, give.y, left);
+    prev.z = __shfl_sync(kFull, give.z, left);
+    prev.w = __shfl_sync(kFull, give.w, left);
+    if (row == nullptr || at > chunks) continue;
+    uint8_t* q = row + uint64_t(at) * 16;
+    const bool joined = map.lane != 0 || c > 0;        // the left neighbour's bytes are here
+    if (s == 0) {
+      store_chunk<sizeof(T)>(q, mine, row, end);
+      continue;
+    }
+    store_chunk<sizeof(T)>(q - s, shifted(prev, mine, 16u - s), joined ? row : q, end);
+    if (c == CHUNKS - 1 && to_next) {
+      // the end of the warp's run: nobody joins this chunk's last bytes
+      const uint4 none = make_uint4(0, 0, 0, 0);
+      const uint8_t* stop = q + 16 < end ? q + 16 : end;
+      store_chunk<sizeof(T)>(q - s + 16, shifted(mine, none, 16u - s), row, stop);
     }
   }
+}
+
+// weight or bias of a chunk's columns; 1 or 0 where there is none or no column.
+template <typename T, bool WHOLE, int N>
+__device__ __forceinline__ void load_params(const void* p, bool f32, uint32_t column, uint32_t dim,
+                                            float none, float (&out)[N]) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = none;
+  } else if (WHOLE) {
+    // whole chunks of columns, and the launcher has checked the address
+    if (f32) {
+      const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + column);
+#pragma unroll
+      for (int e = 0; e < N; e += 4) {
+        const float4 v = __ldg(s + e / 4);
+        out[e] = v.x;
+        out[e + 1] = v.y;
+        out[e + 2] = v.z;
+        out[e + 3] = v.w;
+      }
+    } else {
+      Chunk<T> v;
+      v.raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p) + column));
+#pragma unroll
+      for (int e = 0; e < N; ++e) out[e] = v.get(e);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      out[e] = none;
+      if (column + e < dim) {
+        out[e] = f32 ? static_cast<const float*>(p)[column + e]
+                     : to_float(static_cast<const T*>(p)[column + e]);
+      }
+    }
+  }
+}
+
+// CHUNKS chunks per thread, `group` threads per row, one row per group.
+template <typename T, int CHUNKS, bool WHOLE>
+__global__ void __launch_bounds__(1024)
+    norm_kernel(const NormArgs a, const uint32_t group, const uint32_t chunks, const RowsIn in) {
+  using C = Chunk<T>;
+  __shared__ float scratch[32][2][1];
+  const uint64_t r = (uint64_t(blockIdx.x) * blockDim.x + threadIdx.x) / group;
+  const ChunkMap map(group, CHUNKS);
+  const uint64_t row_bytes = a.dim * sizeof(T);
+  const uint8_t *row = nullptr, *first = in.first, *last = in.last;
+  if (r < a.n) {
+    if (a.row_ptrs != nullptr) {
+      row = first = static_cast<const uint8_t*>(a.row_ptrs[r]);
+      last = row + row_bytes;
+    } else {
+      row = in.first + r * in.stride;
+    }
+  }
+  C x[CHUNKS];
+  load_row<T, CHUNKS, WHOLE>(row, row_bytes, chunks, map, first, last, x);
+  GroupSum<1> group_sum(group, scratch);
   const float inv_dim = a.inv_dim;
   float sum[1] = {0.f};
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
 #pragma unroll
-    for (int e = 0; e < P::kElems; ++e) sum[0] += x[c].get(e);
+    for (int e = 0; e < C::kElems; ++e) sum[0] += x[c].get(e);
   }
-  group_sum<1>(sum, group, scratch);
+  group_sum(sum);
   const float mean = sum[0] * inv_dim;
   float sq[1] = {0.f};
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-    if (lane + c * group < chunks) {
+    const uint32_t column = map(c) * C::kElems;
 #pragma unroll
-      for (int e = 0; e < P::kElems; ++e) {
-        const float d = x[c].get(e) - mean;
-        sq[0] = fmaf(d, d, sq[0]);
-      }
+    for (int e = 0; e < C::kElems; ++e) {
+      const float d = x[c].get(e) - mean;
+      if (column + (WHOLE ? 0 : e) < a.dim) sq[0] = fmaf(d, d, sq[0]);
     }
   }
-  group_sum<1>(sq, group, scratch);
-  if (row == nullptr) return;
+  group_sum(sq);
   const float rstd = 1.f / sqrtf(fmaf(sq[0], inv_dim, a.eps));
-  uint8_t* out = static_cast<uint8_t*>(a.y) + r * a.y_stride;
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-    const uint32_t at = lane + c * group;
-    if (at >= chunks) break;
-    float w[P::kElems], b[P::kElems];
+    if (map(c) >= chunks) break;
+    float w[C::kElems], b[C::kElems];
+    const uint32_t column = map(c) * C::kElems;
+    load_params<T, WHOLE>(a.weight, a.params_f32, column, uint32_t(a.dim), 1.f, w);
+    load_params<T, WHOLE>(a.bias, a.params_f32, column, uint32_t(a.dim), 0.f, b);
 #pragma unroll
-    for (int e = 0; e < P::kElems; ++e) {
-      w[e] = 1.f;
-      b[e] = 0.f;
-    }
-    if (a.weight != nullptr) load_params<T>(a.weight, a.params_f32, at * P::kElems, w);
-    if (a.bias != nullptr) load_params<T>(a.bias, a.params_f32, at * P::kElems, b);
-    P y;
-#pragma unroll
-    for (int e = 0; e < P::kElems; ++e) y.set(e, fmaf((x[c].get(e) - mean) * rstd, w[e], b[e]));
-    *reinterpret_cast<typename P::Raw*>(out + uint64_t(at) * VB) = y.raw;
+    for (int e = 0; e < C::kElems; ++e) x[c].set(e, fmaf((x[c].get(e) - mean) * rstd, w[e], b[e]));
   }
-  if (lane == 0) {
+  uint8_t* to = row == nullptr ? nullptr : static_cast<uint8_t*>(a.y) + r * a.y_stride;
+  store_row<T, CHUNKS, WHOLE>(to, row_bytes, chunks, map, x);
+  if (row != nullptr && (threadIdx.x & (group - 1u)) == 0) {
     if (a.mean != nullptr) a.mean[r] = mean;
     if (a.rstd != nullptr) a.rstd[r] = rstd;
   }
@@ -130,51 +256,34 @@ __global__ void __launch_bounds__(1024)
 
 // Rows too long for the registers of a block: three passes over the row, which
 // stays in L2 between them.
-template <typename T, int VB>
+template <typename T>
 __global__ void __launch_bounds__(1024)
-    norm_long_kernel(const NormArgs a, const uint32_t chunks) {
-  using P = Pack<T, VB>;
-  __shared__ float scratch[32][1];
+    norm_long_kernel(const NormArgs a) {
+  __shared__ float scratch[32][2][1];
+  GroupSum<1> group_sum(blockDim.x, scratch);
+  const uint32_t dim = uint32_t(a.dim);
   for (uint64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
-    const uint8_t* row = a.row_ptrs != nullptr ? static_cast<const uint8_t*>(a.row_ptrs[r])
-                                               : static_cast<const uint8_t*>(a.x) + r * a.x_stride;
+    const T* row = a.row_ptrs != nullptr
+                       ? static_cast<const T*>(a.row_ptrs[r])
+                       : reinterpret_cast<const T*>(static_cast<const uint8_t*>(a.x) + r * a.x_stride);
     if (row == nullptr) continue;
     float sum[1] = {0.f};
-    for (uint32_t at = threadIdx.x; at < chunks; at += blockDim.x) {
-      P x;
-      x.raw = *reinterpret_cast<const typename P::Raw*>(row + uint64_t(at) * VB);
-#pragma unroll
-      for (int e = 0; e < P::kElems; ++e) sum[0] += x.get(e);
-    }
-    group_sum<1>(sum, blockDim.x, scratch);
+    for (uint32_t i = threadIdx.x; i < dim; i += blockDim.x) sum[0] += to_float(row[i]);
+    group_sum(sum);
     const float mean = sum[0] * a.inv_dim;
     float sq[1] = {0.f};
-    for (uint32_t at = threadIdx.x; at < chunks; at += blockDim.x) {
-      P x;
-      x.raw = *reinterpret_cast<const typename P::Raw*>(row + uint64_t(at) * VB);
-#pragma unroll
-      for (int e = 0; e < P::kElems; ++e) {
-        const float d = x.get(e) - mean;
-        sq[0] = fmaf(d, d, sq[0]);
-      }
+    for (uint32_t i = threadIdx.x; i < dim; i += blockDim.x) {
+      const float d = to_float(row[i]) - mean;
+      sq[0] = fmaf(d, d, sq[0]);
     }
-    group_sum<1>(sq, blockDim.x, scratch);
+    group_sum(sq);
     const float rstd = 1.f / sqrtf(fmaf(sq[0], a.inv_dim, a.eps));
-    uint8_t* out = static_cast<uint8_t*>(a.y) + r * a.y_stride;
-    for (uint32_t at = threadIdx.x; at < chunks; at += blockDim.x) {
-      P x, y;
-      x.raw = *reinterpret_cast<const typename P::Raw*>(row + uint64_t(at) * VB);
-      float w[P::kElems], b[P::kElems];
-#pragma unroll
-      for (int e = 0; e < P::kElems; ++e) {
-        w[e] = 1.f;
-        b[e] = 0.f;
-      }
-      if (a.weight != nullptr) load_params<T>(a.weight, a.params_f32, at * P::kElems, w);
-      if (a.bias != nullptr) load_params<T>(a.bias, a.params_f32, at * P::kElems, b);
-#pragma unroll
-      for (int e = 0; e < P::kElems; ++e) y.set(e, fmaf((x.get(e) - mean) * rstd, w[e], b[e]));
-      *reinterpret_cast<typename P::Raw*>(out + uint64_t(at) * VB) = y.raw;
+    T* out = reinterpret_cast<T*>(static_cast<uint8_t*>(a.y) + r * a.y_stride);
+    for (uint32_t i = threadIdx.x; i < dim; i += blockDim.x) {
+      float w[1], b[1];
+      load_params<T, false>(a.weight, a.params_f32, i, dim, 1.f, w);
+      load_params<T, false>(a.bias, a.params_f32, i, dim, 0.f, b);
+      out[i] = from_float<T>(fmaf((to_float(row[i]) - mean) * rstd, w[0], b[0]));
     }
     if (threadIdx.x == 0) {
       if (a.mean != nullptr) a.mean[r] = mean;
@@ -188,6 +297,7 @@ __global__ void __launch_bounds__(1024)
 // The blocks stay on the device and take rows in turn: a thread sees the same
 // columns of every row it touches, so the column sums d_weight and d_bias build
 // up in its registers beside the row's own work, and x and dy are read once.
+// The next row's chunks are on their way while the current row is reduced.
 // At the end each block writes one row of column sums (its groups added in a
 // fixed order), and norm_reduce_kernel adds the blocks' rows in a fixed order.
 
@@ -196,110 +306,109 @@ struct NormBackwardPlan {
   bool fits;   // a row fits the registers of a block
 };
 
-template <typename T, int VB, int CHUNKS>
-__global__ void __launch_bounds__(kNormBlock)
+template <typename T, int CHUNKS, bool WHOLE>
+__global__ void __launch_bounds__(kBackwardBlock, 1)
     norm_backward_kernel(const NormBackwardArgs a, const uint32_t group, const uint32_t chunks,
-                         float* __restrict__ sums) {
-  using P = Pack<T, VB>;
-  extern __shared__ float columns[];   // [dim]
-  __shared__ float scratch[kNormBlock / 32][2];
-  const uint32_t lane = threadIdx.x & (group - 1u);
-  const uint32_t groups = kNormBlock / group;
-  const uint32_t my_group = threadIdx.x / group;
-  float dw[CHUNKS][P::kElems], db[CHUNKS][P::kElems];
+                         const RowsIn x_in, const RowsIn dy_in, float* __restrict__ sums) {
+  using C = Chunk<T>;
+  constexpr int kElems = C::kElems;
+  extern __shared__ float columns[];   // [copies][dim]: the column sums of each warp or group
+  __shared__ float scratch[kBackwardBlock / 32][2][2];
+  GroupSum<2> group_sum(group, scratch);
+  const ChunkMap map(group, CHUNKS);
+  const uint32_t dim = uint32_t(a.dim);
+  const uint64_t row_bytes = a.dim * sizeof(T);
+  const uint32_t groups = kBackwardBlock / group;
+  float w[CHUNKS][kElems], dw[CHUNKS][kElems], db[CHUNKS][kElems];
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
 #pragma unroll
-    for (int e = 0; e < P::kElems; ++e) dw[c][e] = db[c][e] = 0.f;
+    for (int e = 0; e < kElems; ++e) dw[c][e] = db[c][e] = w[c][e] = 0.f;
+    if (map(c) < chunks) {
+      load_params<T, WHOLE>(a.weight, a.params_f32, map(c) * kElems, dim, 1.f, w[c]);
+    }
   }
-  // every group of the block runs the same number of turns (the sums of groups
-  // above a warp use block barriers)
-  for (uint64_t first = uint64_t(blockIdx.x) * groups; first < a.n;
-       first += uint64_t(gridDim.x) * groups) {
-    const uint64_t r = first + my_group;
-    const bool live = r < a.n;
-    P x[CHUNKS], dy[CHUNKS];
-    float mean = 0.f, rstd = 0.f;
-    if (live) {
-      mean = a.mean[r];
-      rstd = a.rstd[r];
-    }
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-      const uint32_t at = lane + c * group;
-      x[c].raw = dy[c].raw = typename P::Raw{};
-      if (live && at < chunks) {
-        x[c].raw = *reinterpret_cast<const typename P::Raw*>(static_cast<const uint8_t*>(a.x) +
-                                                             r * a.x_stride + uint64_t(at) * VB);
-        dy[c].raw = *reinterpret_cast<const typename P::Raw*>(static_cast<const uint8_t*>(a.dy) +
-                                                              r * a.dy_stride + uint64_t(at) * VB);
-      }
-    }
+  const uint64_t step = uint64_t(gridDim.x) * groups;
+  uint64_t r = uint64_t(blockIdx.x) * groups + threadIdx.x / group;
+  C x[CHUNKS], dy[CHUNKS];
+  float mean = 0.f, rstd = 0.f;
+  auto fetch = [&](uint64_t row) {
+    const bool live = row < a.n;
+    mean = live ? __ldg(a.mean + row) : 0.f;
+    rstd = live ? __ldg(a.rstd + row) : 0.f;
+    load_row<T, CHUNKS, WHOLE>(live ? x_in.first + row * x_in.stride : nullptr, row_bytes, chunks, map,
+                               x_in.first, x_in.last, x);
+    load_row<T, CHUNKS, WHOLE>(live ? dy_in.first + row * dy_in.stride : nullptr, row_bytes, chunks,
+                               map, dy_in.first, dy_in.last, dy);
+  };
+  fetch(r);
+  // the lanes of a warp leave together: their rows are done when the warp's first is
+  for (uint64_t warp_row = r - (threadIdx.x & 31u) / group; warp_row < a.n;
+       warp_row += step, r += step) {
+    float xhat[CHUNKS][kElems], g[CHUNKS][kElems];
     float sum[2] = {0.f, 0.f};
+    const float row_rstd = rstd;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      const uint32_t at = lane + c * group;
-      if (!live || at >= chunks) continue;
-      float w[P::kElems];
 #pragma unroll
-      for (int e = 0; e < P::kElems; ++e) w[e] = 1.f;
-      if (a.weight != nullptr) load_params<T>(a.weight, a.params_f32, at * P::kElems, w);
-#pragma unroll
-      for (int e = 0; e < P::kElems; ++e) {
-        const float xhat = (x[c].get(e) - mean) * rstd;
+      for (int e = 0; e < kElems; ++e) {
         const float d = dy[c].get(e);
-        const float g = d * w[e];
-        sum[0] += g;
-        sum[1] = fmaf(g, xhat, sum[1]);
-        dw[c][e] = fmaf(d, xhat, dw[c][e]);
+        xhat[c][e] = (x[c].get(e) - mean) * rstd;
+        g[c][e] = d * w[c][e];
+        sum[0] += g[c][e];
+        sum[1] = fmaf(g[c][e], xhat[c][e], sum[1]);
+        dw[c][e] = fmaf(d, xhat[c][e], dw[c][e]);
         db[c][e] += d;
       }
     }
-    group_sum<2>(sum, group, scratch);
-    if (!live) continue;
+    fetch(r + step);
+    group_sum(sum);
     const float m0 = sum[0] * a.inv_dim, m1 = sum[1] * a.inv_dim;
+    C dx[CHUNKS];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      const uint32_t at = lane + c * group;
-      if (at >= chunks) break;
-      float w[P::kElems];
 #pragma unroll
-      for (int e = 0; e < P::kElems; ++e) w[e] = 1.f;
-      if (a.weight != nullptr) load_params<T>(a.weight, a.params_f32, at * P::kElems, w);
-      P dx;
-#pragma unroll
-      for (int e = 0; e < P::kElems; ++e) {
-        const float xhat = (x[c].get(e) - mean) * rstd;
-        dx.set(e, rstd * (dy[c].get(e) * w[e] - m0 - xhat * m1));
+      for (int e = 0; e < kElems; ++e) {
+        dx[c].set(e, row_rstd * (fmaf(-m1, xhat[c][e], g[c][e]) - m0));
       }
-      *reinterpret_cast<typename P::Raw*>(static_cast<uint8_t*>(a.dx) + r * a.dx_stride +
-                                          uint64_t(at) * VB) = dx.raw;
+    }
+    store_row<T, CHUNKS, WHOLE>(
+        r < a.n ? static_cast<uint8_t*>(a.dx) + r * a.dx_stride : nullptr, row_bytes, chunks, map, dx);
+  }
+  // the sums of the block's groups: those of one warp by exchange, the others
+  // one after the other
+  const uint32_t copies = group < 32u ? kBackwardBlock / 32 : groups;
+  const uint32_t copy = group < 32u ? threadIdx.x >> 5 : threadIdx.x / group;
+  for (uint32_t d = 16; d >= group; d >>= 1) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        dw[c][e] += __shfl_xor_sync(kFull, dw[c][e], d);
+        db[c][e] += __shfl_xor_sync(kFull, db[c][e], d);
+      }
     }
   }
-  // the block's groups, one after the other
-  const uint32_t dim = a.dim;
+  const bool writes = group >= 32u || (threadIdx.x & 31u) < group;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     if (which == 0 ? a.d_weight == nullptr : a.d_bias == nullptr) continue;
-    for (uint32_t turn = 0; turn < groups; ++turn) {
-      if (turn == my_group) {
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-          const uint32_t at = lane + c * group;
-          if (at >= chunks) break;
-#pragma unroll
-          for (int e = 0; e < P::kElems; ++e) {
-            const float v = which == 0 ? dw[c][e] : db[c][e];
-            float* to = columns + at * P::kElems + e;
-            *to = turn == 0 ? v : *to + v;
-          }
-        }
-      }
-      __syncthreads();
-    }
-    float* mine = sums + (uint64_t(which) * gridDim.x + blockIdx.x) * dim;
-    for (uint32_t i = threadIdx.x; i < dim; i += kNormBlock) mine[i] = columns[i];
     __syncthreads();
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        const uint32_t column = map(c) * kElems + e;
+        if (writes && column < dim) columns[copy * dim + column] = which == 0 ? dw[c][e] : db[c][e];
+      }
+    }
+    __syncthreads();
+    float* mine = sums + (uint64_t(which) * gridDim.x + blockIdx.x) * dim;
+    for (uint32_t i = threadIdx.x; i < dim; i += kBackwardBlock) {
+      float v = columns[i];
+      for (uint32_t k = 1; k < copies; ++k) v += columns[k * dim + i];
+      mine[i] = v;
+    }
   }
 }
 
@@ -308,27 +417,29 @@ __global__ void __launch_bounds__(kNormBlock)
 template <typename T>
 __global__ void __launch_bounds__(512)
     norm_backward_long_kernel(const NormBackwardArgs a) {
-  __shared__ float scratch[16][2];
+  __shared__ float scratch[16][2][2];
+  GroupSum<2> group_sum(blockDim.x, scratch);
+  const uint32_t dim = uint32_t(a.dim);
   for (uint64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
     const T* x = reinterpret_cast<const T*>(static_cast<const uint8_t*>(a.x) + r * a.x_stride);
     const T* dy = reinterpret_cast<const T*>(static_cast<const uint8_t*>(a.dy) + r * a.dy_stride);
     T* dx = reinterpret_cast<T*>(static_cast<uint8_t*>(a.dx) + r * a.dx_stride);
     const float mean = a.mean[r], rstd = a.rstd[r];
     float sum[2] = {0.f, 0.f};
-    for (uint32_t i = threadIdx.x; i < a.dim; i += blockDim.x) {
-      float w[1] = {1.f};
-      if (a.weight != nullptr) load_params<T>(a.weight, a.params_f32, i, w);
+    for (uint32_t i = threadIdx.x; i < dim; i += blockDim.x) {
+      float w[1];
+      load_params<T, false>(a.weight, a.params_f32, i, dim, 1.f, w);
       const float g = to_float(dy[i]) * w[0];
       sum[0] += g;
       sum[1] = fmaf(g, (to_float(x[i]) - mean) * rstd, sum[1]);
     }
-    group_sum<2>(sum, blockDim.x, scratch);
+    group_sum(sum);
     const float m0 = sum[0] * a.inv_dim, m1 = sum[1] * a.inv_dim;
-    for (uint32_t i = threadIdx.x; i < a.dim; i += blockDim.x) {
-      float w[1] = {1.f};
-      if (a.weight != nullptr) load_params<T>(a.weight, a.params_f32, i, w);
+    for (uint32_t i = threadIdx.x; i < dim; i += blockDim.x) {
+      float w[1];
+      load_params<T, false>(a.weight, a.params_f32, i, dim, 1.f, w);
       const float xhat = (to_float(x[i]) - mean) * rstd;
-      dx[i] = from_float<T>(rstd * (to_float(dy[i]) * w[0] - m0 - xhat * m1));
+      dx[i] = from_float<T>(rstd * (fmaf(-m1, xhat, to_float(dy[i]) * w[0]) - m0));
     }
   }
 }
@@ -339,6 +450,7 @@ __global__ void __launch_bounds__(kNormBlock)
   const uint64_t i = uint64_t(blockIdx.x) * kNormBlock + threadIdx.x;
   if (i >= a.dim) return;
   float dw = 0.f, db = 0.f;
+#pragma unroll 4
   for (uint64_t r = blockIdx.y; r < a.n; r += gridDim.y) {
     const float d = to_float(
         reinterpret_cast<const T*>(static_cast<const uint8_t*>(a.dy) + r * a.dy_stride)[i]);
@@ -389,100 +501,77 @@ uint32_t pow2_at_least(uint64_t v) {
   return p;
 }
 
-#define HKV_FOR_NORM_TYPE(kind, vb, CALL)    \
-  if ((kind) == kValueF32) {                 \
-    switch (vb) {                            \
-      case 16: CALL(float, 16); break;       \
-      default: CALL(float, 4); break;        \
-    }                                        \
-  } else if ((kind) == kValueF16) {          \
-    switch (vb) {                            \
-      case 16: CALL(__half, 16); break;      \
-      case 4: CALL(__half, 4); break;        \
-      default: CALL(__half, 2); break;       \
-    }                                        \
-  } else {                                   \
-    switch (vb) {                            \
-      case 16: CALL(__nv_bfloat16, 16); break; \
-      case 4: CALL(__nv_bfloat16, 4); break; \
-      default: CALL(__nv_bfloat16, 2); break; \
-    }                                        \
-  }
+// Chunks of a row; the last one may be part of one.
+uint64_t chunks_of(uint64_t row_bytes) { return (row_bytes + 15) / 16; }
 
-// 16 bytes, 4, or one element; 0 when an address is no multiple of the element.
-uint32_t norm_access(uint64_t bits, uint32_t size) {
-  const uint32_t v = access_bytes(bits);
-  if (v < size) return 0;
-  return v == 16 ? 16 : v >= 4 ? 4 : size;
+// Parameters are read in chunks where the rows are: their addresses count too.
+uint64_t param_bits(const void* weight, const void* bias) {
+  return address_bits(weight) | address_bits(bias);
 }
 
-constexpr uint32_t kMaxChunks = 8;   // accesses a thread of norm_kernel holds
+constexpr uint32_t kMaxGroup = 1024;
 
-template <typename T, int VB>
-void launch_norm_vb(const NormArgs& a, cudaStream_t stream) {
-  const uint64_t chunks = a.dim * sizeof(T) / VB;
-  if (chunks > 1024ull * kMaxChunks) {
+template <typename T>
+void launch_norm_type(const NormArgs& a, bool whole, cudaStream_t stream) {
+  const uint64_t chunks = chunks_of(a.dim * sizeof(T));
+  if (chunks > 4ull * kMaxGroup) {
     const uint64_t cap = uint64_t(sm_count()) * 2;
-    norm_long_kernel<T, VB><<<unsigned(a.n < cap ? a.n : cap), 1024, 0, stream>>>(a, uint32_t(chunks));
+    norm_long_kernel<T><<<unsigned(a.n < cap ? a.n : cap), kMaxGroup, 0, stream>>>(a);
     return;
   }
-  // four accesses per thread where the row has them, with at least two threads
-  // on a row
-  uint32_t group = pow2_at_least((chunks + 3) / 4);
-  if (group < 2 && chunks > 1) group = 2;
-  uint32_t per_thread = uint32_t((chunks + group - 1) / group);
-  if (group > 1024) {
-    group = 1024;
-    per_thread = uint32_t((chunks + 1023) / 1024);
+  // four chunks per thread where the row has them, fewer where there are too
+  // few rows to fill the device with that
+  const uint64_t enough = uint64_t(sm_count()) * 512;
+  uint32_t per_thread = 4, group = pow2_at_least((chunks + 3) / 4);
+  while (per_thread > 1 && group < kMaxGroup &&
+         (a.n * group < enough || pow2_at_least(chunks) <= 2)) {
+    per_thread >>= 1;
+    group = pow2_at_least((chunks + per_thread - 1) / per_thread);
   }
   const uint32_t block = group > kNormBlock ? group : kNormBlock;
   const uint64_t grid = (a.n * group + block - 1) / block;
-  auto kernel = per_thread <= 1   ? norm_kernel<T, VB, 1>
-                : per_thread <= 2 ? norm_kernel<T, VB, 2>
-                : per_thread <= 4 ? norm_kernel<T, VB, 4>
-                                  : norm_kernel<T, VB, 8>;
-  kernel<<<unsigned(grid), block, 0, stream>>>(a, group, uint32_t(chunks));
+  const RowsIn in = a.row_ptrs != nullptr ? RowsIn{} : rows_in(a.x, a.n, a.x_stride, a.dim * sizeof(T));
+  auto kernel = whole ? (per_thread == 1   ? norm_kernel<T, 1, true>
+                         : per_thread == 2 ? norm_kernel<T, 2, true>
+                                           : norm_kernel<T, 4, true>)
+                      : (per_thread == 1   ? norm_kernel<T, 1, false>
+                         : per_thread == 2 ? norm_kernel<T, 2, false>
+                                           : norm_kernel<T, 4, false>);
+  kernel<<<unsigned(grid), block, 0, stream>>>(a, group, uint32_t(chunks), in);
 }
 
-// Accesses a thread of the backward kernel holds: their column sums stay in
-// registers, 16 or 32 elements' worth.
-template <typename T, int VB>
-constexpr int backward_chunks() {
-  return VB == 16 ? 4 : 16;
-}
+// Chunks a thread of the backward kernel holds: 16 elements' column sums, row
+// values and weights fill the registers that 512 threads have.
+constexpr uint32_t backward_chunks(uint32_t size) { return size == 4 ? 4 : 2; }
 
-NormBackwardPlan plan_backward(uint64_t n, uint64_t dim, uint32_t size, uint32_t vb) {
+NormBackwardPlan plan_backward(uint64_t n, uint64_t dim, uint32_t size) {
   NormBackwardPlan p{};
-  const uint64_t chunks = dim * size / vb;
-  const uint32_t most = vb == 16 ? 4 : 16;
-  p.fits = chunks <= uint64_t(kNormBlock) * most;
-  const uint64_t sms = uint64_t(sm_count());
+  const uint64_t chunks = chunks_of(dim * size);
+  p.per_thread = backward_chunks(size);
+  p.fits = chunks <= uint64_t(kBackwardBlock) * p.per_thread;
   if (!p.fits) {
     p.blocks = uint32_t(n < 64 ? n : 64);   // row splits of the column sums
     return p;
   }
   p.chunks = uint32_t(chunks);
-  p.per_thread = most;
-  p.group = pow2_at_least((chunks + most - 1) / most);
-  if (p.group < 2 && chunks > 1) p.group = 2;
-  if (vb < 16) {
-    // narrow accesses: a warp reads along the row
-    const uint32_t along = pow2_at_least(chunks);
-    p.group = along > 32 ? (p.group > 32 ? p.group : 32) : along;
-  }
-  const uint64_t groups = kNormBlock / p.group;
+  p.group = pow2_at_least((chunks + p.per_thread - 1) / p.per_thread);
+  const uint64_t groups = kBackwardBlock / p.group;
   const uint64_t want = (n + groups - 1) / groups;
-  const uint64_t cap = sms * 2;
+  const uint64_t cap = uint64_t(sm_count());
   p.blocks = uint32_t(want < cap ? want : cap);
   return p;
 }
 
-template <typename T, int VB>
-void launch_backward_vb(const NormBackwardArgs& a, const NormBackwardPlan& p, float* sums,
-                        cudaStream_t stream) {
-  constexpr int kChunks = backward_chunks<T, VB>();
-  norm_backward_kernel<T, VB, kChunks>
-      <<<p.blocks, kNormBlock, a.dim * sizeof(float), stream>>>(a, p.group, p.chunks, sums);
+template <typename T>
+void launch_backward_type(const NormBackwardArgs& a, const NormBackwardPlan& p, bool whole, float* sums,
+                          cudaStream_t stream) {
+  constexpr int kChunks = backward_chunks(sizeof(T));
+  const uint64_t row_bytes = a.dim * sizeof(T);
+  const uint32_t copies = p.group < 32 ? kBackwardBlock / 32 : kBackwardBlock / p.group;
+  auto kernel = whole ? norm_backward_kernel<T, kChunks, true> : norm_backward_kernel<T, kChunks, false>;
+  kernel<<<p.blocks, kBackwardBlock, copies * a.dim * sizeof(float), stream>>>(
+      a, p.group, p.chunks, rows_in(a.x, a.n, a.x_stride, row_bytes),
+      rows_in(a.dy, a.n, a.dy_stride, row_bytes), sums);
 }
 
 template <typename T>
@@ -490,7 +579,7 @@ void launch_backward_long(const NormBackwardArgs& a, const NormBackwardPlan& p, 
                           cudaStream_t stream) {
   const uint64_t cap = uint64_t(sm_count()) * 4;
   norm_backward_long_kernel<T><<<unsigned(a.n < cap ? a.n : cap), 512, 0, stream>>>(a);
-  if (a.d_weight != nullptr || a.d_bias != nullptr) {
+  if (sums != nullptr) {
     const dim3 grid(unsigned((a.dim + kNormBlock - 1) / kNormBlock), p.blocks);
     norm_columns_kernel<T><<<grid, kNormBlock, 0, stream>>>(a, sums);
   }
@@ -522,11 +611,11 @@ int launch_norm(const NormArgs& args, uint32_t value_kind, cudaStream_t stream) 
   // the pointer form's addresses are on the device: table rows start at
   // multiples of the widest access their length allows
   if (args.row_ptrs == nullptr) bits |= address_bits(args.x) | args.x_stride;
-  const uint32_t vb = norm_access(bits, size);
-  HKV_ROWS_CHECK(vb != 0, "a row does not start at a multiple of its element size");
-#define HKV_CALL(T, VB) launch_norm_vb<T, VB>(args, stream)
-  HKV_FOR_NORM_TYPE(value_kind, vb, HKV_CALL)
-#undef HKV_CALL
+  HKV_ROWS_CHECK(bits % size == 0, "a row does not start at a multiple of its element size");
+  const bool whole = whole_chunks(bits | param_bits(args.weight, args.bias));
+  if (value_kind == kValueF32) launch_norm_type<float>(args, whole, stream);
+  else if (value_kind == kValueF16) launch_norm_type<__half>(args, whole, stream);
+  else launch_norm_type<__nv_bfloat16>(args, whole, stream);
   return rows_launched();
 }
 
@@ -587,10 +676,7 @@ int hkv_layer_norm_ptr(uint64_t n, uint64_t dim, uint32_t value_kind, const void
 
 uint64_t hkv_layer_norm_backward_workspace_bytes(uint64_t n, uint64_t dim, uint32_t value_kind) {
   if (check_norm(n, dim, value_kind, value_kind, 0.f) != HKV_OK || n == 0) return 0;
-  // the most blocks any access width runs
-  uint64_t rows = uint64_t(sm_count()) * 2;
-  rows = rows < 64 ? 64 : rows;
-  return 2 * (n < rows ? n : rows) * dim * sizeof(float);
+  return 2ull * plan_backward(n, dim, row_kind_size(value_kind)).blocks * dim * sizeof(float);
 }
 
 int hkv_layer_norm_backward(uint64_t n, uint64_t dim, uint32_t value_kind, const void* dy,
@@ -633,16 +719,16 @@ int hkv_layer_norm_backward(uint64_t n, uint64_t dim, uint32_t value_kind, const
   a.dx_stride = dx_stride;
   a.d_weight = d_weight;
   a.d_bias = d_bias;
-  const uint32_t vb = norm_access(dim * size | address_bits(dy) | dy_stride | address_bits(x) |
-                                      x_stride | address_bits(dx) | dx_stride,
-                                  size);
-  HKV_ROWS_CHECK(vb != 0, "a row does not start at a multiple of its element size");
-  const NormBackwardPlan p = plan_backward(n, dim, size, vb);
-  float* sums = static_cast<float*>(work);
+  const uint64_t bits = dim * size | address_bits(dy) | dy_stride | address_bits(x) | x_stride |
+                        address_bits(dx) | dx_stride;
+  HKV_ROWS_CHECK(bits % size == 0, "a row does not start at a multiple of its element size");
+  const bool whole = whole_chunks(bits | param_bits(weight, nullptr));
+  const NormBackwardPlan p = plan_backward(n, dim, size);
+  float* sums = sums_wanted ? static_cast<float*>(work) : nullptr;
   if (p.fits) {
-#define HKV_CALL(T, VB) launch_backward_vb<T, VB>(a, p, sums, s)
-    HKV_FOR_NORM_TYPE(value_kind, vb, HKV_CALL)
-#undef HKV_CALL
+    if (value_kind == kValueF32) launch_backward_type<float>(a, p, whole, sums, s);
+    else if (value_kind == kValueF16) launch_backward_type<__half>(a, p, whole, sums, s);
+    else launch_backward_type<__nv_bfloat16>(a, p, whole, sums, s);
   } else if (value_kind == kValueF32) {
     launch_backward_long<float>(a, p, sums, s);
   } else if (value_kind == kValueF16) {
