@@ -1282,6 +1282,8 @@ int hkv_find_layer_norm(hkv_table* t, uint64_t n, const uint64_t* keys, const vo
     a.weight = weight;
     a.bias = bias;
     a.params_f32 = param_kind == hkv::kValueF32;
+    a.params_vec =
+        ((reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(bias)) & 15u) == 0;
     a.eps = eps;
     a.inv_dim = 1.f / float(a.dim);
     a.y = values;

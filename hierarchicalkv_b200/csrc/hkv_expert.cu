@@ -59,11 +59,13 @@ constexpr uint32_t kFull = 0xFFFFFFFFu;
 // ---- sort -------------------------------------------------------------------
 //
 // A counting sort.  Warp w of a block owns a contiguous run of assignments and
-// a row of counters in shared memory; __match_any_sync finds the lanes with
-// the same expert, so an assignment's rank among the warp's earlier ones of
-// its expert is the counter plus the equal lanes below it, and no two lanes
-// touch a counter at once.  Scanning the counters over the warps, the blocks
-// and the experts turns ranks into places.
+// a row of counters in shared memory; the lanes that hold the same expert are
+// found with one ballot per bit of the expert's number, so an assignment's rank
+// among the warp's earlier ones of its expert is the counter plus the equal
+// lanes below it, and no two lanes touch a counter at once.  Scanning the
+// counters over the warps, the blocks and the experts turns ranks into places.
+// (__match_any_sync finds the same lanes in one instruction, at a rate that made
+// 131,072 assignments to 128 experts take 39 us on eight blocks.)
 
 constexpr int kSortCounters = 16384;   // 16-bit counters: warps x experts of a block
 
@@ -87,16 +89,25 @@ __device__ __forceinline__ void rank_in_warp(const ID* __restrict__ ids, uint64_
     if (at < n) id = ids[at];
     expert[i] = (id >= 0 && id < ID(experts)) ? uint32_t(id) : experts;
   }
+  uint32_t same[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) same[i] = kFull;
+  for (uint32_t bit = 1; bit <= experts; bit <<= 1) {   // `experts` itself marks the dropped
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const uint32_t set = __ballot_sync(kFull, (expert[i] & bit) != 0);
+      same[i] &= (expert[i] & bit) != 0 ? set : ~set;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const uint32_t same = __match_any_sync(kFull, expert[i]);
-    const uint32_t below = __popc(same & ((1u << lane) - 1u));
+    const uint32_t below = __popc(same[i] & ((1u << lane) - 1u));
     rank[i] = 0;
     if (expert[i] < experts) {
       const uint32_t before = count[expert[i]];
       rank[i] = before + below;
-      __syncwarp(same);
-      if (below == 0) count[expert[i]] = static_cast<uint16_t>(before + __popc(same));
+      __syncwarp(same[i]);
+      if (below == 0) count[expert[i]] = static_cast<uint16_t>(before + __popc(same[i]));
     }
     __syncwarp();
   }
@@ -241,8 +252,10 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// Large batches: count per tile, scan over the tiles, place.
-constexpr int kTileItems = 16;
+// Large batches: count per tile, scan over the tiles, place.  Up to
+// kTilesSummed tiles the placing blocks sum the counts of the tiles before theirs
+// themselves and the scan's launch is saved.
+constexpr uint32_t kTilesSummed = 64;
 
 template <typename ID>
 __global__ void __launch_bounds__(512)
@@ -298,34 +311,52 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-template <typename ID>
+// totals == nullptr: counts are not scanned yet.
+template <typename ID, int ITEMS>
 __global__ void __launch_bounds__(1024)
     sort_place_kernel(const ID* __restrict__ ids, const uint64_t n, const uint32_t experts,
                       const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals,
                       int32_t* __restrict__ offsets, int32_t* __restrict__ position,
                       int32_t* __restrict__ source) {
   __shared__ SortShared s;
+  __shared__ uint32_t before[kMaxExperts];   // the earlier tiles' assignments of each expert
   const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   for (uint32_t c = threadIdx.x; c < warps * experts; c += blockDim.x) s.count[c] = 0;
+  for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) {
+    before[e] = totals != nullptr ? counts[uint64_t(blockIdx.x) * experts + e] : 0u;
+  }
   __syncthreads();
-  uint32_t expert[kTileItems], rank[kTileItems];
-  const uint64_t first = (uint64_t(blockIdx.x) * warps + warp) * (kTileItems * 32);
-  rank_in_warp<ID, kTileItems>(ids, first, n, experts, s.count + warp * experts, lane, expert, rank);
+  uint32_t expert[ITEMS], rank[ITEMS];
+  const uint64_t first = (uint64_t(blockIdx.x) * warps + warp) * (ITEMS * 32);
+  rank_in_warp<ID, ITEMS>(ids, first, n, experts, s.count + warp * experts, lane, expert, rank);
   __syncthreads();
   scan_warps(s, experts);
+  __syncthreads();   // total[] is the block's own now; from here it is every tile's
+  for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) {
+    s.total[e] = totals != nullptr ? totals[e] : 0u;
+  }
   __syncthreads();
+  if (totals == nullptr) {
+    // whole numbers: the order of these additions does not matter
+    for (uint32_t c = threadIdx.x; c < gridDim.x * experts; c += blockDim.x) {
+      const uint32_t tile = c / experts, e = c - tile * experts;
+      const uint32_t v = counts[c];
+      if (v == 0) continue;
+      atomicAdd(&s.total[e], v);
+      if (tile < blockIdx.x) atomicAdd(&before[e], v);
+    }
+    __syncthreads();
+  }
   const uint32_t total =
-      block_scan(experts, [&](uint32_t e) { return totals[e]; }, s.base, s.scan);
+      block_scan(experts, [&](uint32_t e) { return s.total[e]; }, s.base, s.scan);
   if (blockIdx.x == 0) {
     for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) offsets[e] = int32_t(s.base[e]);
     if (threadIdx.x == 0) offsets[experts] = int32_t(total);
     __syncthreads();
   }
-  for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) {
-    s.base[e] += counts[uint64_t(blockIdx.x) * experts + e];
-  }
+  for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) s.base[e] += before[e];
   __syncthreads();
-  write_places<kTileItems>(s, first, n, experts, lane, warp, expert, rank, position, source);
+  write_places<ITEMS>(s, first, n, experts, lane, warp, expert, rank, position, source);
   for (uint64_t p = total + uint64_t(blockIdx.x) * blockDim.x + threadIdx.x; p < n;
        p += uint64_t(gridDim.x) * blockDim.x) {
     source[p] = -1;
@@ -339,56 +370,50 @@ uint32_t sort_block(uint32_t experts) {
 }
 
 struct SortPlan {
-  uint32_t block, items, blocks;   // blocks == 0: the three-launch form
+  uint32_t block, items;
+  uint32_t cluster;   // blocks of the one-launch form; 0: one block per tile, several launches
+  uint32_t tiles;
 };
 
 SortPlan plan_sort(uint64_t n, uint32_t experts) {
-  SortPlan p{sort_block(experts), 1, 0};
-  if (n <= 1024) {
-    const uint32_t warps = uint32_t((n + 31) / 32);
-    if (warps * 32u <= p.block) {
-      p.block = warps ? warps * 32u : 32u;
-      p.blocks = 1;
-      return p;
-    }
+  SortPlan p{sort_block(experts), 1, 0, 0};
+  if (n <= p.block) {
+    p.block = n ? uint32_t((n + 31) / 32) * 32u : 32u;
+    p.cluster = 1;
+    return p;
   }
-  for (uint32_t items : {4u, uint32_t(kTileItems)}) {
-    const uint64_t tile = uint64_t(p.block) * items;
+  for (uint32_t items : {1u, 4u}) {
+    p.items = items;
     for (uint32_t blocks : {1u, 2u, 4u, 8u}) {
-      if (n <= tile * blocks) {
-        p.items = items;
-        p.blocks = blocks;
+      if (n <= uint64_t(p.block) * items * blocks) {
+        p.cluster = blocks;
         return p;
       }
     }
   }
-  p.items = kTileItems;
+  // tiles that still fill the device, large ones where there are many
+  p.items = n <= uint64_t(p.block) * 4 * 512 ? 4 : 16;
+  const uint64_t tile = uint64_t(p.block) * p.items;
+  p.tiles = uint32_t((n + tile - 1) / tile);
   return p;
-}
-
-uint64_t sort_tiles(uint64_t n, uint32_t experts) {
-  const uint64_t tile = uint64_t(sort_block(experts)) * kTileItems;
-  return (n + tile - 1) / tile;
 }
 
 template <typename ID>
 int launch_sort(uint64_t n, const ID* ids, uint32_t experts, int32_t* offsets, int32_t* position,
                 int32_t* source, void* work, cudaStream_t stream) {
   const SortPlan p = plan_sort(n, experts);
-  if (p.blocks != 0) {
+  if (p.cluster != 0) {
+    auto kernel = p.items == 1 ? sort_cluster_kernel<ID, 1> : sort_cluster_kernel<ID, 4>;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(p.blocks);
+    config.gridDim = dim3(p.cluster);
     config.blockDim = dim3(p.block);
     config.stream = stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = p.blocks;
+    attr.val.clusterDim.x = p.cluster;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = 1;
-    auto kernel = p.items == 1   ? sort_cluster_kernel<ID, 1>
-                  : p.items == 4 ? sort_cluster_kernel<ID, 4>
-                                 : sort_cluster_kernel<ID, kTileItems>;
     const cudaError_t e =
         cudaLaunchKernelEx(&config, kernel, ids, n, experts, offsets, position, source);
     if (e != cudaSuccess) {
@@ -397,13 +422,14 @@ int launch_sort(uint64_t n, const ID* ids, uint32_t experts, int32_t* offsets, i
     }
     return HKV_OK;
   }
-  const uint32_t tiles = uint32_t(sort_tiles(n, experts));
   uint32_t* counts = static_cast<uint32_t*>(work);
-  uint32_t* totals = counts + uint64_t(tiles) * experts;
-  sort_count_kernel<ID><<<tiles, 512, 0, stream>>>(ids, n, experts, p.block * kTileItems, counts);
-  sort_scan_kernel<<<(experts + 31u) / 32u, 1024, 0, stream>>>(experts, tiles, counts, totals);
-  sort_place_kernel<ID><<<tiles, p.block, 0, stream>>>(ids, n, experts, counts, totals, offsets,
-                                                       position, source);
+  uint32_t* totals = p.tiles > kTilesSummed ? counts + uint64_t(p.tiles) * experts : nullptr;
+  sort_count_kernel<ID><<<p.tiles, 512, 0, stream>>>(ids, n, experts, p.block * p.items, counts);
+  if (totals != nullptr) {
+    sort_scan_kernel<<<(experts + 31u) / 32u, 1024, 0, stream>>>(experts, p.tiles, counts, totals);
+  }
+  auto place = p.items == 4 ? sort_place_kernel<ID, 4> : sort_place_kernel<ID, 16>;
+  place<<<p.tiles, p.block, 0, stream>>>(ids, n, experts, counts, totals, offsets, position, source);
   return rows_launched();
 }
 
@@ -439,7 +465,7 @@ __global__ void __launch_bounds__(kMoveBlock)
                     uint8_t* __restrict__ rows, const uint64_t rows_stride,
                     const int32_t* __restrict__ kept) {
   const uint64_t n = tokens * top_k;
-  zero_behind<(G ? G : 16)>(kept, n, rows, rows_stride, row_bytes);
+  zero_behind<(G ? G : 8)>(kept, n, rows, rows_stride, row_bytes);
   const uint64_t c = uint64_t(blockIdx.x) * kMoveBlock + threadIdx.x;
   const uint64_t token = c / chunks;
   if (token >= tokens) return;
@@ -460,9 +486,10 @@ __global__ void __launch_bounds__(kMoveBlock)
       uint8_t* q = row - (uint32_t(reinterpret_cast<uintptr_t>(row)) & 15u) + off;
       if (q >= row + row_bytes) continue;
       const uint8_t* p = from + (q - row);
-      store_chunk<(G ? G : 16)>(
-          q, load_chunk<(G ? G : 16)>(p, p < from ? from : p, from + row_bytes, x.first, x.last),
-          row, row + row_bytes);
+      Cut cut;
+      cut.load(p, x.first, x.last);
+      store_chunk<(G ? G : 8)>(q, cut.get<(G ? G : 8)>(p, from, from + row_bytes), row,
+                               row + row_bytes);
     }
   }
 }
@@ -478,7 +505,7 @@ __global__ void __launch_bounds__(kMoveBlock)
                    const uint64_t row_bytes, const RowsIn rows, const void* __restrict__ weights,
                    const bool weights_f32, const int32_t* __restrict__ position,
                    uint8_t* __restrict__ out, const uint64_t out_stride) {
-  using C = Chunk<T>;
+  constexpr int kElems = kChunkElems<T>;
   const uint64_t c = uint64_t(blockIdx.x) * kMoveBlock + threadIdx.x;
   const uint64_t token = c / chunks;
   if (token >= tokens) return;
@@ -487,11 +514,13 @@ __global__ void __launch_bounds__(kMoveBlock)
   int64_t off = int64_t(c - token * chunks) * 16;
   if (!WHOLE) off -= uint32_t(reinterpret_cast<uintptr_t>(to)) & 15u;
   if (!WHOLE && off >= int64_t(row_bytes)) return;
-  float sum[C::kElems];
+  float sum[kElems];
 #pragma unroll
-  for (int e = 0; e < C::kElems; ++e) sum[e] = 0.f;
+  for (int e = 0; e < kElems; ++e) sum[e] = 0.f;
   for (uint32_t j0 = 0; j0 < top_k; j0 += 4) {
-    C row[4];
+    uint4 row[4];
+    Cut cut[WHOLE ? 1 : 4];
+    const uint8_t* from[4];
     float w[4];
     bool ok[4];
 #pragma unroll
@@ -500,34 +529,36 @@ __global__ void __launch_bounds__(kMoveBlock)
       uint32_t place = kFull;
       if (j0 + u < top_k) place = uint32_t(position[i]);
       ok[u] = place < n;
+      from[u] = rows.first + (ok[u] ? place * rows.stride : 0);
       w[u] = 1.f;
-      if (ok[u]) {
-        const uint8_t* from = rows.first + place * rows.stride;
-        if (WHOLE) {
-          row[u].raw = __ldg(reinterpret_cast<const uint4*>(from + off));
-        } else {
-          const uint8_t* p = from + off;
-          row[u].raw = load_chunk<sizeof(T)>(p, off < 0 ? from : p, from + row_bytes, rows.first,
-                                             rows.last);
-        }
-        if (weights != nullptr) {
-          w[u] = weights_f32 ? static_cast<const float*>(weights)[i]
-                             : to_float(static_cast<const T*>(weights)[i]);
-        }
+      if (ok[u] && weights != nullptr) {
+        w[u] = weights_f32 ? static_cast<const float*>(weights)[i]
+                           : to_float(static_cast<const T*>(weights)[i]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (WHOLE) {
+        if (ok[u]) row[u] = __ldg(reinterpret_cast<const uint4*>(from[u] + off));
+      } else if (ok[u]) {
+        cut[WHOLE ? 0 : u].load(from[u] + off, rows.first, rows.last);
       }
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       if (!ok[u]) continue;
+      if (!WHOLE) {
+        row[u] = cut[WHOLE ? 0 : u].template get<sizeof(T)>(from[u] + off, from[u],
+                                                            from[u] + row_bytes);
+      }
+      float f[kElems];
+      unpack<T>(row[u], f);
 #pragma unroll
-      for (int e = 0; e < C::kElems; ++e) sum[e] = fmaf(w[u], row[u].get(e), sum[e]);
+      for (int e = 0; e < kElems; ++e) sum[e] = fmaf(w[u], f[e], sum[e]);
     }
   }
-  C result;
-#pragma unroll
-  for (int e = 0; e < C::kElems; ++e) result.set(e, sum[e]);
-  if (WHOLE) *reinterpret_cast<uint4*>(to + off) = result.raw;
-  else store_chunk<sizeof(T)>(to + off, result.raw, to, to + row_bytes);
+  if (WHOLE) *reinterpret_cast<uint4*>(to + off) = pack<T>(sum);
+  else store_chunk<sizeof(T)>(to + off, pack<T>(sum), to, to + row_bytes);
 }
 
 // ---- combine, backward ----------------------------------------------------------
@@ -546,7 +577,7 @@ __global__ void __launch_bounds__(256)
                             const bool weights_f32, const int32_t* __restrict__ position,
                             uint8_t* __restrict__ d_rows, const uint64_t d_rows_stride,
                             void* __restrict__ d_weights, const int32_t* __restrict__ kept) {
-  using C = Chunk<T>;
+  constexpr int kElems = kChunkElems<T>;
   __shared__ float partial[8][4];
   const uint64_t n = tokens * top_k;
   zero_behind<sizeof(T)>(kept, n, d_rows, d_rows_stride, row_bytes);
@@ -570,45 +601,49 @@ __global__ void __launch_bounds__(256)
     }
     if (live) {
       for (uint32_t c = lane; c < chunks; c += group) {
-        C d[WHOLE ? 1 : 4], row[4];
+        uint4 d[WHOLE ? 1 : 4], row[4];
+        Cut d_cut[WHOLE ? 1 : 4], row_cut[WHOLE ? 1 : 4];
         int64_t off[4];
-        if (WHOLE) d[0].raw = __ldg(reinterpret_cast<const uint4*>(d_from + uint64_t(c) * 16));
+        if (WHOLE) d[0] = __ldg(reinterpret_cast<const uint4*>(d_from + uint64_t(c) * 16));
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           if (place[u] >= n) continue;
           const uint8_t* from = rows.first + place[u] * rows.stride;
           if (WHOLE) {
-            row[u].raw = __ldg(reinterpret_cast<const uint4*>(from + uint64_t(c) * 16));
+            row[u] = __ldg(reinterpret_cast<const uint4*>(from + uint64_t(c) * 16));
           } else {
             const uint8_t* to = d_rows + place[u] * d_rows_stride;
             off[u] = int64_t(c) * 16 - (uint32_t(reinterpret_cast<uintptr_t>(to)) & 15u);
-            row[u].raw = d[u % (WHOLE ? 1 : 4)].raw = make_uint4(0, 0, 0, 0);
+            row_cut[WHOLE ? 0 : u].none();
+            d_cut[WHOLE ? 0 : u].none();
             if (off[u] < int64_t(row_bytes)) {
-              const uint8_t* p = from + off[u];
-              row[u].raw = load_chunk<sizeof(T)>(p, off[u] < 0 ? from : p, from + row_bytes,
-                                                 rows.first, rows.last);
-              p = d_from + off[u];
-              d[u % (WHOLE ? 1 : 4)].raw = load_chunk<sizeof(T)>(
-                  p, off[u] < 0 ? d_from : p, d_from + row_bytes, d_out.first, d_out.last);
+              row_cut[WHOLE ? 0 : u].load(from + off[u], rows.first, rows.last);
+              d_cut[WHOLE ? 0 : u].load(d_from + off[u], d_out.first, d_out.last);
             }
           }
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           if (place[u] >= n) continue;
-          const C& du = d[WHOLE ? 0 : u];
-          uint8_t* to = d_rows + place[u] * d_rows_stride;
-          C g;
-#pragma unroll
-          for (int e = 0; e < C::kElems; ++e) {
-            const int64_t b = WHOLE ? 0 : off[u] + e * int(sizeof(T));
-            if (WHOLE || (b >= 0 && b < int64_t(row_bytes))) {
-              dot[u] = fmaf(du.get(e), row[u].get(e), dot[u]);
-            }
-            g.set(e, w[u] * du.get(e));
+          if (!WHOLE) {
+            const uint8_t* from = rows.first + place[u] * rows.stride;
+            row[u] = row_cut[WHOLE ? 0 : u].template get<sizeof(T)>(from + off[u], from,
+                                                                        from + row_bytes);
+            d[WHOLE ? 0 : u] = d_cut[WHOLE ? 0 : u].template get<sizeof(T)>(
+                d_from + off[u], d_from, d_from + row_bytes);
           }
-          if (WHOLE) *reinterpret_cast<uint4*>(to + uint64_t(c) * 16) = g.raw;
-          else store_chunk<sizeof(T)>(to + off[u], g.raw, to, to + row_bytes);
+          uint8_t* to = d_rows + place[u] * d_rows_stride;
+          float du[kElems], y[kElems];
+          unpack<T>(d[WHOLE ? 0 : u], du);
+          unpack<T>(row[u], y);
+#pragma unroll
+          for (int e = 0; e < kElems; ++e) {
+            const int64_t b = WHOLE ? 0 : off[u] + e * int(sizeof(T));
+            if (WHOLE || (b >= 0 && b < int64_t(row_bytes))) dot[u] = fmaf(du[e], y[e], dot[u]);
+            du[e] *= w[u];
+          }
+          if (WHOLE) *reinterpret_cast<uint4*>(to + uint64_t(c) * 16) = pack<T>(du);
+          else store_chunk<sizeof(T)>(to + off[u], pack<T>(du), to, to + row_bytes);
         }
       }
     }
@@ -692,8 +727,8 @@ const char* hkv_rows_last_error(void) { return g_rows_error.c_str(); }
 uint64_t hkv_expert_sort_workspace_bytes(uint64_t tokens, uint32_t top_k, uint32_t experts) {
   if (check_order(tokens, top_k, experts) != HKV_OK) return 0;
   const uint64_t n = tokens * top_k;
-  if (n == 0 || plan_sort(n, experts).blocks != 0) return 0;
-  return (sort_tiles(n, experts) + 1) * experts * sizeof(uint32_t);
+  const SortPlan p = plan_sort(n, experts);
+  return p.cluster != 0 ? 0 : (uint64_t(p.tiles) + 1) * experts * sizeof(uint32_t);
 }
 
 int hkv_expert_sort(uint64_t tokens, uint32_t top_k, const void* expert_ids, uint32_t id_bytes,

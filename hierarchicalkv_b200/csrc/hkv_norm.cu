@@ -28,86 +28,82 @@ namespace hkv {
 namespace {
 
 constexpr uint32_t kFull = 0xFFFFFFFFu;
-constexpr int kNormBlock = 256;       // forward; more where a row needs more
-constexpr int kBackwardBlock = 512;
+constexpr int kNormBlock = 256;   // of a batch of few rows; more where a row needs more
+constexpr int kPipeBlock = 512;   // of the kernels that stay on the device
+constexpr int kStages = 3;        // rows of a warp's queue: one in use, two on their way
 
 // Sum over the `group` threads of a row (a power of two: part of a warp, or
-// whole warps of this block); every thread gets it.  scratch: two floats of each
-// value per warp, used in turn, so that one barrier of the group's own (named
-// 1 + its number in the block) is enough.
-template <int N>
+// whole warps of this block); every thread gets it.  WIDE: group >= 32.
+// scratch: two floats of each value per warp, used in turn, so that one barrier
+// of the group's own (named 1 + its number in the block) is enough.
+template <int N, bool WIDE>
 struct GroupSum {
-  uint32_t group, warp, first_warp, barrier;
-  float (*scratch)[2][N];   // [warps of the block]
+  uint32_t group, warps, from, barrier;   // warps: of the group
+  float (*scratch)[2][N];                 // [warps of the block]
   uint32_t turn = 0;
 
   __device__ __forceinline__ GroupSum(uint32_t group_, float (*scratch_)[2][N])
-      : group(group_),
-        warp(threadIdx.x >> 5),
-        first_warp((threadIdx.x >> 5) & ~((group_ >> 5) - (group_ >> 5 ? 1u : 0u))),
-        barrier(1u + threadIdx.x / group_),
-        scratch(scratch_) {}
+      : group(group_), warps(group_ >> 5), barrier(1u + threadIdx.x / group_), scratch(scratch_) {
+    // where this lane reads when the group's warps exchange their sums
+    from = WIDE ? ((threadIdx.x >> 5) & ~(warps - 1u)) + (threadIdx.x & (warps - 1u)) : 0u;
+  }
 
   __device__ __forceinline__ void operator()(float (&v)[N]) {
-    const uint32_t width = group < 32u ? group : 32u;
-    for (uint32_t d = width >> 1; d > 0; d >>= 1) {
+    if (WIDE) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(kFull, v[i], d);
+      for (int d = 16; d > 0; d >>= 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(kFull, v[i], d);
+      }
+      if (warps == 1) return;
+      if ((threadIdx.x & 31u) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) scratch[threadIdx.x >> 5][turn][i] = v[i];
+      }
+      asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(group) : "memory");
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = scratch[from][turn][i];
+      for (uint32_t d = warps >> 1; d > 0; d >>= 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(kFull, v[i], d);
+      }
+      turn ^= 1u;
+    } else {
+      for (uint32_t d = group >> 1; d > 0; d >>= 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(kFull, v[i], d);
+      }
     }
-    if (group <= 32u) return;
-    if ((threadIdx.x & 31u) == 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) scratch[warp][turn][i] = v[i];
-    }
-    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(group) : "memory");
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = 0.f;
-    for (uint32_t w = first_warp; w < first_warp + (group >> 5); ++w) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] += scratch[w][turn][i];
-    }
-    turn ^= 1u;
   }
 };
 
 // Where a thread's chunks lie in its row: chunk c of the thread is
 // first + c * width.  A warp of a group above 32 owns consecutive chunks, so that
 // neighbouring chunks are in neighbouring lanes whatever the group.
+template <int CHUNKS, bool WIDE>
 struct ChunkMap {
   uint32_t first, width, lane;   // lane: within the width
 
-  __device__ __forceinline__ ChunkMap(uint32_t group, int per_thread) {
-    width = group < 32u ? group : 32u;
+  __device__ __forceinline__ explicit ChunkMap(uint32_t group) {
+    width = WIDE ? 32u : group;
     lane = threadIdx.x & (width - 1u);
-    const uint32_t warp_in_group = (threadIdx.x & (group - 1u)) >> 5;
-    first = warp_in_group * 32u * uint32_t(per_thread) + lane;
+    const uint32_t warp_in_group = WIDE ? (threadIdx.x & (group - 1u)) >> 5 : 0u;
+    first = warp_in_group * 32u * CHUNKS + lane;
   }
-  __device__ __forceinline__ uint32_t operator()(int c) const { return first + uint32_t(c) * width; }
+  __device__ __forceinline__ uint32_t operator()(int c) const {
+    return first + uint32_t(c) * (WIDE ? 32u : width);
+  }
 };
 
-// The thread's chunks of a row; what is behind the row's end is zero.
-template <typename T, int CHUNKS, bool WHOLE>
-__device__ __forceinline__ void load_row(const uint8_t* row, uint64_t row_bytes, uint32_t chunks,
-                                         const ChunkMap& map, const uint8_t* first,
-                                         const uint8_t* last, Chunk<T> (&x)[CHUNKS]) {
+// Elements of a chunk that lie behind the row's end (only the last chunk has some).
+template <typename T, int N>
+__device__ __forceinline__ void clear_tail(uint32_t chunk, uint32_t chunks, uint32_t dim, float fill,
+                                           float (&f)[N]) {
+  if (chunk + 1 != chunks) return;
+  const int have = int(dim - chunk * N);
 #pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
-    const uint32_t at = map(c);
-    x[c].raw = make_uint4(0, 0, 0, 0);
-    if (row == nullptr || at >= chunks) continue;
-    const uint8_t* p = row + uint64_t(at) * 16;
-    if (WHOLE) {
-      x[c].raw = __ldg(reinterpret_cast<const uint4*>(p));
-    } else {
-      x[c].raw = load_chunk<sizeof(T)>(p, p, row + row_bytes, first, last);
-      if (p + 16 > row + row_bytes) {
-        const int have = int(row + row_bytes - p) / int(sizeof(T));
-#pragma unroll
-        for (int e = 0; e < Chunk<T>::kElems; ++e) {
-          if (e >= have) x[c].set(e, 0.f);
-        }
-      }
-    }
+  for (int e = 0; e < N; ++e) {
+    if (e >= have) f[e] = fill;
   }
 }
 
@@ -115,14 +111,15 @@ __device__ __forceinline__ void load_row(const uint8_t* row, uint64_t row_bytes,
 // bytes belong to two neighbouring chunks: a lane gets its left neighbour's and
 // stores the joint; only the ends of the row, and of a warp's run of it, are
 // stored element by element.  The whole warp calls; row == nullptr: nothing.
-template <typename T, int CHUNKS, bool WHOLE>
-__device__ __forceinline__ void store_row(uint8_t* row, uint64_t row_bytes, uint32_t chunks,
-                                          const ChunkMap& map, const Chunk<T> (&y)[CHUNKS]) {
+template <typename T, int CHUNKS, bool WHOLE, bool WIDE>
+__device__ __forceinline__ void store_row(uint8_t* row, uint32_t row_bytes, uint32_t chunks,
+                                          const ChunkMap<CHUNKS, WIDE>& map,
+                                          const uint4 (&y)[CHUNKS]) {
   if (WHOLE) {
+    uint4* to = reinterpret_cast<uint4*>(row) + map.first;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      const uint32_t at = map(c);
-      if (row != nullptr && at < chunks) *reinterpret_cast<uint4*>(row + uint64_t(at) * 16) = y[c].raw;
+      if (row != nullptr && map(c) < chunks) to[map(c) - map.first] = y[c];
     }
     return;
   }
@@ -133,76 +130,225 @@ __device__ __forceinline__ void store_row(uint8_t* row, uint64_t row_bytes, uint
   for (int c = 0; c < CHUNKS; ++c) {
     const uint32_t at = map(c);
     const bool to_next = map.lane == map.width - 1u;   // its right neighbour is in the next round
-    const uint4 mine = y[c].raw;
-    const uint4 give = to_next && c > 0 ? y[c > 0 ? c - 1 : 0].raw : mine;
+    const uint4 give = to_next && c > 0 ? y[c > 0 ? c - 1 : 0] : y[c];
     uint4 prev;
     prev.x = __shfl_sync(kFull, give.x, left);
     prev.y = __shfl_sync(kFull, give.y, left);
     prev.z = __shfl_sync(kFull, give.z, left);
     prev.w = __shfl_sync(kFull, give.w, left);
     if (row == nullptr || at > chunks) continue;
-    uint8_t* q = row + uint64_t(at) * 16;
+    uint8_t* q = row + at * 16u;
     const bool joined = map.lane != 0 || c > 0;        // the left neighbour's bytes are here
     if (s == 0) {
-      store_chunk<sizeof(T)>(q, mine, row, end);
+      store_chunk<sizeof(T)>(q, y[c], row, end);
       continue;
     }
-    store_chunk<sizeof(T)>(q - s, shifted(prev, mine, 16u - s), joined ? row : q, end);
+    store_chunk<sizeof(T)>(q - s, shifted(prev, y[c], 16u - s), joined ? row : q, end);
     if (c == CHUNKS - 1 && to_next) {
       // the end of the warp's run: nobody joins this chunk's last bytes
-      const uint4 none = make_uint4(0, 0, 0, 0);
       const uint8_t* stop = q + 16 < end ? q + 16 : end;
-      store_chunk<sizeof(T)>(q - s + 16, shifted(mine, none, 16u - s), row, stop);
+      store_chunk<sizeof(T)>(q - s + 16, shifted(y[c], make_uint4(0, 0, 0, 0), 16u - s), row, stop);
     }
   }
 }
 
-// weight or bias of a chunk's columns; 1 or 0 where there is none or no column.
-template <typename T, bool WHOLE, int N>
-__device__ __forceinline__ void load_params(const void* p, bool f32, uint32_t column, uint32_t dim,
-                                            float none, float (&out)[N]) {
-  if (p == nullptr) {
+// A warp's queue of rows in shared memory, filled ahead with asynchronous copies
+// that hold no registers.  The slots belong to the warp alone: no barrier of the
+// block is needed, and of the warp only for unaligned rows.  A slot holds an
+// aligned chunk; unaligned rows have one more chunk per row (of the warp's part of
+// the row), and a thread cuts its chunks out of neighbouring slots.
+template <typename T, int CHUNKS, bool WHOLE, bool WIDE>
+struct RowQueue {
+  using Map = ChunkMap<CHUNKS, WIDE>;
+  uint32_t mine;         // shared address of this lane's slot 0 (WHOLE) or of its row's first
+  uint32_t stage_bytes;  // distance of a warp's stages
+  uint32_t row_bytes;
+  uint32_t chunks;
+
+  // `shared`: kStages * operands * warps * slots_per_warp slots; operand: which
+  // of the row's matrices this queue holds
+  __device__ __forceinline__ RowQueue(const uint4* shared, uint32_t operand, uint32_t operands,
+                                      const Map& map, uint32_t row_bytes_, uint32_t chunks_)
+      : row_bytes(row_bytes_), chunks(chunks_) {
+    const uint32_t warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t slots = slots_per_warp(map.width);
+    stage_bytes = operands * warps * slots * 16u;
+    mine = static_cast<uint32_t>(__cvta_generic_to_shared(shared)) +
+           (operand * warps + warp) * slots * 16u +
+           (WHOLE ? lane : (lane / map.width) * (map.width * CHUNKS + 1u)) * 16u;
+  }
+  static __host__ __device__ __forceinline__ uint32_t slots_per_warp(uint32_t width) {
+    return WHOLE ? 32u * CHUNKS : 32u * CHUNKS + 32u / width;
+  }
+
+  // Puts a row (null: none) into a stage.
+  __device__ __forceinline__ void fill(uint32_t stage, const uint8_t* row, const Map& map,
+                                       const uint8_t* first, const uint8_t* last) const {
+    if (row == nullptr) return;
+    const uint32_t to = mine + stage * stage_bytes;
+    if (WHOLE) {
+      const uint8_t* from = row + map.first * 16u;
 #pragma unroll
-    for (int e = 0; e < N; ++e) out[e] = none;
-  } else if (WHOLE) {
-    // whole chunks of columns, and the launcher has checked the address
-    if (f32) {
-      const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + column);
-#pragma unroll
-      for (int e = 0; e < N; e += 4) {
-        const float4 v = __ldg(s + e / 4);
-        out[e] = v.x;
-        out[e + 1] = v.y;
-        out[e + 2] = v.z;
-        out[e + 3] = v.w;
+      for (int c = 0; c < CHUNKS; ++c) {
+        if (map(c) < chunks) copy_async(to + c * 512u, from + (map(c) - map.first) * 16u);
       }
     } else {
-      Chunk<T> v;
-      v.raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p) + column));
+      const uint8_t* aligned = row - (reinterpret_cast<uintptr_t>(row) & 15u);
+      const uint8_t* end = row + row_bytes;
 #pragma unroll
-      for (int e = 0; e < N; ++e) out[e] = v.get(e);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      out[e] = none;
-      if (column + e < dim) {
-        out[e] = f32 ? static_cast<const float*>(p)[column + e]
-                     : to_float(static_cast<const T*>(p)[column + e]);
+      for (int c = 0; c <= CHUNKS; ++c) {
+        if (c == CHUNKS && map.lane != 0) break;
+        const uint8_t* a = aligned + map(c) * 16u;
+        if (a >= end) break;
+        const uint32_t slot = to + (c * map.width + map.lane) * 16u;
+        if (a >= first && a + 16 <= last) {
+          copy_async(slot, a);
+        } else {   // at an end of the matrix
+          const uint4 v = pieces<sizeof(T)>(a, row, end);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(slot), "r"(v.x), "r"(v.y),
+                       "r"(v.z), "r"(v.w)
+                       : "memory");
+        }
       }
+    }
+  }
+
+  static __device__ __forceinline__ uint4 slot_at(uint32_t address) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(address)
+                 : "memory");
+    return v;
+  }
+
+  // Chunk c of the thread of the row in a stage, as floats; zeros where there is none.
+  __device__ __forceinline__ void take(uint32_t stage, int c, const uint8_t* row, const Map& map,
+                                       uint32_t dim, float (&f)[kChunkElems<T>]) const {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    const uint32_t from = mine + stage * stage_bytes;
+    if (row != nullptr && map(c) < chunks) {
+      if (WHOLE) {
+        v = slot_at(from + c * 512u);
+      } else {
+        const uint32_t s = uint32_t(reinterpret_cast<uintptr_t>(row)) & 15u;
+        const uint32_t slot = from + (c * map.width + map.lane) * 16u;
+        v = slot_at(slot);
+        if (s != 0) v = shifted(v, slot_at(slot + 16u), s);
+      }
+    }
+    unpack<T>(v, f);
+    if (!WHOLE) clear_tail<T>(map(c), chunks, dim, 0.f, f);
+  }
+};
+
+// Weights or biases of a chunk's columns; `none` where there is no pointer or no
+// column.  vec: the address is a multiple of 16 (of the columns, only the last
+// chunk's may be part of a chunk).
+template <typename T, int N>
+__device__ __forceinline__ void load_params(const void* p, bool f32, bool vec, uint32_t column,
+                                            uint32_t dim, float none, float (&out)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) out[e] = none;
+  if (p == nullptr) return;
+  if constexpr (N == kChunkElems<T>) {
+    if (vec && column + N <= dim) {
+      if (f32) {
+        const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + column);
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+          const float4 v = __ldg(s + e / 4);
+          out[e] = v.x;
+          out[e + 1] = v.y;
+          out[e + 2] = v.z;
+          out[e + 3] = v.w;
+        }
+      } else {
+        unpack<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p) + column)), out);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    if (column + e < dim) {
+      out[e] = f32 ? static_cast<const float*>(p)[column + e]
+                   : to_float(static_cast<const T*>(p)[column + e]);
     }
   }
 }
 
-// CHUNKS chunks per thread, `group` threads per row, one row per group.
-template <typename T, int CHUNKS, bool WHOLE>
+// Normalises the row whose elements are in x and stores it; row == nullptr: none.
+// w, b: the thread's columns of weight and bias.
+template <typename T, int CHUNKS, bool WHOLE, bool WIDE>
+__device__ __forceinline__ void norm_row(const NormArgs& a, uint32_t r, const uint8_t* row,
+                                         uint32_t chunks, const ChunkMap<CHUNKS, WIDE>& map,
+                                         GroupSum<1, WIDE>& group_sum,
+                                         float (&x)[CHUNKS][kChunkElems<T>],
+                                         const float (&w)[CHUNKS][kChunkElems<T>],
+                                         const float (&b)[CHUNKS][kChunkElems<T>]) {
+  constexpr int kElems = kChunkElems<T>;
+  const uint32_t dim = uint32_t(a.dim);
+  float sum[1] = {0.f};
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) sum[0] += x[c][e];
+  }
+  group_sum(sum);
+  const float mean = sum[0] * a.inv_dim;
+  float sq[1] = {0.f};
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    if (map(c) < chunks) {
+      if (!WHOLE) clear_tail<T>(map(c), chunks, dim, mean, x[c]);
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        x[c][e] -= mean;
+        sq[0] = fmaf(x[c][e], x[c][e], sq[0]);
+      }
+    }
+  }
+  group_sum(sq);
+  const float rstd = rsqrtf(fmaf(sq[0], a.inv_dim, a.eps));
+  uint4 y[CHUNKS];
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) x[c][e] = fmaf(x[c][e] * rstd, w[c][e], b[c][e]);
+    y[c] = pack<T>(x[c]);
+  }
+  uint8_t* to = row == nullptr ? nullptr : static_cast<uint8_t*>(a.y) + r * a.y_stride;
+  store_row<T, CHUNKS, WHOLE, WIDE>(to, dim * uint32_t(sizeof(T)), chunks, map, y);
+  if (row != nullptr && map.first == 0) {
+    if (a.mean != nullptr) a.mean[r] = mean;
+    if (a.rstd != nullptr) a.rstd[r] = rstd;
+  }
+}
+
+template <typename T, int CHUNKS, bool WIDE>
+__device__ __forceinline__ void load_norm_params(const NormArgs& a, uint32_t chunks,
+                                                 const ChunkMap<CHUNKS, WIDE>& map,
+                                                 float (&w)[CHUNKS][kChunkElems<T>],
+                                                 float (&b)[CHUNKS][kChunkElems<T>]) {
+  const uint32_t dim = uint32_t(a.dim);
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const uint32_t column = map(c) < chunks ? map(c) * kChunkElems<T> : dim;
+    load_params<T>(a.weight, a.params_f32, a.params_vec, column, dim, 1.f, w[c]);
+    load_params<T>(a.bias, a.params_f32, a.params_vec, column, dim, 0.f, b[c]);
+  }
+}
+
+// Few rows: one per group of `group` threads, CHUNKS chunks per thread.  The
+// weights are on their way while the row is reduced.
+template <typename T, int CHUNKS, bool WHOLE, bool WIDE>
 __global__ void __launch_bounds__(1024)
     norm_kernel(const NormArgs a, const uint32_t group, const uint32_t chunks, const RowsIn in) {
-  using C = Chunk<T>;
   __shared__ float scratch[32][2][1];
-  const uint64_t r = (uint64_t(blockIdx.x) * blockDim.x + threadIdx.x) / group;
-  const ChunkMap map(group, CHUNKS);
-  const uint64_t row_bytes = a.dim * sizeof(T);
+  const uint32_t r = uint32_t((uint64_t(blockIdx.x) * blockDim.x + threadIdx.x) / group);
+  const ChunkMap<CHUNKS, WIDE> map(group);
+  const uint32_t dim = uint32_t(a.dim), row_bytes = dim * uint32_t(sizeof(T));
   const uint8_t *row = nullptr, *first = in.first, *last = in.last;
   if (r < a.n) {
     if (a.row_ptrs != nullptr) {
@@ -212,46 +358,77 @@ __global__ void __launch_bounds__(1024)
       row = in.first + r * in.stride;
     }
   }
-  C x[CHUNKS];
-  load_row<T, CHUNKS, WHOLE>(row, row_bytes, chunks, map, first, last, x);
-  GroupSum<1> group_sum(group, scratch);
-  const float inv_dim = a.inv_dim;
-  float sum[1] = {0.f};
+  float x[CHUNKS][kChunkElems<T>], w[CHUNKS][kChunkElems<T>], b[CHUNKS][kChunkElems<T>];
+  Cut cut[CHUNKS];
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-#pragma unroll
-    for (int e = 0; e < C::kElems; ++e) sum[0] += x[c].get(e);
-  }
-  group_sum(sum);
-  const float mean = sum[0] * inv_dim;
-  float sq[1] = {0.f};
-#pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
-    const uint32_t column = map(c) * C::kElems;
-#pragma unroll
-    for (int e = 0; e < C::kElems; ++e) {
-      const float d = x[c].get(e) - mean;
-      if (column + (WHOLE ? 0 : e) < a.dim) sq[0] = fmaf(d, d, sq[0]);
+    cut[c].none();
+    if (row != nullptr && map(c) < chunks) {
+      if (WHOLE) cut[c].lo = __ldg(reinterpret_cast<const uint4*>(row) + map(c));
+      else cut[c].load(row + map(c) * 16u, first, last);
     }
   }
-  group_sum(sq);
-  const float rstd = 1.f / sqrtf(fmaf(sq[0], inv_dim, a.eps));
+  load_norm_params<T, CHUNKS, WIDE>(a, chunks, map, w, b);
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-    if (map(c) >= chunks) break;
-    float w[C::kElems], b[C::kElems];
-    const uint32_t column = map(c) * C::kElems;
-    load_params<T, WHOLE>(a.weight, a.params_f32, column, uint32_t(a.dim), 1.f, w);
-    load_params<T, WHOLE>(a.bias, a.params_f32, column, uint32_t(a.dim), 0.f, b);
+    const uint8_t* p = row + map(c) * 16u;
+    unpack<T>(WHOLE ? cut[c].lo : cut[c].template get<sizeof(T)>(p, row, row + row_bytes), x[c]);
+    if (!WHOLE) clear_tail<T>(map(c), chunks, dim, 0.f, x[c]);
+  }
+  GroupSum<1, WIDE> group_sum(group, scratch);
+  norm_row<T, CHUNKS, WHOLE, WIDE>(a, r, row, chunks, map, group_sum, x, w, b);
+}
+
+// Many rows: the blocks stay on the device, their threads keep the weights of
+// their columns, and their groups take rows in turn out of the warps' queues.
+template <typename T, int CHUNKS, bool WHOLE, bool WIDE>
+__global__ void __launch_bounds__(kPipeBlock, 1)
+    norm_pipe_kernel(const NormArgs a, const uint32_t group, const uint32_t chunks, const RowsIn in) {
+  extern __shared__ uint4 slots[];
+  __shared__ float scratch[kPipeBlock / 32][2][1];
+  GroupSum<1, WIDE> group_sum(group, scratch);
+  const ChunkMap<CHUNKS, WIDE> map(group);
+  const uint32_t n = uint32_t(a.n), dim = uint32_t(a.dim), row_bytes = dim * uint32_t(sizeof(T));
+  const RowQueue<T, CHUNKS, WHOLE, WIDE> queue(slots, 0, 1, map, row_bytes, chunks);
+  float w[CHUNKS][kChunkElems<T>], b[CHUNKS][kChunkElems<T>];
+  load_norm_params<T, CHUNKS, WIDE>(a, chunks, map, w, b);
+  const uint32_t step = gridDim.x * (kPipeBlock / group);
+  uint32_t r = blockIdx.x * (kPipeBlock / group) + threadIdx.x / group;
+  auto address = [&](uint32_t row) -> const uint8_t* {
+    if (row >= n) return nullptr;
+    return a.row_ptrs != nullptr ? static_cast<const uint8_t*>(a.row_ptrs[row])
+                                 : in.first + row * in.stride;
+  };
+  auto fill = [&](uint32_t stage, const uint8_t* row) {
+    const bool by_address = a.row_ptrs != nullptr;
+    queue.fill(stage, row, map, by_address ? row : in.first, by_address ? row + row_bytes : in.last);
+    copies_commit();
+  };
+  // rows[0]: the current row, rows[1 ...]: those in the queue, rows[kStages]: the
+  // one whose address has arrived by the time its copies start
+  const uint8_t* rows[kStages + 1];
 #pragma unroll
-    for (int e = 0; e < C::kElems; ++e) x[c].set(e, fmaf((x[c].get(e) - mean) * rstd, w[e], b[e]));
+  for (int i = 0; i < kStages; ++i) rows[i + 1] = address(r + i * step);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fill(i, rows[i + 1]);
+  uint32_t stage = 0;
+  // the lanes of a warp leave together: when the row of its first group is past the end
+  for (uint32_t warp_row = r - (WIDE ? 0u : (threadIdx.x & 31u) / group); warp_row < n;
+       warp_row += step, r += step) {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) rows[i] = rows[i + 1];
+    fill(stage == 0 ? kStages - 1 : stage - 1, rows[kStages - 1]);
+    rows[kStages] = address(r + kStages * step);
+    copies_wait<kStages - 1>();
+    if (!WHOLE) __syncwarp();
+    float x[CHUNKS][kChunkElems<T>];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) queue.take(stage, c, rows[0], map, dim, x[c]);
+    if (!WHOLE) __syncwarp();   // the slots are free again
+    norm_row<T, CHUNKS, WHOLE, WIDE>(a, r, rows[0], chunks, map, group_sum, x, w, b);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
-  uint8_t* to = row == nullptr ? nullptr : static_cast<uint8_t*>(a.y) + r * a.y_stride;
-  store_row<T, CHUNKS, WHOLE>(to, row_bytes, chunks, map, x);
-  if (row != nullptr && (threadIdx.x & (group - 1u)) == 0) {
-    if (a.mean != nullptr) a.mean[r] = mean;
-    if (a.rstd != nullptr) a.rstd[r] = rstd;
-  }
+  copies_wait<0>();
 }
 
 // Rows too long for the registers of a block: three passes over the row, which
@@ -260,7 +437,7 @@ template <typename T>
 __global__ void __launch_bounds__(1024)
     norm_long_kernel(const NormArgs a) {
   __shared__ float scratch[32][2][1];
-  GroupSum<1> group_sum(blockDim.x, scratch);
+  GroupSum<1, true> group_sum(blockDim.x, scratch);
   const uint32_t dim = uint32_t(a.dim);
   for (uint64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
     const T* row = a.row_ptrs != nullptr
@@ -277,12 +454,12 @@ __global__ void __launch_bounds__(1024)
       sq[0] = fmaf(d, d, sq[0]);
     }
     group_sum(sq);
-    const float rstd = 1.f / sqrtf(fmaf(sq[0], a.inv_dim, a.eps));
+    const float rstd = rsqrtf(fmaf(sq[0], a.inv_dim, a.eps));
     T* out = reinterpret_cast<T*>(static_cast<uint8_t*>(a.y) + r * a.y_stride);
     for (uint32_t i = threadIdx.x; i < dim; i += blockDim.x) {
       float w[1], b[1];
-      load_params<T, false>(a.weight, a.params_f32, i, dim, 1.f, w);
-      load_params<T, false>(a.bias, a.params_f32, i, dim, 0.f, b);
+      load_params<T>(a.weight, a.params_f32, false, i, dim, 1.f, w);
+      load_params<T>(a.bias, a.params_f32, false, i, dim, 0.f, b);
       out[i] = from_float<T>(fmaf((to_float(row[i]) - mean) * rstd, w[0], b[0]));
     }
     if (threadIdx.x == 0) {
@@ -297,7 +474,7 @@ __global__ void __launch_bounds__(1024)
 // The blocks stay on the device and take rows in turn: a thread sees the same
 // columns of every row it touches, so the column sums d_weight and d_bias build
 // up in its registers beside the row's own work, and x and dy are read once.
-// The next row's chunks are on their way while the current row is reduced.
+// The next rows are on their way into the warps' queues meanwhile.
 // At the end each block writes one row of column sums (its groups added in a
 // fixed order), and norm_reduce_kernel adds the blocks' rows in a fixed order.
 
@@ -306,78 +483,87 @@ struct NormBackwardPlan {
   bool fits;   // a row fits the registers of a block
 };
 
-template <typename T, int CHUNKS, bool WHOLE>
-__global__ void __launch_bounds__(kBackwardBlock, 1)
+template <typename T, int CHUNKS, bool WHOLE, bool WIDE>
+__global__ void __launch_bounds__(kPipeBlock, 1)
     norm_backward_kernel(const NormBackwardArgs a, const uint32_t group, const uint32_t chunks,
                          const RowsIn x_in, const RowsIn dy_in, float* __restrict__ sums) {
-  using C = Chunk<T>;
-  constexpr int kElems = C::kElems;
-  extern __shared__ float columns[];   // [copies][dim]: the column sums of each warp or group
-  __shared__ float scratch[kBackwardBlock / 32][2][2];
-  GroupSum<2> group_sum(group, scratch);
-  const ChunkMap map(group, CHUNKS);
-  const uint32_t dim = uint32_t(a.dim);
-  const uint64_t row_bytes = a.dim * sizeof(T);
-  const uint32_t groups = kBackwardBlock / group;
+  constexpr int kElems = kChunkElems<T>;
+  extern __shared__ uint4 slots[];
+  float* columns = reinterpret_cast<float*>(slots);   // [copies][dim], after the last row
+  __shared__ float scratch[kPipeBlock / 32][2][2];
+  GroupSum<2, WIDE> group_sum(group, scratch);
+  const ChunkMap<CHUNKS, WIDE> map(group);
+  const uint32_t n = uint32_t(a.n), dim = uint32_t(a.dim), row_bytes = dim * uint32_t(sizeof(T));
+  const uint32_t groups = kPipeBlock / group;
+  const RowQueue<T, CHUNKS, WHOLE, WIDE> x_queue(slots, 0, 2, map, row_bytes, chunks);
+  const RowQueue<T, CHUNKS, WHOLE, WIDE> dy_queue(slots, 1, 2, map, row_bytes, chunks);
   float w[CHUNKS][kElems], dw[CHUNKS][kElems], db[CHUNKS][kElems];
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
 #pragma unroll
-    for (int e = 0; e < kElems; ++e) dw[c][e] = db[c][e] = w[c][e] = 0.f;
-    if (map(c) < chunks) {
-      load_params<T, WHOLE>(a.weight, a.params_f32, map(c) * kElems, dim, 1.f, w[c]);
-    }
+    for (int e = 0; e < kElems; ++e) dw[c][e] = db[c][e] = 0.f;
+    load_params<T>(a.weight, a.params_f32, a.params_vec, map(c) < chunks ? map(c) * kElems : dim, dim,
+                   1.f, w[c]);
   }
-  const uint64_t step = uint64_t(gridDim.x) * groups;
-  uint64_t r = uint64_t(blockIdx.x) * groups + threadIdx.x / group;
-  C x[CHUNKS], dy[CHUNKS];
-  float mean = 0.f, rstd = 0.f;
-  auto fetch = [&](uint64_t row) {
-    const bool live = row < a.n;
-    mean = live ? __ldg(a.mean + row) : 0.f;
-    rstd = live ? __ldg(a.rstd + row) : 0.f;
-    load_row<T, CHUNKS, WHOLE>(live ? x_in.first + row * x_in.stride : nullptr, row_bytes, chunks, map,
-                               x_in.first, x_in.last, x);
-    load_row<T, CHUNKS, WHOLE>(live ? dy_in.first + row * dy_in.stride : nullptr, row_bytes, chunks,
-                               map, dy_in.first, dy_in.last, dy);
+  const uint32_t step = gridDim.x * groups;
+  uint32_t r = blockIdx.x * groups + threadIdx.x / group;
+  auto x_row = [&](uint32_t row) { return row < n ? x_in.first + row * x_in.stride : nullptr; };
+  auto dy_row = [&](uint32_t row) { return row < n ? dy_in.first + row * dy_in.stride : nullptr; };
+  auto fill = [&](uint32_t stage, uint32_t row) {
+    x_queue.fill(stage, x_row(row), map, x_in.first, x_in.last);
+    dy_queue.fill(stage, dy_row(row), map, dy_in.first, dy_in.last);
+    copies_commit();
   };
-  fetch(r);
-  // the lanes of a warp leave together: their rows are done when the warp's first is
-  for (uint64_t warp_row = r - (threadIdx.x & 31u) / group; warp_row < a.n;
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fill(i, r + i * step);
+  float next_mean = r < n ? __ldg(a.mean + r) : 0.f, next_rstd = r < n ? __ldg(a.rstd + r) : 0.f;
+  uint32_t stage = 0;
+  // the lanes of a warp leave together: when the row of its first group is past the end
+  for (uint32_t warp_row = r - (WIDE ? 0u : (threadIdx.x & 31u) / group); warp_row < n;
        warp_row += step, r += step) {
+    fill(stage == 0 ? kStages - 1 : stage - 1, r + (kStages - 1) * step);
+    const float mean = next_mean, rstd = next_rstd;
+    next_mean = r + step < n ? __ldg(a.mean + r + step) : 0.f;
+    next_rstd = r + step < n ? __ldg(a.rstd + r + step) : 0.f;
+    copies_wait<kStages - 1>();
+    if (!WHOLE) __syncwarp();
     float xhat[CHUNKS][kElems], g[CHUNKS][kElems];
     float sum[2] = {0.f, 0.f};
-    const float row_rstd = rstd;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
+      float x[kElems], dy[kElems];
+      x_queue.take(stage, c, x_row(r), map, dim, x);
+      dy_queue.take(stage, c, dy_row(r), map, dim, dy);
 #pragma unroll
       for (int e = 0; e < kElems; ++e) {
-        const float d = dy[c].get(e);
-        xhat[c][e] = (x[c].get(e) - mean) * rstd;
-        g[c][e] = d * w[c][e];
+        xhat[c][e] = (x[e] - mean) * rstd;
+        g[c][e] = dy[e] * w[c][e];
         sum[0] += g[c][e];
         sum[1] = fmaf(g[c][e], xhat[c][e], sum[1]);
-        dw[c][e] = fmaf(d, xhat[c][e], dw[c][e]);
-        db[c][e] += d;
+        dw[c][e] = fmaf(dy[e], xhat[c][e], dw[c][e]);
+        db[c][e] += dy[e];
       }
     }
-    fetch(r + step);
+    if (!WHOLE) __syncwarp();   // the slots are free again
     group_sum(sum);
-    const float m0 = sum[0] * a.inv_dim, m1 = sum[1] * a.inv_dim;
-    C dx[CHUNKS];
+    // dx = rstd * (g - m0 - xhat * m1)
+    const float r0 = rstd * (sum[0] * a.inv_dim), m1 = sum[1] * a.inv_dim;
+    uint4 dx[CHUNKS];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
+      float f[kElems];
 #pragma unroll
-      for (int e = 0; e < kElems; ++e) {
-        dx[c].set(e, row_rstd * (fmaf(-m1, xhat[c][e], g[c][e]) - m0));
-      }
+      for (int e = 0; e < kElems; ++e) f[e] = fmaf(rstd, fmaf(-m1, xhat[c][e], g[c][e]), -r0);
+      dx[c] = pack<T>(f);
     }
-    store_row<T, CHUNKS, WHOLE>(
-        r < a.n ? static_cast<uint8_t*>(a.dx) + r * a.dx_stride : nullptr, row_bytes, chunks, map, dx);
+    store_row<T, CHUNKS, WHOLE, WIDE>(r < n ? static_cast<uint8_t*>(a.dx) + r * a.dx_stride : nullptr,
+                                      row_bytes, chunks, map, dx);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
+  copies_wait<0>();
   // the sums of the block's groups: those of one warp by exchange, the others
   // one after the other
-  const uint32_t copies = group < 32u ? kBackwardBlock / 32 : groups;
+  const uint32_t copies = group < 32u ? kPipeBlock / 32 : groups;
   const uint32_t copy = group < 32u ? threadIdx.x >> 5 : threadIdx.x / group;
   for (uint32_t d = 16; d >= group; d >>= 1) {
 #pragma unroll
@@ -404,7 +590,7 @@ __global__ void __launch_bounds__(kBackwardBlock, 1)
     }
     __syncthreads();
     float* mine = sums + (uint64_t(which) * gridDim.x + blockIdx.x) * dim;
-    for (uint32_t i = threadIdx.x; i < dim; i += kBackwardBlock) {
+    for (uint32_t i = threadIdx.x; i < dim; i += kPipeBlock) {
       float v = columns[i];
       for (uint32_t k = 1; k < copies; ++k) v += columns[k * dim + i];
       mine[i] = v;
@@ -418,7 +604,7 @@ template <typename T>
 __global__ void __launch_bounds__(512)
     norm_backward_long_kernel(const NormBackwardArgs a) {
   __shared__ float scratch[16][2][2];
-  GroupSum<2> group_sum(blockDim.x, scratch);
+  GroupSum<2, true> group_sum(blockDim.x, scratch);
   const uint32_t dim = uint32_t(a.dim);
   for (uint64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
     const T* x = reinterpret_cast<const T*>(static_cast<const uint8_t*>(a.x) + r * a.x_stride);
@@ -428,7 +614,7 @@ __global__ void __launch_bounds__(512)
     float sum[2] = {0.f, 0.f};
     for (uint32_t i = threadIdx.x; i < dim; i += blockDim.x) {
       float w[1];
-      load_params<T, false>(a.weight, a.params_f32, i, dim, 1.f, w);
+      load_params<T>(a.weight, a.params_f32, false, i, dim, 1.f, w);
       const float g = to_float(dy[i]) * w[0];
       sum[0] += g;
       sum[1] = fmaf(g, (to_float(x[i]) - mean) * rstd, sum[1]);
@@ -437,7 +623,7 @@ __global__ void __launch_bounds__(512)
     const float m0 = sum[0] * a.inv_dim, m1 = sum[1] * a.inv_dim;
     for (uint32_t i = threadIdx.x; i < dim; i += blockDim.x) {
       float w[1];
-      load_params<T, false>(a.weight, a.params_f32, i, dim, 1.f, w);
+      load_params<T>(a.weight, a.params_f32, false, i, dim, 1.f, w);
       const float xhat = (to_float(x[i]) - mean) * rstd;
       dx[i] = from_float<T>(rstd * (fmaf(-m1, xhat, to_float(dy[i]) * w[0]) - m0));
     }
@@ -504,40 +690,71 @@ uint32_t pow2_at_least(uint64_t v) {
 // Chunks of a row; the last one may be part of one.
 uint64_t chunks_of(uint64_t row_bytes) { return (row_bytes + 15) / 16; }
 
-// Parameters are read in chunks where the rows are: their addresses count too.
-uint64_t param_bits(const void* weight, const void* bias) {
-  return address_bits(weight) | address_bits(bias);
+// A kernel that needs more shared memory than the default.
+template <typename Kernel>
+int allow_shared(Kernel kernel, size_t bytes) {
+  if (bytes <= 40 * 1024) return HKV_OK;   // the kernels' static part comes on top
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  if (e == cudaSuccess) return HKV_OK;
+  cudaGetLastError();
+  return rows_fail(HKV_ERR_CUDA, cudaGetErrorString(e));
 }
 
-constexpr uint32_t kMaxGroup = 1024;
+template <typename T, bool WHOLE, bool WIDE>
+int launch_norm_pipe(const NormArgs& a, uint32_t group, uint32_t chunks, const RowsIn& in,
+                     cudaStream_t stream) {
+  auto kernel = norm_pipe_kernel<T, 4, WHOLE, WIDE>;
+  const size_t shared = size_t(kStages) * (kPipeBlock / 32) *
+                        RowQueue<T, 4, WHOLE, WIDE>::slots_per_warp(group < 32 ? group : 32) * 16;
+  const int rc = allow_shared(kernel, shared);
+  if (rc != HKV_OK) return rc;
+  const uint64_t want = (a.n * group + kPipeBlock - 1) / kPipeBlock, cap = uint64_t(sm_count());
+  kernel<<<unsigned(want < cap ? want : cap), kPipeBlock, shared, stream>>>(a, group, chunks, in);
+  return HKV_OK;
+}
+
+template <typename T, int CHUNKS>
+void launch_norm_few(const NormArgs& a, bool whole, uint32_t group, uint32_t chunks, const RowsIn& in,
+                     cudaStream_t stream) {
+  const uint32_t block = group > kNormBlock ? group : kNormBlock;
+  const unsigned grid = unsigned((a.n * group + block - 1) / block);
+  auto kernel = group >= 32 ? (whole ? norm_kernel<T, CHUNKS, true, true> : norm_kernel<T, CHUNKS, false, true>)
+                            : (whole ? norm_kernel<T, CHUNKS, true, false> : norm_kernel<T, CHUNKS, false, false>);
+  kernel<<<grid, block, 0, stream>>>(a, group, chunks, in);
+}
+
+// Threads on a row that hold `per_thread` chunks each.  Two at least: they share a
+// sector of 32 bytes, and a queue for rows of single threads would not fit.
+uint32_t group_for(uint64_t chunks, uint32_t per_thread) {
+  const uint32_t group = pow2_at_least((chunks + per_thread - 1) / per_thread);
+  return group < 2 ? 2 : group;
+}
 
 template <typename T>
-void launch_norm_type(const NormArgs& a, bool whole, cudaStream_t stream) {
+int launch_norm_type(const NormArgs& a, bool whole, cudaStream_t stream) {
   const uint64_t chunks = chunks_of(a.dim * sizeof(T));
-  if (chunks > 4ull * kMaxGroup) {
+  if (chunks > 4ull * kPipeBlock) {
     const uint64_t cap = uint64_t(sm_count()) * 2;
-    norm_long_kernel<T><<<unsigned(a.n < cap ? a.n : cap), kMaxGroup, 0, stream>>>(a);
-    return;
+    norm_long_kernel<T><<<unsigned(a.n < cap ? a.n : cap), 1024, 0, stream>>>(a);
+    return HKV_OK;
   }
-  // four chunks per thread where the row has them, fewer where there are too
-  // few rows to fill the device with that
-  const uint64_t enough = uint64_t(sm_count()) * 512;
-  uint32_t per_thread = 4, group = pow2_at_least((chunks + 3) / 4);
-  while (per_thread > 1 && group < kMaxGroup &&
-         (a.n * group < enough || pow2_at_least(chunks) <= 2)) {
-    per_thread >>= 1;
-    group = pow2_at_least((chunks + per_thread - 1) / per_thread);
-  }
-  const uint32_t block = group > kNormBlock ? group : kNormBlock;
-  const uint64_t grid = (a.n * group + block - 1) / block;
   const RowsIn in = a.row_ptrs != nullptr ? RowsIn{} : rows_in(a.x, a.n, a.x_stride, a.dim * sizeof(T));
-  auto kernel = whole ? (per_thread == 1   ? norm_kernel<T, 1, true>
-                         : per_thread == 2 ? norm_kernel<T, 2, true>
-                                           : norm_kernel<T, 4, true>)
-                      : (per_thread == 1   ? norm_kernel<T, 1, false>
-                         : per_thread == 2 ? norm_kernel<T, 2, false>
-                                           : norm_kernel<T, 4, false>);
-  kernel<<<unsigned(grid), block, 0, stream>>>(a, group, uint32_t(chunks), in);
+  const uint32_t count = uint32_t(chunks);
+  uint32_t group = group_for(chunks, 4);
+  // more than two rows for every group that the device holds: they are worth a queue
+  if (a.n * group > uint64_t(sm_count()) * kPipeBlock * 2) {
+    if (group >= 32) {
+      return whole ? launch_norm_pipe<T, true, true>(a, group, count, in, stream)
+                   : launch_norm_pipe<T, false, true>(a, group, count, in, stream);
+    }
+    return whole ? launch_norm_pipe<T, true, false>(a, group, count, in, stream)
+                 : launch_norm_pipe<T, false, false>(a, group, count, in, stream);
+  }
+  // few: as many threads on a row as it has chunks for
+  if (chunks > 1024) launch_norm_few<T, 2>(a, whole, group_for(chunks, 2), count, in, stream);
+  else launch_norm_few<T, 1>(a, whole, group_for(chunks, 1), count, in, stream);
+  return HKV_OK;
 }
 
 // Chunks a thread of the backward kernel holds: 16 elements' column sums, row
@@ -548,30 +765,48 @@ NormBackwardPlan plan_backward(uint64_t n, uint64_t dim, uint32_t size) {
   NormBackwardPlan p{};
   const uint64_t chunks = chunks_of(dim * size);
   p.per_thread = backward_chunks(size);
-  p.fits = chunks <= uint64_t(kBackwardBlock) * p.per_thread;
+  p.fits = chunks <= uint64_t(kPipeBlock) * p.per_thread;
   if (!p.fits) {
     p.blocks = uint32_t(n < 64 ? n : 64);   // row splits of the column sums
     return p;
   }
   p.chunks = uint32_t(chunks);
-  p.group = pow2_at_least((chunks + p.per_thread - 1) / p.per_thread);
-  const uint64_t groups = kBackwardBlock / p.group;
+  p.group = group_for(chunks, p.per_thread);
+  const uint64_t groups = kPipeBlock / p.group;
   const uint64_t want = (n + groups - 1) / groups;
   const uint64_t cap = uint64_t(sm_count());
   p.blocks = uint32_t(want < cap ? want : cap);
   return p;
 }
 
-template <typename T>
-void launch_backward_type(const NormBackwardArgs& a, const NormBackwardPlan& p, bool whole, float* sums,
-                          cudaStream_t stream) {
+template <typename T, bool WHOLE, bool WIDE>
+int launch_backward_pipe(const NormBackwardArgs& a, const NormBackwardPlan& p, float* sums,
+                         cudaStream_t stream) {
   constexpr int kChunks = backward_chunks(sizeof(T));
   const uint64_t row_bytes = a.dim * sizeof(T);
-  const uint32_t copies = p.group < 32 ? kBackwardBlock / 32 : kBackwardBlock / p.group;
-  auto kernel = whole ? norm_backward_kernel<T, kChunks, true> : norm_backward_kernel<T, kChunks, false>;
-  kernel<<<p.blocks, kBackwardBlock, copies * a.dim * sizeof(float), stream>>>(
+  const size_t copies = p.group < 32 ? kPipeBlock / 32 : kPipeBlock / p.group;
+  const size_t queue = size_t(kStages) * 2 * (kPipeBlock / 32) * 16 *
+                       RowQueue<T, kChunks, WHOLE, WIDE>::slots_per_warp(p.group < 32 ? p.group : 32);
+  const size_t columns = copies * a.dim * sizeof(float);
+  const size_t shared = queue > columns ? queue : columns;
+  auto kernel = norm_backward_kernel<T, kChunks, WHOLE, WIDE>;
+  const int rc = allow_shared(kernel, shared);
+  if (rc != HKV_OK) return rc;
+  kernel<<<p.blocks, kPipeBlock, shared, stream>>>(
       a, p.group, p.chunks, rows_in(a.x, a.n, a.x_stride, row_bytes),
       rows_in(a.dy, a.n, a.dy_stride, row_bytes), sums);
+  return HKV_OK;
+}
+
+template <typename T>
+int launch_backward_type(const NormBackwardArgs& a, const NormBackwardPlan& p, bool whole, float* sums,
+                         cudaStream_t stream) {
+  if (p.group >= 32) {
+    return whole ? launch_backward_pipe<T, true, true>(a, p, sums, stream)
+                 : launch_backward_pipe<T, false, true>(a, p, sums, stream);
+  }
+  return whole ? launch_backward_pipe<T, true, false>(a, p, sums, stream)
+               : launch_backward_pipe<T, false, false>(a, p, sums, stream);
 }
 
 template <typename T>
@@ -612,11 +847,11 @@ int launch_norm(const NormArgs& args, uint32_t value_kind, cudaStream_t stream) 
   // multiples of the widest access their length allows
   if (args.row_ptrs == nullptr) bits |= address_bits(args.x) | args.x_stride;
   HKV_ROWS_CHECK(bits % size == 0, "a row does not start at a multiple of its element size");
-  const bool whole = whole_chunks(bits | param_bits(args.weight, args.bias));
-  if (value_kind == kValueF32) launch_norm_type<float>(args, whole, stream);
-  else if (value_kind == kValueF16) launch_norm_type<__half>(args, whole, stream);
-  else launch_norm_type<__nv_bfloat16>(args, whole, stream);
-  return rows_launched();
+  const bool whole = whole_chunks(bits);
+  const int rc = value_kind == kValueF32   ? launch_norm_type<float>(args, whole, stream)
+                 : value_kind == kValueF16 ? launch_norm_type<__half>(args, whole, stream)
+                                           : launch_norm_type<__nv_bfloat16>(args, whole, stream);
+  return rc != HKV_OK ? rc : rows_launched();
 }
 
 }  // namespace hkv
@@ -641,6 +876,7 @@ int hkv_layer_norm(uint64_t n, uint64_t dim, uint32_t value_kind, const void* x,
   a.weight = weight;
   a.bias = bias;
   a.params_f32 = param_kind == kValueF32;
+  a.params_vec = whole_chunks(address_bits(weight) | address_bits(bias));
   a.eps = eps;
   a.inv_dim = 1.f / float(dim);
   a.y = y;
@@ -665,6 +901,7 @@ int hkv_layer_norm_ptr(uint64_t n, uint64_t dim, uint32_t value_kind, const void
   a.weight = weight;
   a.bias = bias;
   a.params_f32 = param_kind == kValueF32;
+  a.params_vec = whole_chunks(address_bits(weight) | address_bits(bias));
   a.eps = eps;
   a.inv_dim = 1.f / float(dim);
   a.y = y;
@@ -712,6 +949,7 @@ int hkv_layer_norm_backward(uint64_t n, uint64_t dim, uint32_t value_kind, const
   a.dy_stride = dy_stride;
   a.weight = weight;
   a.params_f32 = param_kind == kValueF32;
+  a.params_vec = whole_chunks(address_bits(weight));
   a.inv_dim = 1.f / float(dim);
   a.mean = mean;
   a.rstd = rstd;
@@ -722,13 +960,16 @@ int hkv_layer_norm_backward(uint64_t n, uint64_t dim, uint32_t value_kind, const
   const uint64_t bits = dim * size | address_bits(dy) | dy_stride | address_bits(x) | x_stride |
                         address_bits(dx) | dx_stride;
   HKV_ROWS_CHECK(bits % size == 0, "a row does not start at a multiple of its element size");
-  const bool whole = whole_chunks(bits | param_bits(weight, nullptr));
+  const bool whole = whole_chunks(bits);
   const NormBackwardPlan p = plan_backward(n, dim, size);
   float* sums = sums_wanted ? static_cast<float*>(work) : nullptr;
   if (p.fits) {
-    if (value_kind == kValueF32) launch_backward_type<float>(a, p, whole, sums, s);
-    else if (value_kind == kValueF16) launch_backward_type<__half>(a, p, whole, sums, s);
-    else launch_backward_type<__nv_bfloat16>(a, p, whole, sums, s);
+#define HKV_CALL(T) launch_backward_type<T>(a, p, whole, sums, s)
+    const int launched = value_kind == kValueF32   ? HKV_CALL(float)
+                         : value_kind == kValueF16 ? HKV_CALL(__half)
+                                                   : HKV_CALL(__nv_bfloat16);
+#undef HKV_CALL
+    if (launched != HKV_OK) return launched;
   } else if (value_kind == kValueF32) {
     launch_backward_long<float>(a, p, sums, s);
   } else if (value_kind == kValueF16) {

@@ -16,6 +16,7 @@ struct NormArgs {
   const void* weight = nullptr;            // null: ones
   const void* bias = nullptr;              // null: zeros
   bool params_f32 = false;                 // weight and bias are float, else the rows' type
+  bool params_vec = false;                 // both start at a multiple of 16 bytes
   float eps = 0.f;
   float inv_dim = 1.f;
   void* y = nullptr;
@@ -33,6 +34,7 @@ struct NormBackwardArgs {
   uint64_t x_stride = 0;
   const void* weight = nullptr;
   bool params_f32 = false;
+  bool params_vec = false;
   float inv_dim = 1.f;
   const float* mean = nullptr;
   const float* rstd = nullptr;

@@ -45,16 +45,62 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
 // unaligned address is cut out of the two aligned ones it touches.
 
 template <typename T>
-struct Chunk {
-  static constexpr int kElems = 16 / int(sizeof(T));
-  union {
-    uint4 raw;
-    T elem[kElems];
-  };
-  __device__ __forceinline__ Chunk() {}
-  __device__ __forceinline__ float get(int i) const { return to_float(elem[i]); }
-  __device__ __forceinline__ void set(int i, float v) { elem[i] = from_float<T>(v); }
-};
+constexpr int kChunkElems = 16 / int(sizeof(T));
+
+// A chunk's elements as floats, and back with one rounding each.
+__device__ __forceinline__ void unpack(const uint4& v, float (&f)[4], const float*) {
+  f[0] = __uint_as_float(v.x);
+  f[1] = __uint_as_float(v.y);
+  f[2] = __uint_as_float(v.z);
+  f[3] = __uint_as_float(v.w);
+}
+__device__ __forceinline__ void unpack(const uint4& v, float (&f)[8], const __half*) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    f[2 * i] = two.x;
+    f[2 * i + 1] = two.y;
+  }
+}
+__device__ __forceinline__ void unpack(const uint4& v, float (&f)[8], const __nv_bfloat16*) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {   // a bfloat16 is the upper half of its float
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& v, float (&f)[kChunkElems<T>]) {
+  unpack(v, f, static_cast<const T*>(nullptr));
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[4], const float*) {
+  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                    __float_as_uint(f[3]));
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[8], const __half*) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 two = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&two);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[8], const __nv_bfloat16*) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 two = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&two);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float (&f)[kChunkElems<T>]) {
+  return pack(f, static_cast<const T*>(nullptr));
+}
 
 // A matrix of rows: base, distance and count of the rows in bytes; every row
 // that is read lies in [first, last).
@@ -81,37 +127,54 @@ __device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, uint3
                     __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
 }
 
-// An element of G bytes of a chunk, for the ends of rows.
+// The 16 bytes at p, those inside [from, to) element by element (of G bytes) and
+// zeros for the others.
 template <int G>
-__device__ __forceinline__ void put_piece(uint4& v, int at, const uint8_t* from) {
-  *reinterpret_cast<typename VecType<G>::type*>(reinterpret_cast<uint8_t*>(&v) + at) =
-      *reinterpret_cast<const typename VecType<G>::type*>(from);
+__device__ __forceinline__ uint4 pieces(const uint8_t* p, const uint8_t* from, const uint8_t* to) {
+  uint64_t half[2] = {0, 0};
+#pragma unroll 1
+  for (int b = 0; b < 16; b += G) {
+    if (p + b < from || p + b >= to) continue;
+    uint64_t piece;
+    if constexpr (G == 8) piece = *reinterpret_cast<const uint64_t*>(p + b);
+    else piece = *reinterpret_cast<const typename VecType<G>::type*>(p + b);
+    half[0] |= b < 8 ? piece << (8 * b) : 0;
+    half[1] |= b < 8 ? 0 : piece << (8 * (b - 8));
+  }
+  return make_uint4(uint32_t(half[0]), uint32_t(half[0] >> 32), uint32_t(half[1]),
+                    uint32_t(half[1] >> 32));
 }
 
-// The 16 bytes at p, of which those inside [from, to) matter (the others are
-// anything).  Aligned chunks are read whole where they lie inside the matrix,
-// element by element (of G bytes) at its ends: nothing outside it is touched.
-template <int G>
-__device__ __forceinline__ uint4 load_chunk(const uint8_t* p, const uint8_t* from,
-                                            const uint8_t* to, const uint8_t* first,
-                                            const uint8_t* last) {
-  const uint32_t s = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
-  const uint8_t* a = p - s;
-  const bool need_lo = from < a + 16;
-  const bool need_hi = s != 0 && to > a + 16;
-  if ((need_lo && (a < first || a + 16 > last)) || (need_hi && (a + 16 < first || a + 32 > last))) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int b = 0; b < 16; b += G) {
-      if (p + b >= from && p + b < to) put_piece<G>(v, b, p + b);
-    }
-    return v;
+// The 16 bytes at an address p of any alignment, of which those inside a row
+// [from, to) matter (the others are anything).  The aligned chunks that hold them
+// are read whole where they lie inside the matrix [first, last), and element by
+// element (of G bytes) at its ends: nothing outside it is touched.  Loading and
+// cutting are two steps, without a branch in the first, so that the loads of
+// several chunks are in flight together.
+struct Cut {
+  uint4 lo, hi;
+  uint32_t s;
+  bool inside;
+
+  __device__ __forceinline__ void load(const uint8_t* p, const uint8_t* first, const uint8_t* last) {
+    s = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
+    const uint8_t* a = p - s;
+    inside = a >= first && a + (s ? 32 : 16) <= last;
+    lo = hi = make_uint4(0, 0, 0, 0);
+    if (inside) lo = __ldg(reinterpret_cast<const uint4*>(a));
+    if (inside && s) hi = __ldg(reinterpret_cast<const uint4*>(a + 16));
   }
-  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-  if (need_lo) lo = __ldg(reinterpret_cast<const uint4*>(a));
-  if (need_hi) hi = __ldg(reinterpret_cast<const uint4*>(a + 16));
-  return s == 0 ? lo : shifted(lo, hi, s);
-}
+  __device__ __forceinline__ void none() {
+    lo = hi = make_uint4(0, 0, 0, 0);
+    s = 0;
+    inside = true;
+  }
+  template <int G>
+  __device__ __forceinline__ uint4 get(const uint8_t* p, const uint8_t* from, const uint8_t* to) const {
+    if (inside) return s == 0 ? lo : shifted(lo, hi, s);
+    return pieces<G>(p, from, to);
+  }
+};
 
 // Stores the bytes of v (for the aligned address q) that lie inside [from, to).
 template <int G>
@@ -139,6 +202,15 @@ inline uint32_t piece_bytes(uint64_t bits) {
   uint32_t v = 8;
   while (v > 1 && (bits & (v - 1)) != 0) v >>= 1;
   return v;
+}
+
+__device__ __forceinline__ void copy_async(uint32_t shared, const uint8_t* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 int rows_fail(int code, const char* message) noexcept;

@@ -16,7 +16,6 @@ step, as accum_or_assign is.
 """
 from __future__ import annotations
 
-import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -24,6 +23,14 @@ import torch
 from .table import _VALUE_KINDS, CudaException, load_library
 
 _ROW_KINDS = {t: _VALUE_KINDS[t] for t in (torch.float32, torch.float16, torch.bfloat16)}
+_F32 = torch.float32
+
+# The host's part of a call is most of its time on a decoding step's few rows,
+# so it asks torch for as little as it can: the raw handle of the current stream
+# costs 0.1 us where the stream object costs 2.3 us, empty_like 1.4 us where
+# empty with a shape, type and device costs 2.4 us.
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 class ExpertOrder(NamedTuple):
@@ -35,103 +42,120 @@ class ExpertOrder(NamedTuple):
     source: torch.Tensor     # int32 [tokens * top_k]: the assignment of each row, -1 behind the last
 
 
-def _chk(lib, rc: int) -> None:
-    if rc:
-        msg = (lib.hkv_rows_last_error() or b"").decode()
-        if rc == 2:
-            raise CudaException(msg)
-        raise ValueError(msg) if rc == 4 else RuntimeError(msg)
+def _fail(lib, rc: int) -> None:
+    msg = (lib.hkv_rows_last_error() or b"").decode()
+    if rc == 2:
+        raise CudaException(msg)
+    raise ValueError(msg) if rc == 4 else RuntimeError(msg)
 
 
-def _on_stream(fn):
-    """Runs a call whose first tensor is on another device than the current one,
-    or that names a stream, with that device and stream as the current ones, so
-    that what it allocates belongs to them."""
-
-    @functools.wraps(fn)
-    def call(*args, stream=None, **kwargs):
-        first = next((a for a in (*args, *kwargs.values()) if isinstance(a, torch.Tensor)), None)
-        dev = first.device if first is not None else None
-        if dev is None or dev.type != "cuda" or (stream is None and dev.index == torch.cuda.current_device()):
-            return fn(*args, **kwargs)   # not on a GPU: the call itself refuses
-        with torch.cuda.device(dev):
-            if stream is None:
-                stream = torch.cuda.current_stream(dev)
-            elif isinstance(stream, int):
-                stream = torch.cuda.ExternalStream(stream, dev) if stream else torch.cuda.default_stream(dev)
-            with torch.cuda.stream(stream):
-                return fn(*args, **kwargs)
-
-    return call
+def _elsewhere(t: torch.Tensor, stream) -> bool:
+    """Whether a call has to change the device or the stream first."""
+    return t.is_cuda and (stream is not None or t.get_device() != _current_device())
 
 
-def _current_stream(t: torch.Tensor) -> Optional[int]:
-    return torch.cuda.current_stream(t.device).cuda_stream or None
+def _run_there(fn, t: torch.Tensor, stream, *args):
+    """Runs fn with the device of t and ``stream`` as the current ones, so that
+    what it allocates belongs to them."""
+    with torch.cuda.device(t.device):
+        if stream is None:
+            return fn(*args)
+        if isinstance(stream, int):
+            stream = torch.cuda.ExternalStream(stream, t.device) if stream else torch.cuda.default_stream(t.device)
+        with torch.cuda.stream(stream):
+            return fn(*args)
 
 
-def _rows(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None, shape=None, typed: bool = True) -> int:
-    """Checks a row matrix; its stride in bytes."""
+def _rows(t: torch.Tensor, name: str):
+    """Checks a row matrix: (rows, columns, distance of the rows in bytes)."""
     if t.dim() != 2:
         raise ValueError(f"{name} must have two dimensions")
     n, dim = t.shape
-    if shape is not None and (n, dim) != tuple(shape):
-        raise ValueError(f"{name} must have the shape {tuple(shape)}")
     if dim < 1:
         raise ValueError(f"{name} has no columns")
-    if dim > 1 and t.stride(1) != 1:
+    stride, step = t.stride()
+    if step != 1 and dim > 1:
         raise ValueError(f"the rows of {name} must be contiguous")
-    if like is None:
-        if typed and t.dtype not in _ROW_KINDS:
-            raise ValueError(f"{name} must be float32, float16 or bfloat16")
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be on a GPU")
-    elif t.dtype != like.dtype or t.device != like.device:
+    # of a single row, what the stride says is of no account
+    return n, dim, (stride if n > 1 else dim) * t.element_size()
+
+
+def _float_rows(t: torch.Tensor, name: str):
+    """_rows of float rows on a GPU, and their kind."""
+    checked = _rows(t, name)
+    kind = _ROW_KINDS.get(t.dtype)
+    if kind is None:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a GPU")
+    return *checked, kind
+
+
+def _more_rows(t: torch.Tensor, name: str, n: int, dim: int, like: torch.Tensor) -> int:
+    """Checks another row matrix of a call; its stride in bytes."""
+    rows, columns, stride = _rows(t, name)
+    if rows != n or columns != dim:
+        raise ValueError(f"{name} must have the shape {(n, dim)}")
+    if t.dtype is not like.dtype or t.get_device() != like.get_device():
         raise ValueError(f"{name} must have the type and device of the other rows")
-    # one row, or rows without a distance: what the stride says is of no account
-    return (t.stride(0) if n > 1 else dim) * t.element_size()
+    return stride
 
 
-def _out(out: Optional[torch.Tensor], shape, like: torch.Tensor, name: str = "out"):
-    """The tensor a row matrix goes to, and its stride in bytes."""
+def _out(out: Optional[torch.Tensor], n: int, dim: int, like: torch.Tensor):
+    """The matrix a result goes to, and its stride in bytes."""
     if out is None:
-        out = torch.empty(shape, dtype=like.dtype, device=like.device)
-        return out, shape[1] * out.element_size()
-    stride = _rows(out, name, like, shape)
-    if stride < shape[1] * out.element_size():
-        raise ValueError(f"the rows of {name} overlap")
+        same = like.shape[0] == n and like.is_contiguous()
+        out = torch.empty_like(like) if same else like.new_empty((n, dim))
+        return out, dim * out.element_size()
+    stride = _more_rows(out, "out", n, dim, like)
+    if stride < dim * out.element_size():
+        raise ValueError("the rows of out overlap")
     return out, stride
 
 
-def _vector(t: Optional[torch.Tensor], name: str, n: int, dtypes, device):
+def _vector(t: Optional[torch.Tensor], name: str, n: int, like: torch.Tensor):
+    """Address of n parameters in the type of the rows `like` or float32."""
     if t is None:
         return None
-    if t.dtype not in dtypes:
-        raise ValueError(f"{name} must be " + " or ".join(str(d) for d in dict.fromkeys(dtypes)))
+    if t.dtype is not _F32 and t.dtype is not like.dtype:
+        raise ValueError(f"{name} must be float32 or have the type of the rows")
     if t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous and have {n} elements")
-    if t.device != device:
+    if t.get_device() != like.get_device():
         raise ValueError(f"{name} must be on the device of the rows")
     return t.data_ptr()
 
 
-def _order(order: ExpertOrder, device):
-    """(tokens, top_k, experts) of an order."""
+def _statistic(t: Optional[torch.Tensor], name: str, n: int, like: torch.Tensor):
+    """Address of the float32 statistics of n rows."""
+    if t is None:
+        return None
+    if t.dtype is not _F32 or t.numel() < n or not t.is_contiguous() or t.get_device() != like.get_device():
+        raise ValueError(f"{name} must be contiguous, on the device of the rows and hold {n} float32 elements")
+    return t.data_ptr()
+
+
+def _order(order: ExpertOrder, like: torch.Tensor):
+    """(tokens, top_k, experts, addresses of offsets and position) of an order."""
     offsets, position = order[0], order[1]
-    if position.dim() != 2 or position.dtype != torch.int32 or not position.is_contiguous():
+    if position.dim() != 2 or position.dtype is not torch.int32 or not position.is_contiguous():
         raise ValueError("order.position must be a contiguous int32 matrix [tokens, top_k]")
-    if offsets.dim() != 1 or offsets.dtype != torch.int32 or not offsets.is_contiguous():
+    if offsets.dim() != 1 or offsets.dtype is not torch.int32 or not offsets.is_contiguous():
         raise ValueError("order.offsets must be a contiguous int32 vector [experts + 1]")
-    if position.device != device or offsets.device != device:
+    dev = like.get_device()
+    if position.get_device() != dev or offsets.get_device() != dev:
         raise ValueError("the order must be on the device of the rows")
-    return position.shape[0], position.shape[1], offsets.numel() - 1
+    tokens, top_k = position.shape
+    return tokens, top_k, offsets.shape[0] - 1, offsets.data_ptr(), position.data_ptr()
 
 
-@_on_stream
-def expert_sort(expert_ids: torch.Tensor, num_experts: int) -> ExpertOrder:
+def expert_sort(expert_ids: torch.Tensor, num_experts: int, stream=None) -> ExpertOrder:
     """Sorts token assignments by expert.  ``expert_ids``: int32 or int64
     [tokens, top_k]; an id outside [0, num_experts) drops its assignment.  The
     sort is stable: an expert's rows keep the order of the assignments."""
-    if expert_ids.dim() != 2 or expert_ids.dtype not in (torch.int32, torch.int64):
+    if _elsewhere(expert_ids, stream):
+        return _run_there(expert_sort, expert_ids, stream, expert_ids, num_experts)
+    if expert_ids.dim() != 2 or expert_ids.dtype not in (torch.int64, torch.int32):
         raise ValueError("expert_ids must be an int32 or int64 matrix [tokens, top_k]")
     if not expert_ids.is_contiguous():
         raise ValueError("expert_ids must be contiguous")
@@ -143,185 +167,201 @@ def expert_sort(expert_ids: torch.Tensor, num_experts: int) -> ExpertOrder:
     if not expert_ids.is_cuda:
         raise ValueError("expert_ids must be on a GPU")
     lib = load_library()
-    dev = expert_ids.device
-    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
-    position = torch.empty((tokens, top_k), dtype=torch.int32, device=dev)
-    source = torch.empty(tokens * top_k, dtype=torch.int32, device=dev)
+    n = tokens * top_k
+    position = torch.empty_like(expert_ids, dtype=torch.int32)
+    source = expert_ids.new_empty(n, dtype=torch.int32)
+    offsets = expert_ids.new_empty(num_experts + 1, dtype=torch.int32)
     work_bytes = lib.hkv_expert_sort_workspace_bytes(tokens, top_k, num_experts)
-    work = torch.empty(work_bytes, dtype=torch.uint8, device=dev) if work_bytes else None
-    _chk(lib, lib.hkv_expert_sort(
+    work = expert_ids.new_empty(work_bytes, dtype=torch.uint8) if work_bytes else None
+    rc = lib.hkv_expert_sort(
         tokens, top_k, expert_ids.data_ptr(), expert_ids.element_size(), num_experts,
         offsets.data_ptr(), position.data_ptr(), source.data_ptr(),
-        work.data_ptr() if work is not None else None, work_bytes, _current_stream(expert_ids)))
+        work.data_ptr() if work_bytes else None, work_bytes, _raw_stream(expert_ids.get_device()))
+    if rc:
+        _fail(lib, rc)
     return ExpertOrder(offsets, position, source)
 
 
-@_on_stream
-def expert_dispatch(x: torch.Tensor, order: ExpertOrder, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+def expert_dispatch(x: torch.Tensor, order: ExpertOrder, out: Optional[torch.Tensor] = None,
+                    stream=None) -> torch.Tensor:
     """Copies of the token rows in the order of the experts: [tokens * top_k, dim]
     with row ``order.position[t, j]`` = x[t].  Rows behind the last expert's are
     zeros in a new tensor and left as they are in ``out``.  Any element type."""
-    x_stride = _rows(x, "x", typed=False)
-    tokens, top_k, experts = _order(order, x.device)
-    if x.shape[0] != tokens:
+    if _elsewhere(x, stream):
+        return _run_there(expert_dispatch, x, stream, x, order, out)
+    n, dim, x_stride = _rows(x, "x")
+    if not x.is_cuda:
+        raise ValueError("x must be on a GPU")
+    tokens, top_k, experts, offsets, position = _order(order, x)
+    if n != tokens:
         raise ValueError("x must have a row for every token of the order")
     new = out is None
-    out, out_stride = _out(out, (tokens * top_k, x.shape[1]), x)
+    out, out_stride = _out(out, tokens * top_k, dim, x)
     lib = load_library()
-    _chk(lib, lib.hkv_expert_dispatch(
-        tokens, top_k, x.shape[1] * x.element_size(), x.data_ptr(), x_stride, experts,
-        order[0].data_ptr(), order[1].data_ptr(), out.data_ptr(), out_stride, int(new),
-        _current_stream(x)))
+    rc = lib.hkv_expert_dispatch(
+        tokens, top_k, dim * x.element_size(), x.data_ptr(), x_stride, experts, offsets, position,
+        out.data_ptr(), out_stride, new, _raw_stream(x.get_device()))
+    if rc:
+        _fail(lib, rc)
     return out
 
 
 def _combine(rows, weights, order, out):
-    stride = _rows(rows, "rows")
-    tokens, top_k, _ = _order(order, rows.device)
-    if rows.shape[0] != tokens * top_k:
+    n, dim, stride, kind = _float_rows(rows, "rows")
+    tokens, top_k, _, _, position = _order(order, rows)
+    if n != tokens * top_k:
         raise ValueError("rows must have a row for every assignment of the order")
-    kind = _ROW_KINDS[rows.dtype]
-    w = _vector(weights, "weights", tokens * top_k, (rows.dtype, torch.float32), rows.device)
-    out, out_stride = _out(out, (tokens, rows.shape[1]), rows)
+    w = _vector(weights, "weights", n, rows)
+    out, out_stride = _out(out, tokens, dim, rows)
     lib = load_library()
-    _chk(lib, lib.hkv_expert_combine(
-        tokens, top_k, rows.shape[1], kind, rows.data_ptr(), stride, w,
-        kind if weights is None else _ROW_KINDS[weights.dtype], order[1].data_ptr(), out.data_ptr(),
-        out_stride, _current_stream(rows)))
+    rc = lib.hkv_expert_combine(
+        tokens, top_k, dim, kind, rows.data_ptr(), stride, w,
+        kind if weights is None else _ROW_KINDS[weights.dtype], position, out.data_ptr(), out_stride,
+        _raw_stream(rows.get_device()))
+    if rc:
+        _fail(lib, rc)
     return out
 
 
-@_on_stream
 def expert_dispatch_backward(d_rows: torch.Tensor, order: ExpertOrder,
-                             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                             out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """Gradient of expert_dispatch: every token sums the gradients of its copies
     [tokens, dim].  Rows behind the last expert's are not read."""
+    if _elsewhere(d_rows, stream):
+        return _run_there(_combine, d_rows, stream, d_rows, None, order, out)
     return _combine(d_rows, None, order, out)
 
 
-@_on_stream
 def expert_combine(rows: torch.Tensor, weights: torch.Tensor, order: ExpertOrder,
-                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """The experts' rows back in token order: out[t] is the sum over j of
     weights[t, j] * rows[order.position[t, j]].  Dropped assignments add nothing,
     whatever their weight; a token without any gets zeros."""
+    if _elsewhere(rows, stream):
+        return _run_there(_combine, rows, stream, rows, weights, order, out)
     return _combine(rows, weights, order, out)
 
 
-@_on_stream
 def expert_combine_backward(d_out: torch.Tensor, rows: torch.Tensor, weights: torch.Tensor,
-                            order: ExpertOrder, out: Optional[torch.Tensor] = None):
+                            order: ExpertOrder, out: Optional[torch.Tensor] = None, stream=None):
     """Gradients of expert_combine: (d_rows, d_weights).  The rows of d_rows
     behind the last expert's are zeros in a new tensor and left as they are in
     ``out``; the weights of dropped assignments get 0."""
-    d_stride = _rows(d_out, "d_out")
-    tokens, top_k, experts = _order(order, d_out.device)
-    if d_out.shape[0] != tokens:
+    if _elsewhere(d_out, stream):
+        return _run_there(expert_combine_backward, d_out, stream, d_out, rows, weights, order, out)
+    n, dim, d_stride, kind = _float_rows(d_out, "d_out")
+    tokens, top_k, experts, offsets, position = _order(order, d_out)
+    if n != tokens:
         raise ValueError("d_out must have a row for every token of the order")
-    dim = d_out.shape[1]
-    stride = _rows(rows, "rows", d_out, (tokens * top_k, dim))
-    w = _vector(weights, "weights", tokens * top_k, (rows.dtype, torch.float32), d_out.device)
+    stride = _more_rows(rows, "rows", tokens * top_k, dim, d_out)
+    w = _vector(weights, "weights", tokens * top_k, rows)
     new = out is None
-    out, out_stride = _out(out, (tokens * top_k, dim), d_out)
-    d_weights = torch.empty((tokens, top_k), dtype=weights.dtype, device=d_out.device)
+    out, out_stride = _out(out, tokens * top_k, dim, rows)
+    d_weights = weights.new_empty((tokens, top_k))
     lib = load_library()
-    _chk(lib, lib.hkv_expert_combine_backward(
-        tokens, top_k, dim, _ROW_KINDS[rows.dtype], d_out.data_ptr(), d_stride, rows.data_ptr(),
-        stride, w, _ROW_KINDS[weights.dtype], experts, order[0].data_ptr(), order[1].data_ptr(),
-        out.data_ptr(), out_stride, int(new), d_weights.data_ptr(), _current_stream(d_out)))
+    rc = lib.hkv_expert_combine_backward(
+        tokens, top_k, dim, kind, d_out.data_ptr(), d_stride, rows.data_ptr(), stride, w,
+        _ROW_KINDS[weights.dtype], experts, offsets, position, out.data_ptr(), out_stride, new,
+        d_weights.data_ptr(), _raw_stream(d_out.get_device()))
+    if rc:
+        _fail(lib, rc)
     return out, d_weights
 
 
-def _params(weight, bias, dim, dtype, device):
+def _params(weight, bias, dim, like):
     """Addresses of weight and bias and their kind."""
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+    w = _vector(weight, "weight", dim, like)
+    b = _vector(bias, "bias", dim, like)
+    if weight is None:
+        return w, b, _ROW_KINDS[like.dtype if bias is None else bias.dtype]
+    if bias is not None and weight.dtype is not bias.dtype:
         raise ValueError("weight and bias must have one type")
-    w = _vector(weight, "weight", dim, (dtype, torch.float32), device)
-    b = _vector(bias, "bias", dim, (dtype, torch.float32), device)
-    given = weight if weight is not None else bias
-    return w, b, _ROW_KINDS[dtype if given is None else given.dtype]
+    return w, b, _ROW_KINDS[weight.dtype]
 
 
-@_on_stream
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                bias: Optional[torch.Tensor] = None, eps: float = 1e-5, stats: bool = True,
-               out: Optional[torch.Tensor] = None):
+               out: Optional[torch.Tensor] = None, stream=None):
     """Layer norm of every row of x [n, dim].  Returns (y, mean, rstd), the
     statistics (float32 [n]) being what layer_norm_backward needs, or y alone
     with ``stats=False``."""
-    stride = _rows(x, "x")
-    n, dim = x.shape
-    w, b, kind = _params(weight, bias, dim, x.dtype, x.device)
-    y, y_stride = _out(out, (n, dim), x)
+    if _elsewhere(x, stream):
+        return _run_there(layer_norm, x, stream, x, weight, bias, eps, stats, out)
+    n, dim, stride, kind = _float_rows(x, "x")
+    w, b, param_kind = _params(weight, bias, dim, x)
+    y, y_stride = _out(out, n, dim, x)
     mean = rstd = None
     if stats:
-        mean = torch.empty(n, dtype=torch.float32, device=x.device)
-        rstd = torch.empty(n, dtype=torch.float32, device=x.device)
+        mean, rstd = x.new_empty(n, dtype=_F32), x.new_empty(n, dtype=_F32)
     lib = load_library()
-    _chk(lib, lib.hkv_layer_norm(
-        n, dim, _ROW_KINDS[x.dtype], x.data_ptr(), stride, w, b, kind, eps, y.data_ptr(), y_stride,
-        mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None, _current_stream(x)))
+    rc = lib.hkv_layer_norm(
+        n, dim, kind, x.data_ptr(), stride, w, b, param_kind, eps, y.data_ptr(), y_stride,
+        mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None,
+        _raw_stream(x.get_device()))
+    if rc:
+        _fail(lib, rc)
     return (y, mean, rstd) if stats else y
 
 
-@_on_stream
 def layer_norm_ptr(n: int, row_ptrs: torch.Tensor, out: torch.Tensor,
                    weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                    eps: float = 1e-5, mean: Optional[torch.Tensor] = None,
-                   rstd: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   rstd: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """layer_norm of n rows by address: ``row_ptrs`` (int64) as HashTable.find_ptr
     fills them, rows of the type and length of ``out``'s.  The rows are read where
     the table keeps them and must not change meanwhile (HashTable.find_layer_norm
     holds the table's lock over both steps).  Null addresses leave their row of
     ``out`` (and of ``mean`` and ``rstd``, float32, optional) as it is."""
-    stride = _rows(out, "out")
-    dim = out.shape[1]
-    if not 0 <= n <= out.shape[0]:
+    if _elsewhere(out, stream):
+        return _run_there(layer_norm_ptr, out, stream, n, row_ptrs, out, weight, bias, eps, mean, rstd)
+    rows, dim, stride, kind = _float_rows(out, "out")
+    if not 0 <= n <= rows:
         raise ValueError("out must have n rows")
     if stride < dim * out.element_size():
         raise ValueError("the rows of out overlap")
-    if row_ptrs.dtype != torch.int64 or not row_ptrs.is_contiguous() or row_ptrs.numel() < n:
+    if row_ptrs.dtype is not torch.int64 or not row_ptrs.is_contiguous() or row_ptrs.numel() < n:
         raise ValueError("row_ptrs must be contiguous and hold n int64 addresses")
-    if row_ptrs.device != out.device:
+    if row_ptrs.get_device() != out.get_device():
         raise ValueError("row_ptrs must be on the device of out")
-    w, b, kind = _params(weight, bias, dim, out.dtype, out.device)
-    for name, s in (("mean", mean), ("rstd", rstd)):
-        if s is not None and (s.dtype != torch.float32 or s.numel() < n or not s.is_contiguous()
-                              or s.device != out.device):
-            raise ValueError(f"{name} must be contiguous, on the device of out and hold n float32 elements")
+    w, b, param_kind = _params(weight, bias, dim, out)
+    m, r = _statistic(mean, "mean", n, out), _statistic(rstd, "rstd", n, out)
     lib = load_library()
-    _chk(lib, lib.hkv_layer_norm_ptr(
-        n, dim, _ROW_KINDS[out.dtype], row_ptrs.data_ptr(), w, b, kind, eps, out.data_ptr(), stride,
-        mean.data_ptr() if mean is not None else None, rstd.data_ptr() if rstd is not None else None,
-        _current_stream(out)))
+    rc = lib.hkv_layer_norm_ptr(n, dim, kind, row_ptrs.data_ptr(), w, b, param_kind, eps, out.data_ptr(),
+                                stride, m, r, _raw_stream(out.get_device()))
+    if rc:
+        _fail(lib, rc)
     return out
 
 
-@_on_stream
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor],
                         mean: torch.Tensor, rstd: torch.Tensor, bias: bool = True,
-                        out: Optional[torch.Tensor] = None):
+                        out: Optional[torch.Tensor] = None, stream=None):
     """Gradients of layer_norm: (dx, d_weight, d_bias).  d_weight is None where
     the layer has no ``weight``, d_bias where ``bias`` is false; both have the
     type of ``weight`` (of the rows where there is none)."""
-    stride = _rows(x, "x")
-    n, dim = x.shape
-    dy_stride = _rows(dy, "dy", x, (n, dim))
-    w, _, kind = _params(weight, None, dim, x.dtype, x.device)
-    m = _vector(mean, "mean", n, (torch.float32,), x.device)
-    r = _vector(rstd, "rstd", n, (torch.float32,), x.device)
-    dx, dx_stride = _out(out, (n, dim), x)
+    if _elsewhere(x, stream):
+        return _run_there(layer_norm_backward, x, stream, dy, x, weight, mean, rstd, bias, out)
+    n, dim, stride, kind = _float_rows(x, "x")
+    dy_stride = _more_rows(dy, "dy", n, dim, x)
+    w, _, param_kind = _params(weight, None, dim, x)
+    m, r = _statistic(mean, "mean", n, x), _statistic(rstd, "rstd", n, x)
+    if m is None or r is None:
+        raise ValueError("mean and rstd must be those of layer_norm")
+    dx, dx_stride = _out(out, n, dim, x)
     lib = load_library()
-    ptype = x.dtype if weight is None else weight.dtype
-    d_weight = torch.empty(dim, dtype=ptype, device=x.device) if weight is not None else None
-    d_bias = torch.empty(dim, dtype=ptype, device=x.device) if bias else None
+    d_weight = torch.empty_like(weight) if weight is not None else None
+    d_bias = None
+    if bias:
+        d_bias = torch.empty_like(weight) if weight is not None else x.new_empty(dim)
     work, work_bytes = None, 0
-    if d_weight is not None or bias:
-        work_bytes = lib.hkv_layer_norm_backward_workspace_bytes(n, dim, _ROW_KINDS[x.dtype])
-        work = torch.empty(work_bytes, dtype=torch.uint8, device=x.device)
-    _chk(lib, lib.hkv_layer_norm_backward(
-        n, dim, _ROW_KINDS[x.dtype], dy.data_ptr(), dy_stride, x.data_ptr(), stride, w, kind, m, r,
+    if bias or weight is not None:
+        work_bytes = lib.hkv_layer_norm_backward_workspace_bytes(n, dim, kind)
+        work = x.new_empty(work_bytes, dtype=torch.uint8)
+    rc = lib.hkv_layer_norm_backward(
+        n, dim, kind, dy.data_ptr(), dy_stride, x.data_ptr(), stride, w, param_kind, m, r,
         dx.data_ptr(), dx_stride, d_weight.data_ptr() if d_weight is not None else None,
         d_bias.data_ptr() if bias else None, work.data_ptr() if work is not None else None,
-        work_bytes, _current_stream(x)))
+        work_bytes, _raw_stream(x.get_device()))
+    if rc:
+        _fail(lib, rc)
     return dx, d_weight, d_bias
