@@ -443,6 +443,16 @@ int launch_sort(uint64_t n, const ID* ids, uint32_t experts, int32_t* offsets, i
 
 constexpr int kMoveBlock = 256;
 
+// Division by the chunks of a row, by multiplication: exact while the dividend
+// times the divisor stays below 2^64.
+struct PerRow {
+  uint32_t chunks;
+  uint64_t magic;   // floor(2^64 / chunks) + 1; 0 for one chunk
+  __device__ __forceinline__ uint64_t row(uint64_t c) const {
+    return magic == 0 ? c : __umul64hi(c, magic);
+  }
+};
+
 // Zeroes the rows behind the last expert's, if the caller asked for it.
 template <int G>
 __device__ __forceinline__ void zero_behind(const int32_t* kept, uint64_t n, uint8_t* rows,
@@ -450,9 +460,9 @@ __device__ __forceinline__ void zero_behind(const int32_t* kept, uint64_t n, uin
   if (kept == nullptr) return;
   for (uint64_t r = uint64_t(max(*kept, 0)) + blockIdx.x; r < n; r += gridDim.x) {
     uint8_t* row = rows + r * rows_stride;
-    const uint32_t ahead = uint32_t(reinterpret_cast<uintptr_t>(row)) & 15u;
-    for (uint64_t at = threadIdx.x * 16ull; at < row_bytes + ahead; at += blockDim.x * 16ull) {
-      store_chunk<G>(row - ahead + at, make_uint4(0, 0, 0, 0), row, row + row_bytes);
+    const int ahead = int(reinterpret_cast<uintptr_t>(row) & 15u);
+    for (int64_t at = threadIdx.x * 16ll - ahead; at < int64_t(row_bytes); at += blockDim.x * 16ll) {
+      store_chunk<G>(row, int(at), make_uint4(0, 0, 0, 0), 0, int(row_bytes));
     }
   }
 }
@@ -460,16 +470,16 @@ __device__ __forceinline__ void zero_behind(const int32_t* kept, uint64_t n, uin
 // G == 0: all rows are whole aligned chunks; else pieces of G bytes at their ends.
 template <int G>
 __global__ void __launch_bounds__(kMoveBlock)
-    dispatch_kernel(const uint64_t tokens, const uint32_t top_k, const uint32_t chunks,
-                    const uint64_t row_bytes, const RowsIn x, const int32_t* __restrict__ position,
+    dispatch_kernel(const uint64_t tokens, const uint32_t top_k, const PerRow per_row,
+                    const uint32_t row_bytes, const RowsIn x, const int32_t* __restrict__ position,
                     uint8_t* __restrict__ rows, const uint64_t rows_stride,
                     const int32_t* __restrict__ kept) {
   const uint64_t n = tokens * top_k;
   zero_behind<(G ? G : 8)>(kept, n, rows, rows_stride, row_bytes);
   const uint64_t c = uint64_t(blockIdx.x) * kMoveBlock + threadIdx.x;
-  const uint64_t token = c / chunks;
+  const uint64_t token = per_row.row(c);
   if (token >= tokens) return;
-  const uint64_t off = (c - token * chunks) * 16;
+  const uint32_t off = uint32_t(c - token * per_row.chunks) * 16;
   const int32_t* at = position + token * top_k;
   const uint8_t* from = x.first + token * x.stride;
   if (G == 0) {
@@ -483,13 +493,12 @@ __global__ void __launch_bounds__(kMoveBlock)
       const uint32_t place = uint32_t(at[j]);
       if (place >= n) continue;
       uint8_t* row = rows + place * rows_stride;
-      uint8_t* q = row - (uint32_t(reinterpret_cast<uintptr_t>(row)) & 15u) + off;
-      if (q >= row + row_bytes) continue;
-      const uint8_t* p = from + (q - row);
+      const int o = int(off) - int(reinterpret_cast<uintptr_t>(row) & 15u);
+      if (o >= int(row_bytes)) continue;
       Cut cut;
-      cut.load(p, x.first, x.last);
-      store_chunk<(G ? G : 8)>(q, cut.get<(G ? G : 8)>(p, from, from + row_bytes), row,
-                               row + row_bytes);
+      cut.load(from + o, x.first, x.last);
+      store_chunk<(G ? G : 8)>(row, o, cut.get<(G ? G : 8)>(from + o, from, from + row_bytes), 0,
+                               int(row_bytes));
     }
   }
 }
@@ -501,19 +510,19 @@ __global__ void __launch_bounds__(kMoveBlock)
 
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(kMoveBlock)
-    combine_kernel(const uint64_t tokens, const uint32_t top_k, const uint32_t chunks,
-                   const uint64_t row_bytes, const RowsIn rows, const void* __restrict__ weights,
+    combine_kernel(const uint64_t tokens, const uint32_t top_k, const PerRow per_row,
+                   const uint32_t row_bytes, const RowsIn rows, const void* __restrict__ weights,
                    const bool weights_f32, const int32_t* __restrict__ position,
                    uint8_t* __restrict__ out, const uint64_t out_stride) {
   constexpr int kElems = kChunkElems<T>;
   const uint64_t c = uint64_t(blockIdx.x) * kMoveBlock + threadIdx.x;
-  const uint64_t token = c / chunks;
+  const uint64_t token = per_row.row(c);
   if (token >= tokens) return;
   const uint64_t n = tokens * top_k;
   uint8_t* to = out + token * out_stride;
-  int64_t off = int64_t(c - token * chunks) * 16;
-  if (!WHOLE) off -= uint32_t(reinterpret_cast<uintptr_t>(to)) & 15u;
-  if (!WHOLE && off >= int64_t(row_bytes)) return;
+  int off = int(c - token * per_row.chunks) * 16;
+  if (!WHOLE) off -= int(reinterpret_cast<uintptr_t>(to) & 15u);
+  if (!WHOLE && off >= int(row_bytes)) return;
   float sum[kElems];
 #pragma unroll
   for (int e = 0; e < kElems; ++e) sum[e] = 0.f;
@@ -558,7 +567,7 @@ __global__ void __launch_bounds__(kMoveBlock)
     }
   }
   if (WHOLE) *reinterpret_cast<uint4*>(to + off) = pack<T>(sum);
-  else store_chunk<sizeof(T)>(to + off, pack<T>(sum), to, to + row_bytes);
+  else store_chunk<sizeof(T)>(to, off, pack<T>(sum), 0, int(row_bytes));
 }
 
 // ---- combine, backward ----------------------------------------------------------
@@ -572,7 +581,7 @@ __global__ void __launch_bounds__(kMoveBlock)
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(256)
     combine_backward_kernel(const uint64_t tokens, const uint32_t top_k, const uint32_t chunks,
-                            const uint32_t group, const uint64_t row_bytes, const RowsIn d_out,
+                            const uint32_t group, const uint32_t row_bytes, const RowsIn d_out,
                             const RowsIn rows, const void* __restrict__ weights,
                             const bool weights_f32, const int32_t* __restrict__ position,
                             uint8_t* __restrict__ d_rows, const uint64_t d_rows_stride,
@@ -603,7 +612,7 @@ __global__ void __launch_bounds__(256)
       for (uint32_t c = lane; c < chunks; c += group) {
         uint4 d[WHOLE ? 1 : 4], row[4];
         Cut d_cut[WHOLE ? 1 : 4], row_cut[WHOLE ? 1 : 4];
-        int64_t off[4];
+        int off[4];
         if (WHOLE) d[0] = __ldg(reinterpret_cast<const uint4*>(d_from + uint64_t(c) * 16));
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -613,10 +622,10 @@ __global__ void __launch_bounds__(256)
             row[u] = __ldg(reinterpret_cast<const uint4*>(from + uint64_t(c) * 16));
           } else {
             const uint8_t* to = d_rows + place[u] * d_rows_stride;
-            off[u] = int64_t(c) * 16 - (uint32_t(reinterpret_cast<uintptr_t>(to)) & 15u);
+            off[u] = int(c) * 16 - int(reinterpret_cast<uintptr_t>(to) & 15u);
             row_cut[WHOLE ? 0 : u].none();
             d_cut[WHOLE ? 0 : u].none();
-            if (off[u] < int64_t(row_bytes)) {
+            if (off[u] < int(row_bytes)) {
               row_cut[WHOLE ? 0 : u].load(from + off[u], rows.first, rows.last);
               d_cut[WHOLE ? 0 : u].load(d_from + off[u], d_out.first, d_out.last);
             }
@@ -636,14 +645,20 @@ __global__ void __launch_bounds__(256)
           float du[kElems], y[kElems];
           unpack<T>(d[WHOLE ? 0 : u], du);
           unpack<T>(row[u], y);
+          if (!WHOLE && (off[u] < 0 || off[u] + 16 > int(row_bytes))) {   // an end of the row
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) {
+              const int b = off[u] + e * int(sizeof(T));
+              if (b < 0 || b >= int(row_bytes)) du[e] = y[e] = 0.f;
+            }
+          }
 #pragma unroll
           for (int e = 0; e < kElems; ++e) {
-            const int64_t b = WHOLE ? 0 : off[u] + e * int(sizeof(T));
-            if (WHOLE || (b >= 0 && b < int64_t(row_bytes))) dot[u] = fmaf(du[e], y[e], dot[u]);
+            dot[u] = fmaf(du[e], y[e], dot[u]);
             du[e] *= w[u];
           }
           if (WHOLE) *reinterpret_cast<uint4*>(to + uint64_t(c) * 16) = pack<T>(du);
-          else store_chunk<sizeof(T)>(to + off[u], pack<T>(du), to, to + row_bytes);
+          else store_chunk<sizeof(T)>(to, off[u], pack<T>(du), 0, int(row_bytes));
         }
       }
     }
@@ -688,6 +703,9 @@ uint32_t pow2_at_least(uint64_t v) {
 // Chunks per row: unaligned rows touch up to one more at either end.
 uint32_t chunks_of(uint64_t row_bytes, bool whole) {
   return uint32_t(whole ? row_bytes / 16 : (row_bytes + 30) / 16);
+}
+PerRow per_row(uint32_t chunks) {
+  return PerRow{chunks, chunks == 1 ? 0 : ~0ull / chunks + 1};
 }
 
 #define HKV_FOR_TYPE(kind, whole, CALL)                         \
@@ -758,7 +776,7 @@ int hkv_expert_dispatch(uint64_t tokens, uint32_t top_k, uint64_t row_bytes, con
                         int zero_rows_behind, hkv_stream stream) {
   int rc = check_order(tokens, top_k, experts);
   if (rc != HKV_OK) return rc;
-  HKV_ROWS_CHECK(row_bytes >= 1 && row_bytes < (1ull << 31), "row_bytes must be between 1 and 2^31 - 1");
+  HKV_ROWS_CHECK(row_bytes >= 1 && row_bytes < (1ull << 30), "row_bytes must be between 1 and 2^30 - 1");
   HKV_ROWS_CHECK(rows_stride >= row_bytes, "the sorted rows overlap");
   if (tokens == 0) return HKV_OK;
   HKV_ROWS_CHECK(x != nullptr && position != nullptr && rows != nullptr && offsets != nullptr,
@@ -774,7 +792,7 @@ int hkv_expert_dispatch(uint64_t tokens, uint32_t top_k, uint64_t row_bytes, con
   const RowsIn in = rows_in(x, tokens, x_stride, row_bytes);
   const int32_t* kept = zero_rows_behind ? offsets + experts : nullptr;
 #define HKV_CALL(G)                                                                              \
-  dispatch_kernel<G><<<grid, kMoveBlock, 0, s>>>(tokens, top_k, chunks, row_bytes, in, position, \
+  dispatch_kernel<G><<<grid, kMoveBlock, 0, s>>>(tokens, top_k, per_row(chunks), uint32_t(row_bytes), in, position, \
                                                  static_cast<uint8_t*>(rows), rows_stride, kept)
   switch (whole ? 0u : piece_bytes(bits)) {
     case 0: HKV_CALL(0); break;
@@ -797,7 +815,7 @@ int hkv_expert_combine(uint64_t tokens, uint32_t top_k, uint64_t dim, uint32_t v
   HKV_ROWS_CHECK(weights == nullptr || weight_kind == value_kind || weight_kind == kValueF32,
                  "weights have the rows' type or float32");
   const uint32_t size = row_kind_size(value_kind);
-  HKV_ROWS_CHECK(dim >= 1 && dim < (1ull << 29), "dim must be between 1 and 2^29 - 1");
+  HKV_ROWS_CHECK(dim >= 1 && dim < (1ull << 28), "dim must be between 1 and 2^28 - 1");
   HKV_ROWS_CHECK(out_stride >= dim * size, "the output rows overlap");
   if (tokens == 0) return HKV_OK;
   HKV_ROWS_CHECK(rows != nullptr && position != nullptr && out != nullptr,
@@ -815,7 +833,7 @@ int hkv_expert_combine(uint64_t tokens, uint32_t top_k, uint64_t dim, uint32_t v
   const RowsIn in = rows_in(rows, tokens * top_k, rows_stride, row_bytes);
 #define HKV_CALL(T, WHOLE)                                                                \
   combine_kernel<T, WHOLE><<<grid, kMoveBlock, 0, s>>>(                                   \
-      tokens, top_k, chunks, row_bytes, in, weights, weight_kind == kValueF32, position,  \
+      tokens, top_k, per_row(chunks), uint32_t(row_bytes), in, weights, weight_kind == kValueF32, position,  \
       static_cast<uint8_t*>(out), out_stride)
   HKV_FOR_TYPE(value_kind, whole, HKV_CALL)
 #undef HKV_CALL
@@ -834,7 +852,7 @@ int hkv_expert_combine_backward(uint64_t tokens, uint32_t top_k, uint64_t dim, u
   HKV_ROWS_CHECK(weight_kind == value_kind || weight_kind == kValueF32,
                  "weights have the rows' type or float32");
   const uint32_t size = row_kind_size(value_kind);
-  HKV_ROWS_CHECK(dim >= 1 && dim < (1ull << 29), "dim must be between 1 and 2^29 - 1");
+  HKV_ROWS_CHECK(dim >= 1 && dim < (1ull << 28), "dim must be between 1 and 2^28 - 1");
   HKV_ROWS_CHECK(d_rows_stride >= dim * size, "the rows of the gradient overlap");
   if (tokens == 0) return HKV_OK;
   HKV_ROWS_CHECK(d_out != nullptr && rows != nullptr && weights != nullptr && offsets != nullptr &&
@@ -857,7 +875,7 @@ int hkv_expert_combine_backward(uint64_t tokens, uint32_t top_k, uint64_t dim, u
   const int32_t* kept = zero_rows_behind ? offsets + experts : nullptr;
 #define HKV_CALL(T, WHOLE)                                                                       \
   combine_backward_kernel<T, WHOLE><<<grid, 256, 0, s>>>(                                        \
-      tokens, top_k, chunks, group, row_bytes, d_in, in, weights, weight_kind == kValueF32,      \
+      tokens, top_k, chunks, group, uint32_t(row_bytes), d_in, in, weights, weight_kind == kValueF32,      \
       position, static_cast<uint8_t*>(d_rows), d_rows_stride, d_weights, kept)
   HKV_FOR_TYPE(value_kind, whole, HKV_CALL)
 #undef HKV_CALL

@@ -123,31 +123,26 @@ __device__ __forceinline__ void store_row(uint8_t* row, uint32_t row_bytes, uint
     }
     return;
   }
-  const uint32_t s = uint32_t(reinterpret_cast<uintptr_t>(row)) & 15u;
-  const uint8_t* end = row + row_bytes;
+  const int s = int(reinterpret_cast<uintptr_t>(row) & 15u), end = int(row_bytes);
   const uint32_t left = (threadIdx.x & 31u & ~(map.width - 1u)) | ((map.lane - 1u) & (map.width - 1u));
+  const bool last_lane = map.lane == map.width - 1u;   // its right neighbour is in the next round
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-    const uint32_t at = map(c);
-    const bool to_next = map.lane == map.width - 1u;   // its right neighbour is in the next round
-    const uint4 give = to_next && c > 0 ? y[c > 0 ? c - 1 : 0] : y[c];
+    const uint4 give = last_lane && c > 0 ? y[c > 0 ? c - 1 : 0] : y[c];
     uint4 prev;
     prev.x = __shfl_sync(kFull, give.x, left);
     prev.y = __shfl_sync(kFull, give.y, left);
     prev.z = __shfl_sync(kFull, give.z, left);
     prev.w = __shfl_sync(kFull, give.w, left);
-    if (row == nullptr || at > chunks) continue;
-    uint8_t* q = row + at * 16u;
-    const bool joined = map.lane != 0 || c > 0;        // the left neighbour's bytes are here
-    if (s == 0) {
-      store_chunk<sizeof(T)>(q, y[c], row, end);
-      continue;
-    }
-    store_chunk<sizeof(T)>(q - s, shifted(prev, y[c], 16u - s), joined ? row : q, end);
-    if (c == CHUNKS - 1 && to_next) {
+    const int off = int(map(c) * 16u);
+    if (row == nullptr || map(c) > chunks) continue;
+    // the left neighbour's bytes are here, but for the first lane of the run
+    const int from = map.lane != 0 || c > 0 ? 0 : off;
+    store_chunk<sizeof(T)>(row, off - s, s == 0 ? y[c] : shifted(prev, y[c], 16u - s), from, end);
+    if (c == CHUNKS - 1 && last_lane && s != 0) {
       // the end of the warp's run: nobody joins this chunk's last bytes
-      const uint8_t* stop = q + 16 < end ? q + 16 : end;
-      store_chunk<sizeof(T)>(q - s + 16, shifted(y[c], make_uint4(0, 0, 0, 0), 16u - s), row, stop);
+      store_chunk<sizeof(T)>(row, off - s + 16, shifted(y[c], make_uint4(0, 0, 0, 0), 16u - s), 0,
+                             off + 16 < end ? off + 16 : end);
     }
   }
 }
@@ -193,18 +188,20 @@ struct RowQueue {
         if (map(c) < chunks) copy_async(to + c * 512u, from + (map(c) - map.first) * 16u);
       }
     } else {
-      const uint8_t* aligned = row - (reinterpret_cast<uintptr_t>(row) & 15u);
-      const uint8_t* end = row + row_bytes;
+      const int s = int(reinterpret_cast<uintptr_t>(row) & 15u), end = int(row_bytes);
+      const uint8_t* aligned = row - s;
+      const bool inside = aligned >= first && row + row_bytes + 16 <= last;   // not at the matrix's ends
 #pragma unroll
       for (int c = 0; c <= CHUNKS; ++c) {
         if (c == CHUNKS && map.lane != 0) break;
-        const uint8_t* a = aligned + map(c) * 16u;
-        if (a >= end) break;
+        const int off = int(map(c) * 16u);
+        if (off - s >= end) break;
+        const uint8_t* a = aligned + off;
         const uint32_t slot = to + (c * map.width + map.lane) * 16u;
-        if (a >= first && a + 16 <= last) {
+        if (inside || (a >= first && a + 16 <= last)) {
           copy_async(slot, a);
-        } else {   // at an end of the matrix
-          const uint4 v = pieces<sizeof(T)>(a, row, end);
+        } else {
+          const uint4 v = pieces<sizeof(T)>(a, row, row + row_bytes);
           asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(slot), "r"(v.x), "r"(v.y),
                        "r"(v.z), "r"(v.w)
                        : "memory");
@@ -516,15 +513,27 @@ __global__ void __launch_bounds__(kPipeBlock, 1)
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fill(i, r + i * step);
-  float next_mean = r < n ? __ldg(a.mean + r) : 0.f, next_rstd = r < n ? __ldg(a.rstd + r) : 0.f;
+  // of the rows in the queue, the current one's first
+  float means[kStages], rstds[kStages];
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) {
+    means[i] = i > 0 && r + (i - 1) * step < n ? __ldg(a.mean + r + (i - 1) * step) : 0.f;
+    rstds[i] = i > 0 && r + (i - 1) * step < n ? __ldg(a.rstd + r + (i - 1) * step) : 0.f;
+  }
   uint32_t stage = 0;
   // the lanes of a warp leave together: when the row of its first group is past the end
   for (uint32_t warp_row = r - (WIDE ? 0u : (threadIdx.x & 31u) / group); warp_row < n;
        warp_row += step, r += step) {
     fill(stage == 0 ? kStages - 1 : stage - 1, r + (kStages - 1) * step);
-    const float mean = next_mean, rstd = next_rstd;
-    next_mean = r + step < n ? __ldg(a.mean + r + step) : 0.f;
-    next_rstd = r + step < n ? __ldg(a.rstd + r + step) : 0.f;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      means[i] = means[i + 1];
+      rstds[i] = rstds[i + 1];
+    }
+    const uint32_t ahead = r + (kStages - 1) * step;
+    means[kStages - 1] = ahead < n ? __ldg(a.mean + ahead) : 0.f;
+    rstds[kStages - 1] = ahead < n ? __ldg(a.rstd + ahead) : 0.f;
+    const float mean = means[0], rstd = rstds[0];
     copies_wait<kStages - 1>();
     if (!WHOLE) __syncwarp();
     float xhat[CHUNKS][kElems], g[CHUNKS][kElems];

@@ -176,21 +176,49 @@ struct Cut {
   }
 };
 
-// Stores the bytes of v (for the aligned address q) that lie inside [from, to).
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
+  return i < 2 ? (i == 0 ? v.x : v.y) : (i == 2 ? v.z : v.w);
+}
+
+// Stores those bytes of the aligned 16 at row + off (v's) that lie in
+// [from, to) of the row, all three in bytes from its start.  A row's first and
+// last bytes go out in at most one piece of 8, 4, 2 and 1 bytes each, down to the
+// element size G; only rows that begin and end in the same 16 bytes are stored
+// element by element.
 template <int G>
-__device__ __forceinline__ void store_chunk(uint8_t* q, const uint4& v, const uint8_t* from,
-                                            const uint8_t* to) {
-  if (q >= from && q + 16 <= to) {
+__device__ __forceinline__ void store_chunk(uint8_t* row, int off, const uint4& v, int from, int to) {
+  const int lo = from > off ? from - off : 0, hi = to - off < 16 ? to - off : 16;
+  uint8_t* q = row + off;
+  if (lo == 0 && hi == 16) {
     *reinterpret_cast<uint4*>(q) = v;
+  } else if (hi <= lo) {
     return;
-  }
-  const uint8_t* bytes = reinterpret_cast<const uint8_t*>(&v);
-#pragma unroll
-  for (int b = 0; b < 16; b += G) {
-    if (q + b >= from && q + b < to) {
-      *reinterpret_cast<typename VecType<G>::type*>(q + b) =
-          *reinterpret_cast<const typename VecType<G>::type*>(bytes + b);
+  } else if (hi == 16) {   // the row's head: pieces that end at the boundary
+    const int h = 16 - lo;
+    if (h & 8) *reinterpret_cast<uint2*>(q + 8) = make_uint2(v.z, v.w);
+    if (G <= 4 && (h & 4)) *reinterpret_cast<uint32_t*>(q + 12 - (h & 8)) = h & 8 ? v.y : v.w;
+    if (G <= 2 && (h & 2)) {
+      const int at = 14 - (h & 12);
+      *reinterpret_cast<uint16_t*>(q + at) = static_cast<uint16_t>(word_of(v, at >> 2) >> 16);
     }
+    if (G <= 1 && (h & 1)) {
+      const int at = 15 - (h & 14);
+      q[at] = static_cast<uint8_t>(word_of(v, at >> 2) >> (8 * (at & 3)));
+    }
+  } else if (lo == 0) {    // its tail: pieces that start at the boundary
+    if (hi & 8) *reinterpret_cast<uint2*>(q) = make_uint2(v.x, v.y);
+    if (G <= 4 && (hi & 4)) *reinterpret_cast<uint32_t*>(q + (hi & 8)) = hi & 8 ? v.z : v.x;
+    if (G <= 2 && (hi & 2)) {
+      const int at = hi & 12;
+      *reinterpret_cast<uint16_t*>(q + at) = static_cast<uint16_t>(word_of(v, at >> 2));
+    }
+    if (G <= 1 && (hi & 1)) {
+      const int at = hi & 14;
+      q[at] = static_cast<uint8_t>(word_of(v, at >> 2) >> (8 * (at & 3)));
+    }
+  } else {
+#pragma unroll 1
+    for (int b = lo; b < hi; ++b) q[b] = static_cast<uint8_t>(word_of(v, b >> 2) >> (8 * (b & 3)));
   }
 }
 
