@@ -18,8 +18,9 @@ ROOT = os.path.dirname(HERE)
 LIB_PATH = os.path.join(HERE, "libhkv_b200.so")
 
 SOURCES = ["hkv_api.cu", "hkv_find.cu", "hkv_upsert.cu", "hkv_scan.cu", "hkv_noalloc.cu", "hkv_shard.cu",
-           "hkv_sharded.cu", "hkv_expert.cu", "hkv_norm.cu"]
-HEADERS = ["hkv_device.cuh", "hkv_internal.h", "hkv_rows.cuh", "hkv_norm.h"]
+           "hkv_sharded.cu", "hkv_expert.cu", "hkv_norm.cu",
+           "hkv_norm_backward.cu"]
+HEADERS = ["hkv_device.cuh", "hkv_internal.h", "hkv_rows.cuh", "hkv_norm.h", "hkv_norm.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -433,258 +433,307 @@ int launch_sort(uint64_t n, const ID* ids, uint32_t experts, int32_t* offsets, i
   return rows_launched();
 }
 
-// ---- dispatch -----------------------------------------------------------------
+// ---- rows -----------------------------------------------------------------------
 //
-// Bound by HBM: T rows read, N written.  Token by token: a thread loads one
-// chunk of a token's row and stores it to the row's k places, so every row is
-// read from memory once whatever k is.  Unaligned rows: the thread owns chunk i
-// of each place instead (places have alignments of their own) and cuts it out of
-// the token's row, which is in L1 after the first place.
+// The three operators below are bound by HBM.  A group of lanes (a power of two up
+// to a warp) takes a part of a token's row, V units per lane, and goes through the
+// token's assignments: their places and weights are looked up once for V units.
 
 constexpr int kMoveBlock = 256;
 
-// Division by the chunks of a row, by multiplication: exact while the dividend
-// times the divisor stays below 2^64.
-struct PerRow {
-  uint32_t chunks;
-  uint64_t magic;   // floor(2^64 / chunks) + 1; 0 for one chunk
-  __device__ __forceinline__ uint64_t row(uint64_t c) const {
-    return magic == 0 ? c : __umul64hi(c, magic);
+// The part of a token's row that a group of LANES lanes takes: V units per lane.
+struct RowParts {
+  uint32_t units;    // of a row
+  uint32_t parts;    // per row
+  uint64_t magic;    // floor(2^64 / parts) + 1, 0 for one part: division by multiplication,
+                     // exact while the dividend times the divisor stays below 2^64
+};
+
+template <int LANES, int V>
+struct MyPart {
+  uint64_t token;
+  uint32_t first;    // unit v of the lane is first + v * LANES
+  bool full;         // the part has all its units
+  uint32_t units;
+  __device__ __forceinline__ explicit MyPart(const RowParts& p) {
+    const uint64_t task = (uint64_t(blockIdx.x) * kMoveBlock + threadIdx.x) / LANES;
+    token = p.magic == 0 ? task : __umul64hi(task, p.magic);
+    const uint32_t begin = uint32_t(task - token * p.parts) * (LANES * V);
+    first = begin + (threadIdx.x & (LANES - 1u));
+    full = begin + LANES * V <= p.units;
+    units = p.units;
   }
+  __device__ __forceinline__ bool has(int v) const { return first + v * LANES < units; }
 };
 
 // Zeroes the rows behind the last expert's, if the caller asked for it.
-template <int G>
+template <int BYTES>
 __device__ __forceinline__ void zero_behind(const int32_t* kept, uint64_t n, uint8_t* rows,
-                                            uint64_t rows_stride, uint64_t row_bytes) {
+                                            uint64_t rows_stride, uint32_t units) {
+  using Raw = typename VecType<BYTES>::type;
   if (kept == nullptr) return;
   for (uint64_t r = uint64_t(max(*kept, 0)) + blockIdx.x; r < n; r += gridDim.x) {
-    uint8_t* row = rows + r * rows_stride;
-    const int ahead = int(reinterpret_cast<uintptr_t>(row) & 15u);
-    for (int64_t at = threadIdx.x * 16ll - ahead; at < int64_t(row_bytes); at += blockDim.x * 16ll) {
-      store_chunk<G>(row, int(at), make_uint4(0, 0, 0, 0), 0, int(row_bytes));
-    }
+    Raw* row = reinterpret_cast<Raw*>(rows + r * rows_stride);
+    for (uint32_t u = threadIdx.x; u < units; u += blockDim.x) row[u] = Raw{};
   }
 }
 
-// G == 0: all rows are whole aligned chunks; else pieces of G bytes at their ends.
-template <int G>
-__global__ void __launch_bounds__(kMoveBlock)
-    dispatch_kernel(const uint64_t tokens, const uint32_t top_k, const PerRow per_row,
-                    const uint32_t row_bytes, const RowsIn x, const int32_t* __restrict__ position,
-                    uint8_t* __restrict__ rows, const uint64_t rows_stride,
-                    const int32_t* __restrict__ kept) {
-  const uint64_t n = tokens * top_k;
-  zero_behind<(G ? G : 8)>(kept, n, rows, rows_stride, row_bytes);
-  const uint64_t c = uint64_t(blockIdx.x) * kMoveBlock + threadIdx.x;
-  const uint64_t token = per_row.row(c);
-  if (token >= tokens) return;
-  const uint32_t off = uint32_t(c - token * per_row.chunks) * 16;
-  const int32_t* at = position + token * top_k;
-  const uint8_t* from = x.first + token * x.stride;
-  if (G == 0) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(from + off));
-    for (uint32_t j = 0; j < top_k; ++j) {
-      const uint32_t place = uint32_t(at[j]);   // -1 is above every place
-      if (place < n) *reinterpret_cast<uint4*>(rows + place * rows_stride + off) = v;
-    }
-  } else {
-    for (uint32_t j = 0; j < top_k; ++j) {
-      const uint32_t place = uint32_t(at[j]);
-      if (place >= n) continue;
-      uint8_t* row = rows + place * rows_stride;
-      const int o = int(off) - int(reinterpret_cast<uintptr_t>(row) & 15u);
-      if (o >= int(row_bytes)) continue;
-      Cut cut;
-      cut.load(from + o, x.first, x.last);
-      store_chunk<(G ? G : 8)>(row, o, cut.get<(G ? G : 8)>(from + o, from, from + row_bytes), 0,
-                               int(row_bytes));
-    }
-  }
-}
-
-// ---- combine ------------------------------------------------------------------
+// ---- dispatch
 //
-// Bound by HBM: N rows read, T written.  A thread owns one chunk of a token's
-// output row and sums the k rows' chunks in registers, in the order of j.
+// T rows read, N written: a lane loads its units of the token's row and stores
+// them to the row's k places, so every row is read once whatever k is.
+template <int BYTES, int LANES, int V, bool FULL>
+__device__ __forceinline__ void dispatch_part(const MyPart<LANES, V>& my, uint64_t n, uint32_t top_k,
+                                              const RowsIn& x, const int32_t* __restrict__ position,
+                                              uint8_t* __restrict__ rows, uint64_t rows_stride) {
+  using Raw = typename VecType<BYTES>::type;
+  const Raw* from = reinterpret_cast<const Raw*>(x.first + my.token * x.stride) + my.first;
+  Raw v[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (FULL || my.has(i)) v[i] = __ldg(from + i * LANES);
+  }
+  const int32_t* at = position + my.token * top_k;
+  for (uint32_t j = 0; j < top_k; ++j) {
+    const uint32_t place = uint32_t(__ldg(at + j));   // -1 is above every place
+    if (place >= n) continue;
+    Raw* to = reinterpret_cast<Raw*>(rows + place * rows_stride) + my.first;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (FULL || my.has(i)) to[i * LANES] = v[i];
+    }
+  }
+}
 
-template <typename T, bool WHOLE>
+template <int BYTES, int LANES, int V>
 __global__ void __launch_bounds__(kMoveBlock)
-    combine_kernel(const uint64_t tokens, const uint32_t top_k, const PerRow per_row,
-                   const uint32_t row_bytes, const RowsIn rows, const void* __restrict__ weights,
-                   const bool weights_f32, const int32_t* __restrict__ position,
-                   uint8_t* __restrict__ out, const uint64_t out_stride) {
-  constexpr int kElems = kChunkElems<T>;
-  const uint64_t c = uint64_t(blockIdx.x) * kMoveBlock + threadIdx.x;
-  const uint64_t token = per_row.row(c);
-  if (token >= tokens) return;
+    dispatch_kernel(const uint64_t tokens, const uint32_t top_k, const RowParts parts, const RowsIn x,
+                    const int32_t* __restrict__ position, uint8_t* __restrict__ rows,
+                    const uint64_t rows_stride, const int32_t* __restrict__ kept) {
   const uint64_t n = tokens * top_k;
-  uint8_t* to = out + token * out_stride;
-  int off = int(c - token * per_row.chunks) * 16;
-  if (!WHOLE) off -= int(reinterpret_cast<uintptr_t>(to) & 15u);
-  if (!WHOLE && off >= int(row_bytes)) return;
-  float sum[kElems];
+  zero_behind<BYTES>(kept, n, rows, rows_stride, parts.units);
+  const MyPart<LANES, V> my(parts);
+  if (my.token >= tokens) return;
+  if (my.full) dispatch_part<BYTES, LANES, V, true>(my, n, top_k, x, position, rows, rows_stride);
+  else dispatch_part<BYTES, LANES, V, false>(my, n, top_k, x, position, rows, rows_stride);
+}
+
+// J assignments of a token, from j0 on: their rows' places and weights.  No branch
+// stands between the loads, so that all of them are in flight together (with one
+// per assignment, to skip the dropped, 16384 x 4096 bf16 of 8 rows each took 272 us
+// instead of 190): beyond the last assignment the last is read again, a dropped
+// one reads row 0, and neither is used.
+template <typename T, int J>
+struct Assigned {
+  uint32_t place[J];   // 0 if not ok
+  bool ok[J];
+  float w[J];
+  __device__ __forceinline__ Assigned(uint64_t token, uint32_t top_k, uint32_t j0, uint64_t n,
+                                      const int32_t* __restrict__ position,
+                                      const void* __restrict__ weights, bool weights_f32) {
+    const uint64_t first = token * top_k;
 #pragma unroll
-  for (int e = 0; e < kElems; ++e) sum[e] = 0.f;
-  for (uint32_t j0 = 0; j0 < top_k; j0 += 4) {
-    uint4 row[4];
-    Cut cut[WHOLE ? 1 : 4];
-    const uint8_t* from[4];
-    float w[4];
-    bool ok[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint64_t i = token * top_k + j0 + u;
-      uint32_t place = kFull;
-      if (j0 + u < top_k) place = uint32_t(position[i]);
-      ok[u] = place < n;
-      from[u] = rows.first + (ok[u] ? place * rows.stride : 0);
+    for (int u = 0; u < J; ++u) {
+      place[u] = uint32_t(__ldg(position + first + min(j0 + u, top_k - 1u)));
       w[u] = 1.f;
-      if (ok[u] && weights != nullptr) {
-        w[u] = weights_f32 ? static_cast<const float*>(weights)[i]
-                           : to_float(static_cast<const T*>(weights)[i]);
+    }
+    if (weights != nullptr) {
+      if (weights_f32) {
+        const float* from = static_cast<const float*>(weights) + first;
+#pragma unroll
+        for (int u = 0; u < J; ++u) w[u] = __ldg(from + min(j0 + u, top_k - 1u));
+      } else {
+        const T* from = static_cast<const T*>(weights) + first;
+#pragma unroll
+        for (int u = 0; u < J; ++u) w[u] = to_float(from[min(j0 + u, top_k - 1u)]);
       }
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (WHOLE) {
-        if (ok[u]) row[u] = __ldg(reinterpret_cast<const uint4*>(from[u] + off));
-      } else if (ok[u]) {
-        cut[WHOLE ? 0 : u].load(from[u] + off, rows.first, rows.last);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (!ok[u]) continue;
-      if (!WHOLE) {
-        row[u] = cut[WHOLE ? 0 : u].template get<sizeof(T)>(from[u] + off, from[u],
-                                                            from[u] + row_bytes);
-      }
-      float f[kElems];
-      unpack<T>(row[u], f);
-#pragma unroll
-      for (int e = 0; e < kElems; ++e) sum[e] = fmaf(w[u], f[e], sum[e]);
+    for (int u = 0; u < J; ++u) {
+      ok[u] = j0 + u < top_k && place[u] < n;   // -1 is above every place
+      place[u] = ok[u] ? place[u] : 0u;
     }
   }
-  if (WHOLE) *reinterpret_cast<uint4*>(to + off) = pack<T>(sum);
-  else store_chunk<sizeof(T)>(to, off, pack<T>(sum), 0, int(row_bytes));
+};
+
+// ---- combine
+//
+// N rows read, T written: a lane sums its units of the k rows in registers, in the
+// order of j, with the loads of J assignments in flight.
+template <typename T, int BYTES, int LANES, int V, int J, bool FULL>
+__device__ __forceinline__ void combine_part(const MyPart<LANES, V>& my, uint64_t n, uint32_t top_k,
+                                             const RowsIn& rows, const void* __restrict__ weights,
+                                             bool weights_f32, const int32_t* __restrict__ position,
+                                             uint8_t* __restrict__ out, uint64_t out_stride) {
+  using U = Unit<T, BYTES>;
+  using Raw = typename U::Raw;
+  float sum[V][U::kElems];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+#pragma unroll
+    for (int e = 0; e < U::kElems; ++e) sum[i][e] = 0.f;
+  }
+#pragma unroll 1
+  for (uint32_t j0 = 0; j0 < top_k; j0 += J) {
+    const Assigned<T, J> a(my.token, top_k, j0, n, position, weights, weights_f32);
+    Raw row[J][V];
+#pragma unroll
+    for (int u = 0; u < J; ++u) {
+      const Raw* from = reinterpret_cast<const Raw*>(rows.first + a.place[u] * rows.stride) + my.first;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        row[u][v] = no_unit<Raw>();
+        if (FULL || my.has(v)) row[u][v] = __ldg(from + v * LANES);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < J; ++u) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float f[U::kElems];
+        U::unpack(row[u][v], f);
+#pragma unroll
+        for (int e = 0; e < U::kElems; ++e) {
+          if (a.ok[u]) sum[v][e] = fmaf(a.w[u], f[e], sum[v][e]);
+        }
+      }
+    }
+  }
+  Raw* to = reinterpret_cast<Raw*>(out + my.token * out_stride) + my.first;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    if (FULL || my.has(v)) to[v * LANES] = U::pack(sum[v]);
+  }
 }
 
-// ---- combine, backward ----------------------------------------------------------
-//
-// Bound by HBM: T + N rows read, N written.  A group of threads takes a token;
-// for four assignments at a time a lane loads its chunks of the rows, stores
-// w * d_out and adds to its four partial dot products, which the group sums at
-// the end.  d_out's chunk is loaded once for the four; with unaligned rows each
-// place has its own cut of it, out of L1.
-
-template <typename T, bool WHOLE>
-__global__ void __launch_bounds__(256)
-    combine_backward_kernel(const uint64_t tokens, const uint32_t top_k, const uint32_t chunks,
-                            const uint32_t group, const uint32_t row_bytes, const RowsIn d_out,
-                            const RowsIn rows, const void* __restrict__ weights,
-                            const bool weights_f32, const int32_t* __restrict__ position,
-                            uint8_t* __restrict__ d_rows, const uint64_t d_rows_stride,
-                            void* __restrict__ d_weights, const int32_t* __restrict__ kept) {
-  constexpr int kElems = kChunkElems<T>;
-  __shared__ float partial[8][4];
+template <typename T, int BYTES, int LANES, int V, int J>
+__global__ void __launch_bounds__(kMoveBlock)
+    combine_kernel(const uint64_t tokens, const uint32_t top_k, const RowParts parts, const RowsIn rows,
+                   const void* __restrict__ weights, const bool weights_f32,
+                   const int32_t* __restrict__ position, uint8_t* __restrict__ out,
+                   const uint64_t out_stride) {
+  const MyPart<LANES, V> my(parts);
+  if (my.token >= tokens) return;
   const uint64_t n = tokens * top_k;
-  zero_behind<sizeof(T)>(kept, n, d_rows, d_rows_stride, row_bytes);
+  if (V > 1 && my.full) {
+    combine_part<T, BYTES, LANES, V, J, true>(my, n, top_k, rows, weights, weights_f32, position, out,
+                                              out_stride);
+  } else {
+    combine_part<T, BYTES, LANES, V, J, false>(my, n, top_k, rows, weights, weights_f32, position, out,
+                                               out_stride);
+  }
+}
+
+// ---- combine, backward
+//
+// T + N rows read, N written.  A group of threads takes a token's whole row (the
+// dot products run over it): LANES of a warp, or (LANES == 32) some warps, which go
+// over it in steps of V units per lane.  For J assignments at a time a lane loads
+// its units of the rows, stores w * d_out and adds to its J partial dot products,
+// which the group sums at the end.
+template <typename T, int BYTES, int LANES, int V, int J, bool FULL>
+__device__ __forceinline__ void combine_backward_step(
+    uint32_t first, uint32_t units, const Assigned<T, J>& a,
+    const typename Unit<T, BYTES>::Raw* __restrict__ d_from,
+    const typename Unit<T, BYTES>::Raw* const (&from)[J], typename Unit<T, BYTES>::Raw* const (&to)[J],
+    float (&dot)[J]) {
+  using U = Unit<T, BYTES>;
+  typename U::Raw d[V], row[J][V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    d[v] = no_unit<typename U::Raw>();
+    if (FULL || first + v * LANES < units) d[v] = __ldg(d_from + first + v * LANES);
+  }
+#pragma unroll
+  for (int u = 0; u < J; ++u) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      row[u][v] = no_unit<typename U::Raw>();
+      if (FULL || first + v * LANES < units) row[u][v] = __ldg(from[u] + first + v * LANES);
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float f[U::kElems];
+    U::unpack(d[v], f);
+#pragma unroll
+    for (int u = 0; u < J; ++u) {
+      float y[U::kElems];
+      U::unpack(row[u][v], y);
+#pragma unroll
+      for (int e = 0; e < U::kElems; ++e) {
+        if (a.ok[u]) dot[u] = fmaf(f[e], y[e], dot[u]);
+        y[e] = a.w[u] * f[e];
+      }
+      if (a.ok[u] && (FULL || first + v * LANES < units)) to[u][first + v * LANES] = U::pack(y);
+    }
+  }
+}
+
+template <typename T, int BYTES, int LANES, int V, int J>
+__global__ void __launch_bounds__(256)
+    combine_backward_kernel(const uint64_t tokens, const uint32_t top_k, const uint32_t units,
+                            const uint32_t warps, const RowsIn d_out, const RowsIn rows,
+                            const void* __restrict__ weights, const bool weights_f32,
+                            const int32_t* __restrict__ position, uint8_t* __restrict__ d_rows,
+                            const uint64_t d_rows_stride, void* __restrict__ d_weights,
+                            const int32_t* __restrict__ kept) {
+  using Raw = typename Unit<T, BYTES>::Raw;
+  __shared__ float partial[8][J];
+  const uint64_t n = tokens * top_k;
+  zero_behind<BYTES>(kept, n, d_rows, d_rows_stride, units);
+  // warps: of a group, a power of two; the part of the row between its warps' steps
+  const uint32_t group = LANES == 32 ? warps * 32u : uint32_t(LANES);
   const uint32_t lane = threadIdx.x & (group - 1u);
   const uint64_t token = (uint64_t(blockIdx.x) * blockDim.x + threadIdx.x) / group;
   const bool live = token < tokens;
-  const uint8_t* d_from = d_out.first + token * d_out.stride;
-  for (uint32_t j0 = 0; j0 < top_k; j0 += 4) {
-    uint32_t place[4];
-    float w[4], dot[4];
+  const Raw* d_from = reinterpret_cast<const Raw*>(d_out.first + token * d_out.stride);
+#pragma unroll 1
+  for (uint32_t j0 = 0; j0 < top_k; j0 += J) {
+    const Assigned<T, J> a(live ? token : 0, top_k, j0, n, position, weights, weights_f32);
+    const Raw* from[J];
+    Raw* to[J];
+    float dot[J];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint64_t i = token * top_k + j0 + u;
-      place[u] = kFull;
-      w[u] = dot[u] = 0.f;
-      if (live && j0 + u < top_k) {
-        place[u] = uint32_t(position[i]);
-        w[u] = weights_f32 ? static_cast<const float*>(weights)[i]
-                           : to_float(static_cast<const T*>(weights)[i]);
-      }
+    for (int u = 0; u < J; ++u) {
+      from[u] = reinterpret_cast<const Raw*>(rows.first + a.place[u] * rows.stride);
+      to[u] = reinterpret_cast<Raw*>(d_rows + a.place[u] * d_rows_stride);
+      dot[u] = 0.f;
     }
     if (live) {
-      for (uint32_t c = lane; c < chunks; c += group) {
-        uint4 d[WHOLE ? 1 : 4], row[4];
-        Cut d_cut[WHOLE ? 1 : 4], row_cut[WHOLE ? 1 : 4];
-        int off[4];
-        if (WHOLE) d[0] = __ldg(reinterpret_cast<const uint4*>(d_from + uint64_t(c) * 16));
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (place[u] >= n) continue;
-          const uint8_t* from = rows.first + place[u] * rows.stride;
-          if (WHOLE) {
-            row[u] = __ldg(reinterpret_cast<const uint4*>(from + uint64_t(c) * 16));
-          } else {
-            const uint8_t* to = d_rows + place[u] * d_rows_stride;
-            off[u] = int(c) * 16 - int(reinterpret_cast<uintptr_t>(to) & 15u);
-            row_cut[WHOLE ? 0 : u].none();
-            d_cut[WHOLE ? 0 : u].none();
-            if (off[u] < int(row_bytes)) {
-              row_cut[WHOLE ? 0 : u].load(from + off[u], rows.first, rows.last);
-              d_cut[WHOLE ? 0 : u].load(d_from + off[u], d_out.first, d_out.last);
-            }
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (place[u] >= n) continue;
-          if (!WHOLE) {
-            const uint8_t* from = rows.first + place[u] * rows.stride;
-            row[u] = row_cut[WHOLE ? 0 : u].template get<sizeof(T)>(from + off[u], from,
-                                                                        from + row_bytes);
-            d[WHOLE ? 0 : u] = d_cut[WHOLE ? 0 : u].template get<sizeof(T)>(
-                d_from + off[u], d_from, d_from + row_bytes);
-          }
-          uint8_t* to = d_rows + place[u] * d_rows_stride;
-          float du[kElems], y[kElems];
-          unpack<T>(d[WHOLE ? 0 : u], du);
-          unpack<T>(row[u], y);
-          if (!WHOLE && (off[u] < 0 || off[u] + 16 > int(row_bytes))) {   // an end of the row
-#pragma unroll
-            for (int e = 0; e < kElems; ++e) {
-              const int b = off[u] + e * int(sizeof(T));
-              if (b < 0 || b >= int(row_bytes)) du[e] = y[e] = 0.f;
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < kElems; ++e) {
-            dot[u] = fmaf(du[e], y[e], dot[u]);
-            du[e] *= w[u];
-          }
-          if (WHOLE) *reinterpret_cast<uint4*>(to + uint64_t(c) * 16) = pack<T>(du);
-          else store_chunk<sizeof(T)>(to, off[u], pack<T>(du), 0, int(row_bytes));
+      const uint32_t own = threadIdx.x & (LANES - 1u);
+#pragma unroll 1
+      for (uint32_t begin = (lane - own) * V; begin < units; begin += group * V) {
+        if (V > 1 && begin + LANES * V <= units) {
+          combine_backward_step<T, BYTES, LANES, V, J, true>(begin + own, units, a, d_from, from, to, dot);
+        } else {
+          combine_backward_step<T, BYTES, LANES, V, J, false>(begin + own, units, a, d_from, from, to, dot);
         }
       }
     }
-    const uint32_t width = group < 32u ? group : 32u;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      for (uint32_t d = width >> 1; d > 0; d >>= 1) dot[u] += __shfl_xor_sync(kFull, dot[u], d);
+    for (int u = 0; u < J; ++u) {
+#pragma unroll
+      for (int d = LANES >> 1; d > 0; d >>= 1) dot[u] += __shfl_xor_sync(kFull, dot[u], d);
     }
     if (group > 32u) {   // uniform over the block: all of it arrives
       __syncthreads();
       const uint32_t warp = threadIdx.x >> 5;
       if ((threadIdx.x & 31u) == 0) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) partial[warp][u] = dot[u];
+        for (int u = 0; u < J; ++u) partial[warp][u] = dot[u];
       }
       __syncthreads();
       if (lane == 0) {
         for (uint32_t v = 1; v < group >> 5; ++v) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) dot[u] += partial[warp + v][u];
+          for (int u = 0; u < J; ++u) dot[u] += partial[warp + v][u];
         }
       }
     }
     if (live && lane == 0) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < J; ++u) {
         if (j0 + u >= top_k) continue;
         const uint64_t i = token * top_k + j0 + u;
         if (weights_f32) static_cast<float*>(d_weights)[i] = dot[u];
@@ -700,21 +749,25 @@ uint32_t pow2_at_least(uint64_t v) {
   return p;
 }
 
-// Chunks per row: unaligned rows touch up to one more at either end.
-uint32_t chunks_of(uint64_t row_bytes, bool whole) {
-  return uint32_t(whole ? row_bytes / 16 : (row_bytes + 30) / 16);
+// Lanes on a part of a row of `units` units with `per_lane` units each: a warp, or
+// eight of its lanes, or two where the row has no more.
+uint32_t lanes_for(uint64_t units, uint32_t per_lane) {
+  return units > 8ull * per_lane ? 32 : units > 2ull * per_lane ? 8 : 2;
 }
-PerRow per_row(uint32_t chunks) {
-  return PerRow{chunks, chunks == 1 ? 0 : ~0ull / chunks + 1};
+RowParts row_parts(uint64_t units, uint32_t lanes, uint32_t per_lane) {
+  RowParts p{};
+  p.units = uint32_t(units);
+  const uint64_t part = uint64_t(lanes) * per_lane;
+  p.parts = uint32_t((units + part - 1) / part);
+  p.magic = p.parts == 1 ? 0 : ~0ull / p.parts + 1;
+  return p;
 }
-
-#define HKV_FOR_TYPE(kind, whole, CALL)                         \
-  if ((kind) == hkv::kValueF32) {                               \
-    if (whole) { CALL(float, true); } else { CALL(float, false); } \
-  } else if ((kind) == hkv::kValueF16) {                        \
-    if (whole) { CALL(__half, true); } else { CALL(__half, false); } \
-  } else {                                                      \
-    if (whole) { CALL(__nv_bfloat16, true); } else { CALL(__nv_bfloat16, false); } \
+// CALL(LANES) for the number of lanes.
+#define HKV_FOR_LANES(lanes, CALL) \
+  switch (lanes) {                 \
+    case 32: CALL(32); break;      \
+    case 8: CALL(8); break;        \
+    default: CALL(2); break;       \
   }
 
 int check_order(uint64_t tokens, uint32_t top_k, uint32_t experts) {
@@ -726,7 +779,7 @@ int check_order(uint64_t tokens, uint32_t top_k, uint32_t experts) {
 }
 
 // Blocks of `threads` threads for `items` threads' work.
-int grid_of(uint64_t items, uint32_t threads, unsigned* grid) {
+int grid_of(uint64_t items, uint32_t threads, unsigned* grid) noexcept {
   const uint64_t blocks = (items + threads - 1) / threads;
   HKV_ROWS_CHECK(blocks < (1ull << 31), "batch too large for one launch");
   *grid = unsigned(blocks);
@@ -781,27 +834,32 @@ int hkv_expert_dispatch(uint64_t tokens, uint32_t top_k, uint64_t row_bytes, con
   if (tokens == 0) return HKV_OK;
   HKV_ROWS_CHECK(x != nullptr && position != nullptr && rows != nullptr && offsets != nullptr,
                  "x, offsets, position and rows must not be null");
-  const uint64_t bits =
-      row_bytes | address_bits(x) | x_stride | address_bits(rows) | rows_stride;
-  const bool whole = whole_chunks(bits);
-  const uint32_t chunks = chunks_of(row_bytes, whole);
+  const uint64_t bits = row_bytes | address_bits(x) | x_stride | address_bits(rows) | rows_stride;
+  uint32_t unit = 16;
+  while (bits % unit != 0) unit >>= 1;
+  const uint32_t per_lane = unit == 16 ? 4 : 8;
+  const uint32_t lanes = lanes_for(row_bytes / unit, per_lane);
+  const RowParts parts = row_parts(row_bytes / unit, lanes, per_lane);
   unsigned grid = 0;
-  rc = grid_of(tokens * chunks, kMoveBlock, &grid);
+  rc = grid_of(tokens * parts.parts * lanes, kMoveBlock, &grid);
   if (rc != HKV_OK) return rc;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const RowsIn in = rows_in(x, tokens, x_stride, row_bytes);
   const int32_t* kept = zero_rows_behind ? offsets + experts : nullptr;
-#define HKV_CALL(G)                                                                              \
-  dispatch_kernel<G><<<grid, kMoveBlock, 0, s>>>(tokens, top_k, per_row(chunks), uint32_t(row_bytes), in, position, \
-                                                 static_cast<uint8_t*>(rows), rows_stride, kept)
-  switch (whole ? 0u : piece_bytes(bits)) {
-    case 0: HKV_CALL(0); break;
-    case 8: HKV_CALL(8); break;
-    case 4: HKV_CALL(4); break;
-    case 2: HKV_CALL(2); break;
-    default: HKV_CALL(1); break;
+#define HKV_RUN(BYTES, LANES)                                                            \
+  dispatch_kernel<BYTES, LANES, (BYTES == 16 ? 4 : 8)>                                   \
+      <<<grid, kMoveBlock, 0, static_cast<cudaStream_t>(stream)>>>(                      \
+          tokens, top_k, parts, in, position, static_cast<uint8_t*>(rows), rows_stride, kept)
+#define HKV_CALL(LANES)                     \
+  switch (unit) {                           \
+    case 16: HKV_RUN(16, LANES); break;     \
+    case 8: HKV_RUN(8, LANES); break;       \
+    case 4: HKV_RUN(4, LANES); break;       \
+    case 2: HKV_RUN(2, LANES); break;       \
+    default: HKV_RUN(1, LANES); break;      \
   }
+  HKV_FOR_LANES(lanes, HKV_CALL)
 #undef HKV_CALL
+#undef HKV_RUN
   return rows_launched();
 }
 
@@ -821,22 +879,34 @@ int hkv_expert_combine(uint64_t tokens, uint32_t top_k, uint64_t dim, uint32_t v
   HKV_ROWS_CHECK(rows != nullptr && position != nullptr && out != nullptr,
                  "rows, position and out must not be null");
   const uint64_t row_bytes = dim * size;
-  const uint64_t bits =
-      row_bytes | address_bits(rows) | rows_stride | address_bits(out) | out_stride;
-  HKV_ROWS_CHECK(bits % size == 0, "a row does not start at a multiple of its element size");
-  const bool whole = whole_chunks(bits);
-  const uint32_t chunks = chunks_of(row_bytes, whole);
+  const uint32_t unit =
+      unit_bytes(row_bytes | address_bits(rows) | rows_stride | address_bits(out) | out_stride, size);
+  HKV_ROWS_CHECK(unit != 0, "a row does not start at a multiple of its element size");
+  // with one or two assignments per token a lane takes more units instead, so that
+  // as many loads are in flight
+  const uint32_t per_lane = unit == 16 ? (top_k <= 2 ? 4 : 1) : 8;
+  const uint32_t lanes = lanes_for(row_bytes / unit, per_lane);
+  const RowParts parts = row_parts(row_bytes / unit, lanes, per_lane);
   unsigned grid = 0;
-  rc = grid_of(tokens * chunks, kMoveBlock, &grid);
+  rc = grid_of(tokens * parts.parts * lanes, kMoveBlock, &grid);
   if (rc != HKV_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const RowsIn in = rows_in(rows, tokens * top_k, rows_stride, row_bytes);
-#define HKV_CALL(T, WHOLE)                                                                \
-  combine_kernel<T, WHOLE><<<grid, kMoveBlock, 0, s>>>(                                   \
-      tokens, top_k, per_row(chunks), uint32_t(row_bytes), in, weights, weight_kind == kValueF32, position,  \
+#define HKV_RUN(T, BYTES, LANES, V, J)                                                    \
+  combine_kernel<T, BYTES, LANES, V, J><<<grid, kMoveBlock, 0, s>>>(                      \
+      tokens, top_k, parts, in, weights, weight_kind == kValueF32, position,              \
       static_cast<uint8_t*>(out), out_stride)
-  HKV_FOR_TYPE(value_kind, whole, HKV_CALL)
+#define HKV_LANES(LANES)                                                 \
+  if (top_k <= 2) HKV_RUN(RowT, kUnit, LANES, (kUnit == 16 ? 4 : 8), 2); \
+  else HKV_RUN(RowT, kUnit, LANES, (kUnit == 16 ? 1 : 8), 4)
+#define HKV_CALL(T, BYTES)         \
+  using RowT = T;                  \
+  constexpr int kUnit = BYTES;     \
+  HKV_FOR_LANES(lanes, HKV_LANES)
+  HKV_FOR_UNIT(value_kind, unit, HKV_CALL)
 #undef HKV_CALL
+#undef HKV_LANES
+#undef HKV_RUN
   return rows_launched();
 }
 
@@ -859,26 +929,37 @@ int hkv_expert_combine_backward(uint64_t tokens, uint32_t top_k, uint64_t dim, u
                      position != nullptr && d_rows != nullptr && d_weights != nullptr,
                  "no argument may be null");
   const uint64_t row_bytes = dim * size;
-  const uint64_t bits = row_bytes | address_bits(d_out) | d_out_stride | address_bits(rows) |
-                        rows_stride | address_bits(d_rows) | d_rows_stride;
-  HKV_ROWS_CHECK(bits % size == 0, "a row does not start at a multiple of its element size");
-  const bool whole = whole_chunks(bits);
-  const uint32_t chunks = chunks_of(row_bytes, whole);
-  uint32_t group = pow2_at_least(chunks);
-  group = group > 256u ? 256u : group;
+  const uint32_t unit = unit_bytes(row_bytes | address_bits(d_out) | d_out_stride | address_bits(rows) |
+                                       rows_stride | address_bits(d_rows) | d_rows_stride,
+                                   size);
+  HKV_ROWS_CHECK(unit != 0, "a row does not start at a multiple of its element size");
+  const uint64_t units = row_bytes / unit;
+  const uint32_t per_lane = unit == 16 ? 1 : 4;
+  const uint32_t lanes = lanes_for(units, per_lane);
+  uint32_t warps = pow2_at_least((units + 32 * per_lane - 1) / (32 * per_lane));
+  warps = warps > 8 ? 8 : warps;
   unsigned grid = 0;
-  rc = grid_of(tokens * group, 256, &grid);
+  rc = grid_of(tokens * (lanes == 32 ? warps * 32 : lanes), 256, &grid);
   if (rc != HKV_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const RowsIn d_in = rows_in(d_out, tokens, d_out_stride, row_bytes);
   const RowsIn in = rows_in(rows, tokens * top_k, rows_stride, row_bytes);
   const int32_t* kept = zero_rows_behind ? offsets + experts : nullptr;
-#define HKV_CALL(T, WHOLE)                                                                       \
-  combine_backward_kernel<T, WHOLE><<<grid, 256, 0, s>>>(                                        \
-      tokens, top_k, chunks, group, uint32_t(row_bytes), d_in, in, weights, weight_kind == kValueF32,      \
-      position, static_cast<uint8_t*>(d_rows), d_rows_stride, d_weights, kept)
-  HKV_FOR_TYPE(value_kind, whole, HKV_CALL)
+#define HKV_RUN(T, BYTES, LANES, J)                                                                 \
+  combine_backward_kernel<T, BYTES, LANES, (BYTES == 16 ? 1 : 4), J><<<grid, 256, 0, s>>>(          \
+      tokens, top_k, uint32_t(units), warps, d_in, in, weights, weight_kind == kValueF32, position, \
+      static_cast<uint8_t*>(d_rows), d_rows_stride, d_weights, kept)
+#define HKV_LANES(LANES)                            \
+  if (top_k <= 2) HKV_RUN(RowT, kUnit, LANES, 2);   \
+  else HKV_RUN(RowT, kUnit, LANES, 4)
+#define HKV_CALL(T, BYTES)         \
+  using RowT = T;                  \
+  constexpr int kUnit = BYTES;     \
+  HKV_FOR_LANES(lanes, HKV_LANES)
+  HKV_FOR_UNIT(value_kind, unit, HKV_CALL)
 #undef HKV_CALL
+#undef HKV_LANES
+#undef HKV_RUN
   return rows_launched();
 }
 

@@ -1,0 +1,342 @@
+// What layer norm and its gradient share: how a row is dealt to threads, the sums
+// over it, and the queues rows wait in.
+#pragma once
+
+#include "hkv_norm.h"
+#include "hkv_rows.cuh"
+
+namespace hkv {
+
+constexpr uint32_t kFull = 0xFFFFFFFFu;
+constexpr int kPipeBlock = 512;   // threads of the kernels that stay on the device
+constexpr int kStages = 3;        // rows of a warp's queue: one in use, two on their way
+
+// Sum over the `group` threads of a row: WIDTH of them where that is below 32 (0:
+// a power of two known at run time), else whole warps; every thread gets it.  scratch: two floats of each
+// value per warp, used in turn, so that one barrier of the group's own (named
+// 1 + its number in the block) is enough.
+template <int N, int WIDTH>
+struct GroupSum {
+  static constexpr bool WIDE = WIDTH == 32;
+  uint32_t group, warps, span, from, barrier;   // warps: of the group; span: the next power of two
+  float (*scratch)[2][N];                       // [warps of the block]
+  uint32_t turn = 0;
+
+  __device__ __forceinline__ GroupSum(uint32_t group_, float (*scratch_)[2][N])
+      : group(group_), warps(group_ >> 5), barrier(1u + threadIdx.x / group_), scratch(scratch_) {
+    span = 1;
+    while (span < warps) span <<= 1;
+    // where this lane reads when the group's warps exchange their sums
+    from = WIDE ? threadIdx.x / group * warps + (threadIdx.x & (span - 1u)) : 0u;
+  }
+
+  __device__ __forceinline__ void operator()(float (&v)[N]) {
+    if (WIDE) {
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(kFull, v[i], d);
+      }
+      if (warps == 1) return;
+      if ((threadIdx.x & 31u) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) scratch[threadIdx.x >> 5][turn][i] = v[i];
+      }
+      asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(group) : "memory");
+      const bool has = (threadIdx.x & (span - 1u)) < warps;
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = has ? scratch[from][turn][i] : 0.f;
+      for (uint32_t d = span >> 1; d > 0; d >>= 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(kFull, v[i], d);
+      }
+      turn ^= 1u;
+    } else {
+#pragma unroll
+      for (uint32_t d = (WIDTH ? uint32_t(WIDTH) : group) >> 1; d > 0; d >>= 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(kFull, v[i], d);
+      }
+    }
+  }
+};
+
+// Where a thread's units lie in its row: unit c of the thread is first + c * width
+// of the row.  A warp of a group of several owns a part of consecutive units, which
+// begins at unit `part` and has `count`; the lanes of a group below a warp own all.
+template <int UNITS, int WIDTH>
+struct UnitMap {
+  uint32_t part, count, lane, width;   // lane: within the width
+
+  __device__ __forceinline__ UnitMap(uint32_t group, uint32_t units) {
+    width = WIDTH ? uint32_t(WIDTH) : group;
+    lane = threadIdx.x & (width - 1u);
+    part = WIDTH == 32 ? (threadIdx.x % group >> 5) * 32u * UNITS : 0u;
+    count = units > part ? min(units - part, width * UNITS) : 0u;
+  }
+  // The unit's number within the part.
+  __device__ __forceinline__ uint32_t operator()(int c) const {
+    return lane + uint32_t(c) * (WIDTH ? uint32_t(WIDTH) : width);
+  }
+  // f(c, mine) for the thread's units c, in runs of RUN: `mine` is a constant where
+  // all lanes have the whole run, and runs that none has are left out.
+  template <int RUN, typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    static_assert(UNITS % RUN == 0, "whole runs");
+#pragma unroll
+    for (int b = 0; b < UNITS; b += RUN) {
+      if ((b + RUN) * width <= count) {
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) f(b + i, true);
+      } else if (b * width < count) {
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) f(b + i, (*this)(b + i) < count);
+      }
+    }
+  }
+};
+// Units of 16 bytes: one run, the loops are straight.
+template <int BYTES, int UNITS>
+constexpr int kRun = BYTES == 16 || UNITS % 4 != 0 ? UNITS : 4;
+
+// A warp's queue of rows (or of its parts of rows) in shared memory, filled ahead
+// with asynchronous copies that hold no registers.  The slots of 16 bytes belong
+// to the warp alone, so no barrier of the block is needed.  Rows in 16-byte units:
+// a lane copies the units it will take.  Narrower units: the lanes of a row copy
+// the aligned 16 bytes around it together and take their units at any alignment.
+template <typename T, int BYTES, int UNITS, int WIDTH>
+struct RowQueue {
+  static constexpr bool WIDE = WIDTH == 32;
+  using Map = UnitMap<UNITS, WIDTH>;
+  using Raw = typename Unit<T, BYTES>::Raw;
+  uint32_t mine;         // shared address of this lane's slot 0 (16-byte units) or of its row's first
+  uint32_t stage_bytes;  // distance of a warp's stages
+  uint32_t row_bytes;
+
+  static __host__ __device__ __forceinline__ uint32_t slots_per_row(uint32_t width) {
+    return BYTES == 16 ? width * UNITS : (width * UNITS * BYTES + 15u) / 16u + 1u;
+  }
+  static __host__ __device__ __forceinline__ uint32_t slots_per_warp(uint32_t width) {
+    return 32u / width * slots_per_row(width);
+  }
+  // Shared memory of a block with queues for `operands` matrices.
+  static size_t bytes(uint32_t group, uint32_t operands) {
+    return size_t(kStages) * operands * (kPipeBlock / 32) * slots_per_warp(group < 32 ? group : 32) * 16;
+  }
+
+  // operand: which of the row's matrices this queue holds
+  __device__ __forceinline__ RowQueue(const uint4* shared, uint32_t operand, uint32_t operands,
+                                      const Map& map, uint32_t row_bytes_)
+      : row_bytes(row_bytes_) {
+    const uint32_t warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t slots = slots_per_warp(map.width);
+    stage_bytes = operands * warps * slots * 16u;
+    mine = static_cast<uint32_t>(__cvta_generic_to_shared(shared)) +
+           (operand * warps + warp) * slots * 16u +
+           (BYTES == 16 ? lane : lane / map.width * slots_per_row(map.width)) * 16u;
+  }
+
+  // Puts a row of the matrix [first, last) into a stage (null: none).
+  __device__ __forceinline__ void fill(uint32_t stage, const uint8_t* row, const Map& map,
+                                       const uint8_t* first, const uint8_t* last) const {
+    if (row == nullptr) return;
+    const uint32_t to = mine + stage * stage_bytes;
+    if constexpr (BYTES == 16) {
+      const uint8_t* from = row + (map.part + map.lane) * 16u;
+#pragma unroll
+      for (int c = 0; c < UNITS; ++c) {
+        if (map(c) < map.count) copy_async(to + c * 512u, from + (map(c) - map.lane) * 16u);
+      }
+    } else {
+      const int begin = int(map.part * BYTES), length = int(map.count * BYTES);
+      if (length == 0) return;
+      const int ahead = int(shift(row, map));
+      const uint8_t* from = row + begin - ahead;   // aligned
+      const int slots = (ahead + length + 15) >> 4;
+      const bool inside = from >= first && from + slots * 16 <= last;
+      constexpr int kRounds = WIDE ? (32 * UNITS * BYTES / 16 + 1 + 31) / 32 : 1;
+      if (inside) {
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int i = 0; i < kRounds; ++i) {
+            const int slot = i * 32 + int(map.lane);
+            if (slot < slots) copy_async(to + slot * 16, from + slot * 16);
+          }
+        } else {
+          for (int slot = int(map.lane); slot < slots; slot += int(map.width)) {
+            copy_async(to + slot * 16, from + slot * 16);
+          }
+        }
+      } else {
+        // at an end of the matrix nothing outside the row's own bytes is read
+        for (int slot = int(map.lane); slot < slots; slot += int(map.width)) {
+          const uint8_t* at = from + slot * 16;
+          if (at >= row && at + 16 <= row + row_bytes) copy_async(to + slot * 16, at);
+          else copy_elements(to + slot * 16, at, row);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void copy_elements(uint32_t to, const uint8_t* at, const uint8_t* row) const {
+#pragma unroll 1
+    for (uint32_t b = 0; b < 16u; b += uint32_t(sizeof(T))) {
+      if (at + b < row || at + b >= row + row_bytes) continue;
+      if constexpr (sizeof(T) == 4) {
+        const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(at + b));
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + b), "r"(v) : "memory");
+      } else {
+        const uint16_t v = __ldg(reinterpret_cast<const uint16_t*>(at + b));
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + b), "h"(v) : "memory");
+      }
+    }
+  }
+
+  // Where the warp's part of the row begins in its first slot.
+  __device__ __forceinline__ uint32_t shift(const uint8_t* row, const Map& map) const {
+    return BYTES == 16 ? 0u : (uint32_t(reinterpret_cast<uintptr_t>(row)) + map.part * BYTES) & 15u;
+  }
+
+  // Before the first take() from a stage and after the last.
+  __device__ __forceinline__ void arrive() const {
+    if (BYTES != 16) __syncwarp();   // other lanes' copies; 16-byte units are a lane's own
+  }
+
+  // Where the lane's first unit of the row in a stage is.
+  __device__ __forceinline__ uint32_t place(uint32_t stage, const uint8_t* row, const Map& map) const {
+    return mine + stage * stage_bytes + (BYTES == 16 ? 0u : shift(row, map) + map.lane * BYTES);
+  }
+  // Unit c of the lane, `from` place(), as floats; zeros where it has none.
+  static __device__ __forceinline__ void take(uint32_t from, int c, bool mine, const Map& map,
+                                              float (&f)[Unit<T, BYTES>::kElems]) {
+    Raw v;
+    const uint32_t at = from + (BYTES == 16 ? c * 512u : (map(c) - map.lane) * BYTES);
+    // inside the queue's slots even where the lane has no such unit
+    if constexpr (BYTES == 16) {
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                   : "r"(at)
+                   : "memory");
+    } else if constexpr (BYTES == 4) {
+      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    } else {
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+    }
+    Unit<T, BYTES>::unpack(v, f);
+#pragma unroll
+    for (int e = 0; e < Unit<T, BYTES>::kElems; ++e) f[e] = mine ? f[e] : 0.f;
+  }
+};
+
+// Weights or biases of the N columns from `column` on; `none` where there is no
+// pointer or no such column.  vec: the address is a multiple of 16.
+template <typename T, int N>
+__device__ __forceinline__ void load_params(const void* p, bool f32, bool vec, uint32_t column,
+                                            uint32_t dim, float none, float (&out)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) out[e] = none;
+  if (p == nullptr || column >= dim) return;   // units are whole: one column in, all in
+  if constexpr (N * sizeof(T) == 16) {
+    if (vec) {
+      if (f32) {
+        const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + column);
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+          const float4 v = __ldg(s + e / 4);
+          out[e] = v.x;
+          out[e + 1] = v.y;
+          out[e + 2] = v.z;
+          out[e + 3] = v.w;
+        }
+      } else {
+        Unit<T, 16>::unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p) + column)), out);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    out[e] = f32 ? static_cast<const float*>(p)[column + e]
+                 : to_float(static_cast<const T*>(p)[column + e]);
+  }
+}
+
+// The rows a group takes.
+struct RowDeal {
+  uint32_t row, step;   // the first row and the distance to the next
+  uint32_t warp_row;    // the first row of the warp's first group: the warp is done when it is
+
+  __device__ __forceinline__ explicit RowDeal(uint32_t group) {
+    const uint32_t groups = blockDim.x / group;
+    step = gridDim.x * groups;
+    row = blockIdx.x * groups + threadIdx.x / group;
+    warp_row = group >= 32u ? row : row - (threadIdx.x & 31u) / group;
+  }
+};
+
+// ---- host ----------------------------------------------------------------------
+
+// Threads on a row that hold `per_thread` units each.  Units of 16 bytes: whole
+// warps, or a power of two, two at least (a sector of 32 bytes).  Narrow units:
+// whole warps, or a quarter or half of one, widths the kernels know when they are built.
+inline uint32_t group_for(uint64_t units, uint32_t per_thread, uint32_t unit) {
+  const uint64_t threads = (units + per_thread - 1) / per_thread;
+  if (unit != 16) return threads <= 8 ? 8 : threads <= 16 ? 16 : uint32_t((threads + 31) / 32 * 32);
+  if (threads > 16) return uint32_t((threads + 31) / 32 * 32);
+  uint32_t group = 2;
+  while (group < threads) group <<= 1;
+  return group;
+}
+
+// Of the numbers of units per thread (ascending, 0 ends them) the one that leaves
+// the fewest places of the group empty, of equals the largest, for the fewest
+// threads; 0: the row is too long for a block.
+inline uint32_t fitting_units(uint64_t units, uint32_t unit, const uint32_t* choices) {
+  uint32_t best = 0;
+  uint64_t least = 0;
+  for (; *choices != 0; ++choices) {
+    const uint64_t group = group_for(units, *choices, unit);
+    if (group > uint32_t(kPipeBlock)) continue;
+    // narrow units: runs of four that no lane of the group has are left out
+    const uint64_t run = unit == 16 ? *choices : 4;
+    const uint64_t width = group < 32 ? group : 32, warps = group / width;
+    uint64_t runs = 0;
+    for (uint64_t w = 0; w < warps; ++w) {
+      const uint64_t from = w * width * *choices;
+      const uint64_t mine = from < units ? units - from : 0;
+      const uint64_t most = (mine + width * run - 1) / (width * run);
+      runs += most < *choices / run ? most : *choices / run;
+    }
+    const uint64_t places = runs * run * width;
+    if (best == 0 || places <= least) {
+      best = *choices;
+      least = places;
+    }
+  }
+  return best;
+}
+
+// Blocks of the kernels that stay on the device: as many as take part, at most
+// one per multiprocessor.
+inline uint32_t pipe_blocks(uint64_t n, uint32_t group) {
+  const uint32_t groups = kPipeBlock / group;
+  const uint64_t want = (n + groups - 1) / groups, most = uint64_t(sm_count());
+  return uint32_t(want < most ? want : most);
+}
+// Threads of such a block: whole groups.
+inline uint32_t pipe_threads(uint32_t group) { return kPipeBlock / group * group; }
+
+// A kernel that needs more shared memory than the default.
+template <typename Kernel>
+int allow_shared(Kernel kernel, size_t bytes) {
+  if (bytes <= 40 * 1024) return HKV_OK;   // the kernels' static part comes on top
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  if (e == cudaSuccess) return HKV_OK;
+  cudaGetLastError();
+  return rows_fail(HKV_ERR_CUDA, cudaGetErrorString(e));
+}
+
+int check_norm(uint64_t n, uint64_t dim, uint32_t value_kind, uint32_t param_kind, float eps) noexcept;
+
+}  // namespace hkv

@@ -1,5 +1,6 @@
-// What the row operators share (hkv_expert.cu, hkv_norm.cu): element types,
-// 16-byte chunks of rows at any alignment and the error text of their C entries.
+// What the row operators share (hkv_expert.cu, hkv_norm.cu, hkv_norm_backward.cu):
+// element types, the units rows are moved in, asynchronous copies and the error
+// text of their C entries.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -36,74 +37,108 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// ---- 16-byte chunks of rows ---------------------------------------------------
+// ---- units -------------------------------------------------------------------
 //
-// Every kernel moves rows in accesses of 16 bytes, whatever their alignment:
-// rows of odd lengths start at multiples of their element only, and accesses of
-// one 2-byte element ran at an eighth of the rate of 16 bytes (layer norm of
-// 65537 x 333 half: 100 us with them, 27 us with chunks).  A chunk at an
-// unaligned address is cut out of the two aligned ones it touches.
+// Rows are moved in units: 16 bytes where every row starts at a multiple of 16
+// and is a multiple of 16 long, else 4 bytes or one element, neighbouring units
+// in neighbouring lanes.  Narrow units cost instructions, not bandwidth, as long
+// as a thread's work per unit is the load, the arithmetic and the store and
+// nothing else.  (Cutting 16-byte chunks out of the aligned ones around them
+// instead, with their masks and shifts, took 1043 instructions per row of 1001
+// bfloat16 in layer norm, where the units take half of that.)
 
-template <typename T>
-constexpr int kChunkElems = 16 / int(sizeof(T));
-
-// A chunk's elements as floats, and back with one rounding each.
-__device__ __forceinline__ void unpack(const uint4& v, float (&f)[4], const float*) {
-  f[0] = __uint_as_float(v.x);
-  f[1] = __uint_as_float(v.y);
-  f[2] = __uint_as_float(v.z);
-  f[3] = __uint_as_float(v.w);
+// A 32-bit word's elements as floats, and back.
+__device__ __forceinline__ void unpack_word(uint32_t w, float* f, const float*) {
+  f[0] = __uint_as_float(w);
 }
-__device__ __forceinline__ void unpack(const uint4& v, float (&f)[8], const __half*) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    f[2 * i] = two.x;
-    f[2 * i + 1] = two.y;
-  }
+__device__ __forceinline__ void unpack_word(uint32_t w, float* f, const __half*) {
+  const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  f[0] = two.x;
+  f[1] = two.y;
 }
-__device__ __forceinline__ void unpack(const uint4& v, float (&f)[8], const __nv_bfloat16*) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {   // a bfloat16 is the upper half of its float
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-  }
+__device__ __forceinline__ void unpack_word(uint32_t w, float* f, const __nv_bfloat16*) {
+  f[0] = __uint_as_float(w << 16);   // a bfloat16 is the upper half of its float
+  f[1] = __uint_as_float(w & 0xFFFF0000u);
 }
-template <typename T>
-__device__ __forceinline__ void unpack(const uint4& v, float (&f)[kChunkElems<T>]) {
-  unpack(v, f, static_cast<const T*>(nullptr));
+__device__ __forceinline__ uint32_t pack_word(const float* f, const float*) {
+  return __float_as_uint(f[0]);
 }
-__device__ __forceinline__ uint4 pack(const float (&f)[4], const float*) {
-  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                    __float_as_uint(f[3]));
+__device__ __forceinline__ uint32_t pack_word(const float* f, const __half*) {
+  const __half2 two = __floats2half2_rn(f[0], f[1]);
+  return *reinterpret_cast<const uint32_t*>(&two);
 }
-__device__ __forceinline__ uint4 pack(const float (&f)[8], const __half*) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2 two = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&two);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ uint4 pack(const float (&f)[8], const __nv_bfloat16*) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 two = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&two);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-template <typename T>
-__device__ __forceinline__ uint4 pack(const float (&f)[kChunkElems<T>]) {
-  return pack(f, static_cast<const T*>(nullptr));
+__device__ __forceinline__ uint32_t pack_word(const float* f, const __nv_bfloat16*) {
+  const __nv_bfloat162 two = __floats2bfloat162_rn(f[0], f[1]);
+  return *reinterpret_cast<const uint32_t*>(&two);
 }
 
-// A matrix of rows: base, distance and count of the rows in bytes; every row
-// that is read lies in [first, last).
+template <typename T, int BYTES>
+struct Unit {
+  static constexpr int kElems = BYTES / int(sizeof(T));
+  using Raw = typename VecType<BYTES>::type;
+
+  static __device__ __forceinline__ void unpack(const Raw& v, float (&f)[kElems]) {
+    if constexpr (BYTES == 16) {
+      constexpr int kPer = 4 / int(sizeof(T));
+      unpack_word(v.x, f, static_cast<const T*>(nullptr));
+      unpack_word(v.y, f + kPer, static_cast<const T*>(nullptr));
+      unpack_word(v.z, f + 2 * kPer, static_cast<const T*>(nullptr));
+      unpack_word(v.w, f + 3 * kPer, static_cast<const T*>(nullptr));
+    } else if constexpr (BYTES == 4) {
+      unpack_word(v, f, static_cast<const T*>(nullptr));
+    } else {
+      T one;
+      *reinterpret_cast<Raw*>(&one) = v;
+      f[0] = to_float(one);
+    }
+  }
+  static __device__ __forceinline__ Raw pack(const float (&f)[kElems]) {
+    if constexpr (BYTES == 16) {
+      constexpr int kPer = 4 / int(sizeof(T));
+      return make_uint4(pack_word(f, static_cast<const T*>(nullptr)),
+                        pack_word(f + kPer, static_cast<const T*>(nullptr)),
+                        pack_word(f + 2 * kPer, static_cast<const T*>(nullptr)),
+                        pack_word(f + 3 * kPer, static_cast<const T*>(nullptr)));
+    } else if constexpr (BYTES == 4) {
+      return pack_word(f, static_cast<const T*>(nullptr));
+    } else {
+      const T one = from_float<T>(f[0]);
+      return *reinterpret_cast<const Raw*>(&one);
+    }
+  }
+};
+
+template <typename Raw>
+__device__ __forceinline__ Raw no_unit() {
+  return Raw{};
+}
+
+inline uint64_t address_bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+// Unit for rows whose addresses, strides and lengths in bytes have these bits (or
+// of all of them) set: 16, 4 or one element; 0 where an element would be split.
+inline uint32_t unit_bytes(uint64_t bits, uint32_t element) {
+  if (bits % 16 == 0) return 16;
+  if (bits % 4 == 0) return 4;
+  return bits % element == 0 ? element : 0;
+}
+
+// CALL(type, unit) for the unit and kind of a launch.
+#define HKV_FOR_UNIT(kind, unit, CALL)                      \
+  if ((kind) == hkv::kValueF32) {                           \
+    if ((unit) == 16) { CALL(float, 16); }                  \
+    else { CALL(float, 4); }                                \
+  } else if ((kind) == hkv::kValueF16) {                    \
+    if ((unit) == 16) { CALL(__half, 16); }                 \
+    else if ((unit) == 4) { CALL(__half, 4); }              \
+    else { CALL(__half, 2); }                               \
+  } else {                                                  \
+    if ((unit) == 16) { CALL(__nv_bfloat16, 16); }          \
+    else if ((unit) == 4) { CALL(__nv_bfloat16, 4); }       \
+    else { CALL(__nv_bfloat16, 2); }                        \
+  }
+
+// A matrix of rows that is read: every row lies in [first, last).
 struct RowsIn {
   const uint8_t* first;
   const uint8_t* last;
@@ -112,124 +147,6 @@ struct RowsIn {
 inline RowsIn rows_in(const void* base, uint64_t n, uint64_t stride, uint64_t row_bytes) {
   const uint8_t* p = static_cast<const uint8_t*>(base);
   return RowsIn{p, p + (n - 1) * stride + row_bytes, stride};
-}
-
-// Bytes s ... s + 15 of the 32 bytes lo, hi.
-__device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, uint32_t s) {
-  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-  const bool by8 = (s & 8u) != 0, by4 = (s & 4u) != 0;
-#pragma unroll
-  for (int i = 0; i < 6; ++i) w[i] = by8 ? w[i + 2] : w[i];
-#pragma unroll
-  for (int i = 0; i < 5; ++i) w[i] = by4 ? w[i + 1] : w[i];
-  const uint32_t bits = (s & 3u) * 8u;
-  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
-                    __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
-}
-
-// The 16 bytes at p, those inside [from, to) element by element (of G bytes) and
-// zeros for the others.
-template <int G>
-__device__ __forceinline__ uint4 pieces(const uint8_t* p, const uint8_t* from, const uint8_t* to) {
-  uint64_t half[2] = {0, 0};
-#pragma unroll 1
-  for (int b = 0; b < 16; b += G) {
-    if (p + b < from || p + b >= to) continue;
-    uint64_t piece;
-    if constexpr (G == 8) piece = *reinterpret_cast<const uint64_t*>(p + b);
-    else piece = *reinterpret_cast<const typename VecType<G>::type*>(p + b);
-    half[0] |= b < 8 ? piece << (8 * b) : 0;
-    half[1] |= b < 8 ? 0 : piece << (8 * (b - 8));
-  }
-  return make_uint4(uint32_t(half[0]), uint32_t(half[0] >> 32), uint32_t(half[1]),
-                    uint32_t(half[1] >> 32));
-}
-
-// The 16 bytes at an address p of any alignment, of which those inside a row
-// [from, to) matter (the others are anything).  The aligned chunks that hold them
-// are read whole where they lie inside the matrix [first, last), and element by
-// element (of G bytes) at its ends: nothing outside it is touched.  Loading and
-// cutting are two steps, without a branch in the first, so that the loads of
-// several chunks are in flight together.
-struct Cut {
-  uint4 lo, hi;
-  uint32_t s;
-  bool inside;
-
-  __device__ __forceinline__ void load(const uint8_t* p, const uint8_t* first, const uint8_t* last) {
-    s = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
-    const uint8_t* a = p - s;
-    inside = a >= first && a + (s ? 32 : 16) <= last;
-    lo = hi = make_uint4(0, 0, 0, 0);
-    if (inside) lo = __ldg(reinterpret_cast<const uint4*>(a));
-    if (inside && s) hi = __ldg(reinterpret_cast<const uint4*>(a + 16));
-  }
-  __device__ __forceinline__ void none() {
-    lo = hi = make_uint4(0, 0, 0, 0);
-    s = 0;
-    inside = true;
-  }
-  template <int G>
-  __device__ __forceinline__ uint4 get(const uint8_t* p, const uint8_t* from, const uint8_t* to) const {
-    if (inside) return s == 0 ? lo : shifted(lo, hi, s);
-    return pieces<G>(p, from, to);
-  }
-};
-
-__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
-  return i < 2 ? (i == 0 ? v.x : v.y) : (i == 2 ? v.z : v.w);
-}
-
-// Stores those bytes of the aligned 16 at row + off (v's) that lie in
-// [from, to) of the row, all three in bytes from its start.  A row's first and
-// last bytes go out in at most one piece of 8, 4, 2 and 1 bytes each, down to the
-// element size G; only rows that begin and end in the same 16 bytes are stored
-// element by element.
-template <int G>
-__device__ __forceinline__ void store_chunk(uint8_t* row, int off, const uint4& v, int from, int to) {
-  const int lo = from > off ? from - off : 0, hi = to - off < 16 ? to - off : 16;
-  uint8_t* q = row + off;
-  if (lo == 0 && hi == 16) {
-    *reinterpret_cast<uint4*>(q) = v;
-  } else if (hi <= lo) {
-    return;
-  } else if (hi == 16) {   // the row's head: pieces that end at the boundary
-    const int h = 16 - lo;
-    if (h & 8) *reinterpret_cast<uint2*>(q + 8) = make_uint2(v.z, v.w);
-    if (G <= 4 && (h & 4)) *reinterpret_cast<uint32_t*>(q + 12 - (h & 8)) = h & 8 ? v.y : v.w;
-    if (G <= 2 && (h & 2)) {
-      const int at = 14 - (h & 12);
-      *reinterpret_cast<uint16_t*>(q + at) = static_cast<uint16_t>(word_of(v, at >> 2) >> 16);
-    }
-    if (G <= 1 && (h & 1)) {
-      const int at = 15 - (h & 14);
-      q[at] = static_cast<uint8_t>(word_of(v, at >> 2) >> (8 * (at & 3)));
-    }
-  } else if (lo == 0) {    // its tail: pieces that start at the boundary
-    if (hi & 8) *reinterpret_cast<uint2*>(q) = make_uint2(v.x, v.y);
-    if (G <= 4 && (hi & 4)) *reinterpret_cast<uint32_t*>(q + (hi & 8)) = hi & 8 ? v.z : v.x;
-    if (G <= 2 && (hi & 2)) {
-      const int at = hi & 12;
-      *reinterpret_cast<uint16_t*>(q + at) = static_cast<uint16_t>(word_of(v, at >> 2));
-    }
-    if (G <= 1 && (hi & 1)) {
-      const int at = hi & 14;
-      q[at] = static_cast<uint8_t>(word_of(v, at >> 2) >> (8 * (at & 3)));
-    }
-  } else {
-#pragma unroll 1
-    for (int b = lo; b < hi; ++b) q[b] = static_cast<uint8_t>(word_of(v, b >> 2) >> (8 * (b & 3)));
-  }
-}
-
-// Or of addresses, strides and lengths in bytes: 16 divides all of them?
-inline bool whole_chunks(uint64_t bits) { return (bits & 15u) == 0; }
-inline uint64_t address_bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
-// The largest power of two up to 8 that divides `bits`.
-inline uint32_t piece_bytes(uint64_t bits) {
-  uint32_t v = 8;
-  while (v > 1 && (bits & (v - 1)) != 0) v >>= 1;
-  return v;
 }
 
 __device__ __forceinline__ void copy_async(uint32_t shared, const uint8_t* global) {
