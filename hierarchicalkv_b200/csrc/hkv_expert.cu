@@ -19,6 +19,8 @@
 //
 // The reference has no such operators; hkv_shard.cu groups keys by their
 // owner rank and moves whole rows by index, unordered inside an owner.
+#include <atomic>
+
 #include "hkv_rows.cuh"
 
 namespace hkv {
@@ -43,10 +45,20 @@ int rows_launched() noexcept {
   return e == cudaSuccess ? HKV_OK : rows_fail(HKV_ERR_CUDA, cudaGetErrorString(e));
 }
 
+// Asked of the driver once per device: the query takes longer than a launch.
 int sm_count() noexcept {
-  int dev = 0, sms = 148;
+  static std::atomic<int> known[64];
+  int dev = 0;
   cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (dev < 0 || dev >= 64) return 148;
+  int sms = known[dev].load(std::memory_order_relaxed);
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) {
+      cudaGetLastError();
+      return 148;
+    }
+    known[dev].store(sms, std::memory_order_relaxed);
+  }
   return sms;
 }
 
@@ -404,6 +416,10 @@ int launch_sort(uint64_t n, const ID* ids, uint32_t experts, int32_t* offsets, i
   const SortPlan p = plan_sort(n, experts);
   if (p.cluster != 0) {
     auto kernel = p.items == 1 ? sort_cluster_kernel<ID, 1> : sort_cluster_kernel<ID, 4>;
+    if (p.cluster == 1) {
+      kernel<<<1, p.block, 0, stream>>>(ids, n, experts, offsets, position, source);
+      return rows_launched();
+    }
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(p.cluster);
     config.blockDim = dim3(p.block);
@@ -639,6 +655,9 @@ __device__ __forceinline__ void combine_backward_step(
     float (&dot)[J]) {
   using U = Unit<T, BYTES>;
   typename U::Raw d[V], row[J][V];
+  float part[J];   // the step's share of the dot products, added to them at once
+#pragma unroll
+  for (int u = 0; u < J; ++u) part[u] = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     d[v] = no_unit<typename U::Raw>();
@@ -662,11 +681,15 @@ __device__ __forceinline__ void combine_backward_step(
       U::unpack(row[u][v], y);
 #pragma unroll
       for (int e = 0; e < U::kElems; ++e) {
-        if (a.ok[u]) dot[u] = fmaf(f[e], y[e], dot[u]);
+        part[u] = fmaf(f[e], y[e], part[u]);
         y[e] = a.w[u] * f[e];
       }
       if (a.ok[u] && (FULL || first + v * LANES < units)) to[u][first + v * LANES] = U::pack(y);
     }
+  }
+#pragma unroll
+  for (int u = 0; u < J; ++u) {
+    if (a.ok[u]) dot[u] += part[u];
   }
 }
 
@@ -704,7 +727,7 @@ __global__ void __launch_bounds__(256)
       const uint32_t own = threadIdx.x & (LANES - 1u);
 #pragma unroll 1
       for (uint32_t begin = (lane - own) * V; begin < units; begin += group * V) {
-        if (V > 1 && begin + LANES * V <= units) {
+        if (begin + LANES * V <= units) {
           combine_backward_step<T, BYTES, LANES, V, J, true>(begin + own, units, a, d_from, from, to, dot);
         } else {
           combine_backward_step<T, BYTES, LANES, V, J, false>(begin + own, units, a, d_from, from, to, dot);
@@ -749,10 +772,10 @@ uint32_t pow2_at_least(uint64_t v) {
   return p;
 }
 
-// Lanes on a part of a row of `units` units with `per_lane` units each: a warp, or
-// eight of its lanes, or two where the row has no more.
+// Lanes on a part of a row of `units` units with `per_lane` units each: a warp where
+// the row has units for all its lanes, else eight, or two where the row has no more.
 uint32_t lanes_for(uint64_t units, uint32_t per_lane) {
-  return units > 8ull * per_lane ? 32 : units > 2ull * per_lane ? 8 : 2;
+  return units >= 32ull * per_lane ? 32 : units > 2ull * per_lane ? 8 : 2;
 }
 RowParts row_parts(uint64_t units, uint32_t lanes, uint32_t per_lane) {
   RowParts p{};
@@ -934,10 +957,14 @@ int hkv_expert_combine_backward(uint64_t tokens, uint32_t top_k, uint64_t dim, u
                                    size);
   HKV_ROWS_CHECK(unit != 0, "a row does not start at a multiple of its element size");
   const uint64_t units = row_bytes / unit;
-  const uint32_t per_lane = unit == 16 ? 1 : 4;
+  const uint32_t per_lane = unit == 16 ? 2 : 8;
   const uint32_t lanes = lanes_for(units, per_lane);
-  uint32_t warps = pow2_at_least((units + 32 * per_lane - 1) / (32 * per_lane));
-  warps = warps > 8 ? 8 : warps;
+  // a warp goes over a whole row, which spreads what it does per row over the most
+  // units; more of them share one where there are too few tokens to fill the device
+  uint32_t warps = 1;
+  while (warps < 8 && units > 32ull * per_lane * warps && tokens * warps < uint64_t(sm_count()) * 16) {
+    warps <<= 1;
+  }
   unsigned grid = 0;
   rc = grid_of(tokens * (lanes == 32 ? warps * 32 : lanes), 256, &grid);
   if (rc != HKV_OK) return rc;
@@ -946,7 +973,7 @@ int hkv_expert_combine_backward(uint64_t tokens, uint32_t top_k, uint64_t dim, u
   const RowsIn in = rows_in(rows, tokens * top_k, rows_stride, row_bytes);
   const int32_t* kept = zero_rows_behind ? offsets + experts : nullptr;
 #define HKV_RUN(T, BYTES, LANES, J)                                                                 \
-  combine_backward_kernel<T, BYTES, LANES, (BYTES == 16 ? 1 : 4), J><<<grid, 256, 0, s>>>(          \
+  combine_backward_kernel<T, BYTES, LANES, (BYTES == 16 ? 2 : 8), J><<<grid, 256, 0, s>>>(          \
       tokens, top_k, uint32_t(units), warps, d_in, in, weights, weight_kind == kValueF32, position, \
       static_cast<uint8_t*>(d_rows), d_rows_stride, d_weights, kept)
 #define HKV_LANES(LANES)                            \

@@ -213,21 +213,21 @@ const uint32_t* unit_choices() {
   return BYTES == 16 ? whole : Unit<T, BYTES>::kElems == 2 ? pairs : ones;
 }
 
+template <typename T, int BYTES, int UNITS, int WIDTH>
+int launch_norm_width(const NormArgs& a, uint32_t group, const RowsIn& in, cudaStream_t stream) {
+  using Queue = RowQueue<T, BYTES, UNITS, WIDTH>;
+  constexpr auto kKernel = norm_pipe_kernel<T, BYTES, UNITS, WIDTH>;
+  const int rc = allow_shared<kKernel>();
+  if (rc != HKV_OK) return rc;
+  kKernel<<<pipe_blocks(a.n, group), pipe_threads(group), Queue::bytes(group, 1), stream>>>(a, group, in);
+  return HKV_OK;
+}
 template <typename T, int BYTES, int UNITS>
 int launch_norm_pipe(const NormArgs& a, uint32_t group, const RowsIn& in, cudaStream_t stream) {
-  auto launch = [&](auto kernel, size_t shared) {
-    const int rc = allow_shared(kernel, shared);
-    if (rc == HKV_OK) {
-      kernel<<<pipe_blocks(a.n, group), pipe_threads(group), shared, stream>>>(a, group, in);
-    }
-    return rc;
-  };
-#define HKV_CALL(WIDTH) \
-  launch(norm_pipe_kernel<T, BYTES, UNITS, WIDTH>, RowQueue<T, BYTES, UNITS, WIDTH>::bytes(group, 1))
-  if (group >= 32) return HKV_CALL(32);
-  if constexpr (BYTES == 16) return HKV_CALL(0);
-  else return group == 16 ? HKV_CALL(16) : HKV_CALL(8);
-#undef HKV_CALL
+  if (group >= 32) return launch_norm_width<T, BYTES, UNITS, 32>(a, group, in, stream);
+  if constexpr (BYTES == 16) return launch_norm_width<T, BYTES, UNITS, 0>(a, group, in, stream);
+  else if (group == 16) return launch_norm_width<T, BYTES, UNITS, 16>(a, group, in, stream);
+  else return launch_norm_width<T, BYTES, UNITS, 8>(a, group, in, stream);
 }
 
 template <typename T, int BYTES, int UNITS, int WIDTH>

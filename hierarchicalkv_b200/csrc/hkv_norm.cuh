@@ -2,6 +2,8 @@
 // over it, and the queues rows wait in.
 #pragma once
 
+#include <atomic>
+
 #include "hkv_norm.h"
 #include "hkv_rows.cuh"
 
@@ -326,15 +328,24 @@ inline uint32_t pipe_blocks(uint64_t n, uint32_t group) {
 // Threads of such a block: whole groups.
 inline uint32_t pipe_threads(uint32_t group) { return kPipeBlock / group * group; }
 
-// A kernel that needs more shared memory than the default.
-template <typename Kernel>
-int allow_shared(Kernel kernel, size_t bytes) {
-  if (bytes <= 40 * 1024) return HKV_OK;   // the kernels' static part comes on top
+// Allows a kernel the shared memory of any of its queues, once per device: the
+// call takes as long as a launch.
+constexpr size_t kMostShared = 220 * 1024;
+template <auto KERNEL>
+int allow_shared() noexcept {
+  static std::atomic<uint64_t> allowed{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+  if (allowed.load(std::memory_order_relaxed) & bit) return HKV_OK;
   const cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-  if (e == cudaSuccess) return HKV_OK;
-  cudaGetLastError();
-  return rows_fail(HKV_ERR_CUDA, cudaGetErrorString(e));
+      cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kMostShared));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return rows_fail(HKV_ERR_CUDA, cudaGetErrorString(e));
+  }
+  allowed.fetch_or(bit, std::memory_order_relaxed);
+  return HKV_OK;
 }
 
 int check_norm(uint64_t n, uint64_t dim, uint32_t value_kind, uint32_t param_kind, float eps) noexcept;

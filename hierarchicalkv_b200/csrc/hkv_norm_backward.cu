@@ -273,10 +273,10 @@ int launch_backward_pipe(const NormBackwardArgs& a, const NormBackwardPlan& p, f
   const size_t queue = RowQueue<T, BYTES, UNITS, WIDTH>::bytes(p.group, 2);
   const size_t columns = copies * a.dim * sizeof(float);
   const size_t shared = queue > columns ? queue : columns;
-  auto kernel = norm_backward_kernel<T, BYTES, UNITS, WIDTH>;
-  const int rc = allow_shared(kernel, shared);
+  constexpr auto kKernel = norm_backward_kernel<T, BYTES, UNITS, WIDTH>;
+  const int rc = allow_shared<kKernel>();
   if (rc != HKV_OK) return rc;
-  kernel<<<p.blocks, pipe_threads(p.group), shared, stream>>>(
+  kKernel<<<p.blocks, pipe_threads(p.group), shared, stream>>>(
       a, p.group, rows_in(a.x, a.n, a.x_stride, row_bytes), rows_in(a.dy, a.n, a.dy_stride, row_bytes),
       sums);
   return HKV_OK;
