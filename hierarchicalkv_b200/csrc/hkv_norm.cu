@@ -111,8 +111,10 @@ __global__ void __launch_bounds__(1024)
 
 // Many rows: the blocks stay on the device, their threads keep the weights of
 // their columns, and their groups take rows in turn out of the warps' queues.
+template <typename T, int BYTES, int UNITS>
+constexpr int kResident = UNITS * Unit<T, BYTES>::kElems <= 12 ? 2 : 1;   // blocks, by their registers
 template <typename T, int BYTES, int UNITS, int WIDTH>
-__global__ void __launch_bounds__(kPipeBlock, 1)
+__global__ void __launch_bounds__(kPipeBlock, (kResident<T, BYTES, UNITS>))
     norm_pipe_kernel(const NormArgs a, const uint32_t group, const RowsIn in) {
   using U = Unit<T, BYTES>;
   extern __shared__ uint4 slots[];
@@ -209,7 +211,7 @@ __global__ void __launch_bounds__(1024)
 // elements, weights and biases, 32 of each at most.
 template <typename T, int BYTES>
 const uint32_t* unit_choices() {
-  static const uint32_t whole[] = {2, 3, 4, 0}, pairs[] = {4, 8, 16, 0}, ones[] = {8, 16, 32, 0};
+  static const uint32_t whole[] = {2, 3, 4, 0}, pairs[] = {4, 8, 16, 0}, ones[] = {8, 12, 16, 32, 0};
   return BYTES == 16 ? whole : Unit<T, BYTES>::kElems == 2 ? pairs : ones;
 }
 
@@ -219,7 +221,7 @@ int launch_norm_width(const NormArgs& a, uint32_t group, const RowsIn& in, cudaS
   constexpr auto kKernel = norm_pipe_kernel<T, BYTES, UNITS, WIDTH>;
   const int rc = allow_shared<kKernel>();
   if (rc != HKV_OK) return rc;
-  kKernel<<<pipe_blocks(a.n, group), pipe_threads(group), Queue::bytes(group, 1), stream>>>(a, group, in);
+  kKernel<<<pipe_blocks(a.n, group, kResident<T, BYTES, UNITS>), pipe_threads(group), Queue::bytes(group, 1), stream>>>(a, group, in);
   return HKV_OK;
 }
 template <typename T, int BYTES, int UNITS>
@@ -273,6 +275,7 @@ int launch_norm_type(const NormArgs& a, cudaStream_t stream) {
   } else {
     switch (per_thread) {
       case 8: HKV_CALL(8);
+      case 12: HKV_CALL(12);
       case 16: HKV_CALL(16);
       default: HKV_CALL(32);
     }

@@ -2,8 +2,6 @@
 // over it, and the queues rows wait in.
 #pragma once
 
-#include <atomic>
-
 #include "hkv_norm.h"
 #include "hkv_rows.cuh"
 
@@ -174,22 +172,8 @@ struct RowQueue {
         for (int slot = int(map.lane); slot < slots; slot += int(map.width)) {
           const uint8_t* at = from + slot * 16;
           if (at >= row && at + 16 <= row + row_bytes) copy_async(to + slot * 16, at);
-          else copy_elements(to + slot * 16, at, row);
+          else copy_elements<sizeof(T)>(to + slot * 16, at, row, row + row_bytes);
         }
-      }
-    }
-  }
-
-  __device__ __forceinline__ void copy_elements(uint32_t to, const uint8_t* at, const uint8_t* row) const {
-#pragma unroll 1
-    for (uint32_t b = 0; b < 16u; b += uint32_t(sizeof(T))) {
-      if (at + b < row || at + b >= row + row_bytes) continue;
-      if constexpr (sizeof(T) == 4) {
-        const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(at + b));
-        asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + b), "r"(v) : "memory");
-      } else {
-        const uint16_t v = __ldg(reinterpret_cast<const uint16_t*>(at + b));
-        asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + b), "h"(v) : "memory");
       }
     }
   }
@@ -211,19 +195,8 @@ struct RowQueue {
   // Unit c of the lane, `from` place(), as floats; zeros where it has none.
   static __device__ __forceinline__ void take(uint32_t from, int c, bool mine, const Map& map,
                                               float (&f)[Unit<T, BYTES>::kElems]) {
-    Raw v;
-    const uint32_t at = from + (BYTES == 16 ? c * 512u : (map(c) - map.lane) * BYTES);
     // inside the queue's slots even where the lane has no such unit
-    if constexpr (BYTES == 16) {
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                   : "r"(at)
-                   : "memory");
-    } else if constexpr (BYTES == 4) {
-      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-    } else {
-      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
-    }
+    const Raw v = load_shared<BYTES>(from + (BYTES == 16 ? c * 512u : (map(c) - map.lane) * BYTES));
     Unit<T, BYTES>::unpack(v, f);
 #pragma unroll
     for (int e = 0; e < Unit<T, BYTES>::kElems; ++e) f[e] = mine ? f[e] : 0.f;
@@ -291,8 +264,12 @@ inline uint32_t group_for(uint64_t units, uint32_t per_thread, uint32_t unit) {
 }
 
 // Of the numbers of units per thread (ascending, 0 ends them) the one that leaves
-// the fewest places of the group empty, of equals the largest, for the fewest
-// threads; 0: the row is too long for a block.
+// the fewest places of the group empty; 0: the row is too long for a block.  A row
+// shared by warps counts one and a half times: its sums need barriers (65536 x
+// 1001 bf16: 126 us on four warps of 8 units per lane, 97 us on one of 32).  Of
+// equals the most units per thread, for the fewest threads; but narrow units that fit
+// a warp the fewest, for the registers (1 Mi x 33 half, gradient: 131 us with 8
+// units on eight lanes, 149 us with 16).
 inline uint32_t fitting_units(uint64_t units, uint32_t unit, const uint32_t* choices) {
   uint32_t best = 0;
   uint64_t least = 0;
@@ -309,44 +286,24 @@ inline uint32_t fitting_units(uint64_t units, uint32_t unit, const uint32_t* cho
       const uint64_t most = (mine + width * run - 1) / (width * run);
       runs += most < *choices / run ? most : *choices / run;
     }
-    const uint64_t places = runs * run * width;
-    if (best == 0 || places <= least) {
+    const uint64_t cost = runs * run * width * (warps > 1 ? 3 : 2);
+    if (best == 0 || cost < least || (cost == least && (unit == 16 || group > 32))) {
       best = *choices;
-      least = places;
+      least = cost;
     }
   }
   return best;
 }
 
 // Blocks of the kernels that stay on the device: as many as take part, at most
-// one per multiprocessor.
-inline uint32_t pipe_blocks(uint64_t n, uint32_t group) {
+// `resident` per multiprocessor.
+inline uint32_t pipe_blocks(uint64_t n, uint32_t group, int resident = 1) {
   const uint32_t groups = kPipeBlock / group;
-  const uint64_t want = (n + groups - 1) / groups, most = uint64_t(sm_count());
+  const uint64_t want = (n + groups - 1) / groups, most = uint64_t(sm_count()) * resident;
   return uint32_t(want < most ? want : most);
 }
 // Threads of such a block: whole groups.
 inline uint32_t pipe_threads(uint32_t group) { return kPipeBlock / group * group; }
-
-// Allows a kernel the shared memory of any of its queues, once per device: the
-// call takes as long as a launch.
-constexpr size_t kMostShared = 220 * 1024;
-template <auto KERNEL>
-int allow_shared() noexcept {
-  static std::atomic<uint64_t> allowed{0};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
-  if (allowed.load(std::memory_order_relaxed) & bit) return HKV_OK;
-  const cudaError_t e =
-      cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kMostShared));
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return rows_fail(HKV_ERR_CUDA, cudaGetErrorString(e));
-  }
-  allowed.fetch_or(bit, std::memory_order_relaxed);
-  return HKV_OK;
-}
 
 int check_norm(uint64_t n, uint64_t dim, uint32_t value_kind, uint32_t param_kind, float eps) noexcept;
 

@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 
 #include "../../include/hkv_b200.h"
@@ -149,6 +150,8 @@ inline RowsIn rows_in(const void* base, uint64_t n, uint64_t stride, uint64_t ro
   return RowsIn{p, p + (n - 1) * stride + row_bytes, stride};
 }
 
+int rows_fail(int code, const char* message) noexcept;
+
 __device__ __forceinline__ void copy_async(uint32_t shared, const uint8_t* global) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared), "l"(global) : "memory");
 }
@@ -158,7 +161,59 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-int rows_fail(int code, const char* message) noexcept;
+// Those of the 16 bytes at `at` that lie in [from, to), element by element.
+template <int ELEMENT>
+__device__ __forceinline__ void copy_elements(uint32_t shared, const uint8_t* at, const uint8_t* from,
+                                              const uint8_t* to) {
+#pragma unroll 1
+  for (uint32_t b = 0; b < 16u; b += ELEMENT) {
+    if (at + b < from || at + b >= to) continue;
+    if constexpr (ELEMENT == 4) {
+      const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(at + b));
+      asm volatile("st.shared.u32 [%0], %1;" ::"r"(shared + b), "r"(v) : "memory");
+    } else {
+      const uint16_t v = __ldg(reinterpret_cast<const uint16_t*>(at + b));
+      asm volatile("st.shared.u16 [%0], %1;" ::"r"(shared + b), "h"(v) : "memory");
+    }
+  }
+}
+
+template <int BYTES>
+__device__ __forceinline__ typename VecType<BYTES>::type load_shared(uint32_t at) {
+  typename VecType<BYTES>::type v;
+  if constexpr (BYTES == 16) {
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(at)
+                 : "memory");
+  } else if constexpr (BYTES == 4) {
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  } else {
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+  }
+  return v;
+}
+
+// Allows a kernel the shared memory of any of its queues, once per device: the
+// call takes as long as a launch.
+constexpr size_t kMostShared = 220 * 1024;
+template <auto KERNEL>
+int allow_shared() noexcept {
+  static std::atomic<uint64_t> allowed{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+  if (allowed.load(std::memory_order_relaxed) & bit) return HKV_OK;
+  const cudaError_t e =
+      cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kMostShared));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return rows_fail(HKV_ERR_CUDA, cudaGetErrorString(e));
+  }
+  allowed.fetch_or(bit, std::memory_order_relaxed);
+  return HKV_OK;
+}
+
 int rows_launched() noexcept;   // HKV_OK, or the launch's error
 int sm_count() noexcept;        // of the current device
 
