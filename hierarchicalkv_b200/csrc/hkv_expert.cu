@@ -461,6 +461,25 @@ int launch_sort(uint64_t n, const ID* ids, uint32_t experts, int32_t* offsets, i
 
 constexpr int kMoveBlock = 256;
 
+// How many units a lane takes at a time, and for how many assignments: as many
+// loads as keep the memory busy while the registers leave room for enough warps.
+// Measured, us, units x assignments (16-byte units; dispatch and combine 16384 tokens
+// of 8 rows of 4096 bf16, combine 300000 of 2 of 64 f32, gradient of combine 8192 of 8
+// of 2048 bf16 and 65536 of 2 of 128 f32; narrow units: 20000 of 6 of 1001 half):
+//   dispatch            2: 187    1: 195    4: 190    8: 190
+//   combine             2 x 2: 182, 37   1 x 4: 184    2 x 3: 177   4 x 2: -, 48
+//     narrow            8 x 1: 64   8 x 2: 66   4 x 2: 71   8 x 4: 82   16 x 2: 69
+//   gradient of combine 2 x 4: 93    2 x 2: 97, 29    1 x 4: 101    4 x 2: 97, 28
+//     narrow            4 x 2: 148   8 x 2: 164   8 x 1: 191   8 x 4: 221
+struct Shape {
+  int units, assigned;
+};
+constexpr Shape dispatch_shape(int unit) { return unit == 16 ? Shape{2, 0} : Shape{8, 0}; }
+constexpr Shape combine_shape(int unit) { return unit == 16 ? Shape{2, 2} : Shape{8, 1}; }
+constexpr Shape backward_shape(int unit, bool few) {
+  return unit != 16 || few ? Shape{4, 2} : Shape{2, 4};
+}
+
 // The part of a token's row that a group of LANES lanes takes: V units per lane.
 struct RowParts {
   uint32_t units;    // of a row
@@ -864,7 +883,7 @@ int hkv_expert_dispatch(uint64_t tokens, uint32_t top_k, uint64_t row_bytes, con
   const uint64_t bits = row_bytes | address_bits(x) | x_stride | address_bits(rows) | rows_stride;
   uint32_t unit = 16;
   while (bits % unit != 0) unit >>= 1;
-  const uint32_t per_lane = unit == 16 ? 4 : 8;
+  const uint32_t per_lane = dispatch_shape(unit).units;
   const uint32_t lanes = lanes_for(row_bytes / unit, per_lane);
   const RowParts parts = row_parts(row_bytes / unit, lanes, per_lane);
   unsigned grid = 0;
@@ -873,7 +892,7 @@ int hkv_expert_dispatch(uint64_t tokens, uint32_t top_k, uint64_t row_bytes, con
   const RowsIn in = rows_in(x, tokens, x_stride, row_bytes);
   const int32_t* kept = zero_rows_behind ? offsets + experts : nullptr;
 #define HKV_RUN(BYTES, LANES)                                                            \
-  dispatch_kernel<BYTES, LANES, (BYTES == 16 ? 4 : 8)>                                   \
+  dispatch_kernel<BYTES, LANES, dispatch_shape(BYTES).units>                             \
       <<<grid, kMoveBlock, 0, static_cast<cudaStream_t>(stream)>>>(                      \
           tokens, top_k, parts, in, position, static_cast<uint8_t*>(rows), rows_stride, kept)
 #define HKV_CALL(LANES)                     \
@@ -909,9 +928,7 @@ int hkv_expert_combine(uint64_t tokens, uint32_t top_k, uint64_t dim, uint32_t v
   const uint32_t unit =
       unit_bytes(row_bytes | address_bits(rows) | rows_stride | address_bits(out) | out_stride, size);
   HKV_ROWS_CHECK(unit != 0, "a row does not start at a multiple of its element size");
-  // with one or two assignments per token a lane takes more units instead, so that
-  // as many loads are in flight
-  const uint32_t per_lane = unit == 16 ? (top_k <= 2 ? 4 : 1) : 8;
+  const uint32_t per_lane = combine_shape(unit).units;
   const uint32_t lanes = lanes_for(row_bytes / unit, per_lane);
   const RowParts parts = row_parts(row_bytes / unit, lanes, per_lane);
   unsigned grid = 0;
@@ -919,13 +936,11 @@ int hkv_expert_combine(uint64_t tokens, uint32_t top_k, uint64_t dim, uint32_t v
   if (rc != HKV_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const RowsIn in = rows_in(rows, tokens * top_k, rows_stride, row_bytes);
-#define HKV_RUN(T, BYTES, LANES, V, J)                                                    \
-  combine_kernel<T, BYTES, LANES, V, J><<<grid, kMoveBlock, 0, s>>>(                      \
+#define HKV_LANES(LANES)                                                                  \
+  combine_kernel<RowT, kUnit, LANES, combine_shape(kUnit).units,                          \
+                 combine_shape(kUnit).assigned><<<grid, kMoveBlock, 0, s>>>(              \
       tokens, top_k, parts, in, weights, weight_kind == kValueF32, position,              \
       static_cast<uint8_t*>(out), out_stride)
-#define HKV_LANES(LANES)                                                 \
-  if (top_k <= 2) HKV_RUN(RowT, kUnit, LANES, (kUnit == 16 ? 4 : 8), 2); \
-  else HKV_RUN(RowT, kUnit, LANES, (kUnit == 16 ? 1 : 8), 4)
 #define HKV_CALL(T, BYTES)         \
   using RowT = T;                  \
   constexpr int kUnit = BYTES;     \
@@ -933,7 +948,6 @@ int hkv_expert_combine(uint64_t tokens, uint32_t top_k, uint64_t dim, uint32_t v
   HKV_FOR_UNIT(value_kind, unit, HKV_CALL)
 #undef HKV_CALL
 #undef HKV_LANES
-#undef HKV_RUN
   return rows_launched();
 }
 
@@ -961,12 +975,15 @@ int hkv_expert_combine_backward(uint64_t tokens, uint32_t top_k, uint64_t dim, u
                                    size);
   HKV_ROWS_CHECK(unit != 0, "a row does not start at a multiple of its element size");
   const uint64_t units = row_bytes / unit;
-  const uint32_t per_lane = unit == 16 ? 2 : 8;
+  const bool few = top_k <= 2;
+  const uint32_t per_lane = backward_shape(unit, few).units;
   const uint32_t lanes = lanes_for(units, per_lane);
-  // a warp goes over a whole row, which spreads what it does per row over the most
-  // units; more of them share one where there are too few tokens to fill the device
+  // a warp goes over four steps of a row at least, which spreads what it does per
+  // row; more warps share one where there are too few tokens to fill the device
+  const uint64_t step = 32ull * per_lane;
   uint32_t warps = 1;
-  while (warps < 8 && units > 32ull * per_lane * warps && tokens * warps < uint64_t(sm_count()) * 16) {
+  while (warps < 8 && (units >= step * 8 * warps ||
+                       (units > step * warps && tokens * warps < uint64_t(sm_count()) * 16))) {
     warps <<= 1;
   }
   unsigned grid = 0;
@@ -976,13 +993,14 @@ int hkv_expert_combine_backward(uint64_t tokens, uint32_t top_k, uint64_t dim, u
   const RowsIn d_in = rows_in(d_out, tokens, d_out_stride, row_bytes);
   const RowsIn in = rows_in(rows, tokens * top_k, rows_stride, row_bytes);
   const int32_t* kept = zero_rows_behind ? offsets + experts : nullptr;
-#define HKV_RUN(T, BYTES, LANES, J)                                                                 \
-  combine_backward_kernel<T, BYTES, LANES, (BYTES == 16 ? 2 : 8), J><<<grid, 256, 0, s>>>(          \
+#define HKV_RUN(T, BYTES, LANES, FEW)                                                               \
+  combine_backward_kernel<T, BYTES, LANES, backward_shape(BYTES, FEW).units,                        \
+                          backward_shape(BYTES, FEW).assigned><<<grid, 256, 0, s>>>(                \
       tokens, top_k, uint32_t(units), warps, d_in, in, weights, weight_kind == kValueF32, position, \
       static_cast<uint8_t*>(d_rows), d_rows_stride, d_weights, kept)
-#define HKV_LANES(LANES)                            \
-  if (top_k <= 2) HKV_RUN(RowT, kUnit, LANES, 2);   \
-  else HKV_RUN(RowT, kUnit, LANES, 4)
+#define HKV_LANES(LANES)                                       \
+  if (kUnit != 16 || few) HKV_RUN(RowT, kUnit, LANES, true);   \
+  else HKV_RUN(RowT, kUnit, LANES, (kUnit != 16))
 #define HKV_CALL(T, BYTES)         \
   using RowT = T;                  \
   constexpr int kUnit = BYTES;     \
