@@ -465,16 +465,22 @@ constexpr int kMoveBlock = 256;
 // loads as keep the memory busy while the registers leave room for enough warps.
 // Measured, us, units x assignments (16-byte units; dispatch and combine 16384 tokens
 // of 8 rows of 4096 bf16, combine 300000 of 2 of 64 f32, gradient of combine 8192 of 8
-// of 2048 bf16 and 65536 of 2 of 128 f32; narrow units: 20000 of 6 of 1001 half):
+// of 2048 bf16 and 65536 of 2 of 128 f32; units of 2: 20000 of 6 of 1001 half; units
+// of 4: 30000 of 4 of 334 bf16 and 333 f32):
 //   dispatch            2: 187    1: 195    4: 190    8: 190
+//     units of 4        4: 17.6   8: 21.2
 //   combine             2 x 2: 182, 37   1 x 4: 184    2 x 3: 177   4 x 2: -, 48
-//     narrow            8 x 1: 64   8 x 2: 66   4 x 2: 71   8 x 4: 82   16 x 2: 69
+//     units of 2        8 x 1: 64   8 x 2: 66   4 x 1: 94   4 x 2: 71   8 x 4: 82   12 x 1: 116
+//     units of 4        8 x 1: 30, 36   8 x 2: 29, 35   4 x 2: 28, 36   4 x 1: 29, 44   4 x 4: 26, 42
 //   gradient of combine 2 x 4: 93    2 x 2: 97, 29    1 x 4: 101    4 x 2: 97, 28
-//     narrow            4 x 2: 148   8 x 2: 164   8 x 1: 191   8 x 4: 221
+//     units of 2        4 x 2: 149   4 x 1: 150   8 x 2: 164   8 x 1: 191   2 x 2: 208   8 x 4: 221
+//     units of 4        4 x 2: 45, 73   2 x 2: 47, 85   4 x 1: 50, 80   6 x 1: 50, 81   4 x 3: 50, 77
 struct Shape {
   int units, assigned;
 };
-constexpr Shape dispatch_shape(int unit) { return unit == 16 ? Shape{2, 0} : Shape{8, 0}; }
+constexpr Shape dispatch_shape(int unit) {
+  return unit == 16 ? Shape{2, 0} : unit == 4 ? Shape{4, 0} : Shape{8, 0};
+}
 constexpr Shape combine_shape(int unit) { return unit == 16 ? Shape{2, 2} : Shape{8, 1}; }
 constexpr Shape backward_shape(int unit, bool few) {
   return unit != 16 || few ? Shape{4, 2} : Shape{2, 4};
@@ -654,7 +660,7 @@ __global__ void __launch_bounds__(kMoveBlock)
   const MyPart<LANES, V> my(parts);
   if (my.token >= tokens) return;
   const uint64_t n = tokens * top_k;
-  if (V > 1 && my.full) {
+  if (my.full) {
     combine_part<T, BYTES, LANES, V, J, true>(my, n, top_k, rows, weights, weights_f32, position, out,
                                               out_stride);
   } else {
