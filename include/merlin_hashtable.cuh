@@ -624,6 +624,21 @@ class HashTable : public HashTableBase<K, V, S> {
     detail::rethrow(hkv_find_host(table_, n, u(keys), values, founds, w(scores), stream));
   }
 
+  /**
+   * @brief find whose rows pass through layer norm on their way into `values`
+   * (not in the reference): they are normalised straight from the table.  V is
+   * float, __half or __nv_bfloat16; `weight` and `bias` (dim elements of V or
+   * float, null: ones / zeros) and `mean` / `rstd` (n floats, null: not kept)
+   * are device pointers.  Rows of misses are left as they are.
+   */
+  template <class P = V>
+  void find_layer_norm(const size_type n, const key_type* keys, const P* weight, const P* bias,
+                       const float eps, value_type* values, bool* founds, float* mean = nullptr,
+                       float* rstd = nullptr, cudaStream_t stream = 0) const {
+    detail::rethrow(hkv_find_layer_norm(table_, n, u(keys), weight, bias, detail::value_kind_of<P>(),
+                                        eps, values, founds, mean, rstd, stream));
+  }
+
   void find(const size_type n, const key_type* keys, value_type* values, key_type* missed_keys,
             int* missed_indices, int* missed_size, score_type* scores = nullptr,
             cudaStream_t stream = 0) const override {

@@ -1,0 +1,28 @@
+"""Runs the C++ client of HashTable::find_layer_norm (tests/cpp/rows_test.cu)."""
+import os
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+BINARY = os.path.join(ROOT, "tests", "cpp", "build", "rows_test")
+
+
+def build():
+    r = subprocess.run(["make", "-C", os.path.join(ROOT, "tests", "cpp"), "build/rows_test"], capture_output=True,
+                       text=True)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+@pytest.mark.gpu
+def test_cpp_client_of_find_layer_norm(product_lib):
+    if not os.path.exists(BINARY):
+        build()
+    r = subprocess.run([BINARY], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert "PASS" in r.stdout
+
+
+def test_cpp_client_compiles(product_lib):
+    build()
+    assert os.path.exists(BINARY)
