@@ -11,7 +11,10 @@
 // Rows are given by base and stride, or (the pointer form) by one address per
 // row, as find* returns them: rows are then normalised straight from where the
 // table keeps them, rows in pinned host memory included, and the output rows of
-// misses (null addresses) are left as they are, as find leaves them.
+// misses (null addresses) are left as they are, as find leaves them.  So are those
+// of addresses that the row's length does not allow: a row of whole 16-byte (else
+// 4-byte) units starts at a multiple of the unit, as the table's rows do, and the
+// host cannot see the addresses to refuse them.
 //
 // The reference has no such operator; what it hands to one are the rows of
 // find (include/merlin_hashtable.cuh:2464-2577) and find* (2729-2787).
@@ -22,6 +25,11 @@ namespace hkv {
 namespace {
 
 constexpr int kNormBlock = 256;   // of a batch of few rows; more where a row needs more
+
+__device__ __forceinline__ const uint8_t* row_address(const NormArgs& a, uint64_t r) {
+  const void* row = a.row_ptrs[r];
+  return (reinterpret_cast<uintptr_t>(row) & a.row_mask) != 0 ? nullptr : static_cast<const uint8_t*>(row);
+}
 
 // Normalises the row whose elements are in x, and whose sum over the thread's is
 // `sum`, and stores it; row == nullptr: none.  w, b: the thread's columns of weight
@@ -87,7 +95,7 @@ __global__ void __launch_bounds__(1024)
   const UnitMap<UNITS, WIDTH> map(group, uint32_t(a.dim) / U::kElems);
   const uint8_t* row = nullptr;
   if (r < a.n) {
-    row = a.row_ptrs != nullptr ? static_cast<const uint8_t*>(a.row_ptrs[r]) : in.first + r * in.stride;
+    row = a.row_ptrs != nullptr ? row_address(a, r) : in.first + r * in.stride;
   }
   typename U::Raw raw[UNITS];
 #pragma unroll
@@ -129,8 +137,7 @@ __global__ void __launch_bounds__(kPipeBlock, (kResident<T, BYTES, UNITS>))
   uint32_t r = deal.row;
   auto address = [&](uint32_t row) -> const uint8_t* {
     if (row >= n) return nullptr;
-    return a.row_ptrs != nullptr ? static_cast<const uint8_t*>(a.row_ptrs[row])
-                                 : in.first + row * in.stride;
+    return a.row_ptrs != nullptr ? row_address(a, row) : in.first + row * in.stride;
   };
   auto fill = [&](uint32_t stage, const uint8_t* row) {
     const bool by_address = a.row_ptrs != nullptr;
@@ -178,9 +185,8 @@ __global__ void __launch_bounds__(1024)
   GroupSum<1, 32> group_sum(blockDim.x, scratch);
   const uint32_t dim = uint32_t(a.dim);
   for (uint64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
-    const T* row = a.row_ptrs != nullptr
-                       ? static_cast<const T*>(a.row_ptrs[r])
-                       : reinterpret_cast<const T*>(static_cast<const uint8_t*>(a.x) + r * a.x_stride);
+    const T* row = reinterpret_cast<const T*>(
+        a.row_ptrs != nullptr ? row_address(a, r) : static_cast<const uint8_t*>(a.x) + r * a.x_stride);
     if (row == nullptr) continue;
     float sum[1] = {0.f};
     for (uint32_t i = threadIdx.x; i < dim; i += blockDim.x) sum[0] += to_float(row[i]);
@@ -221,7 +227,8 @@ int launch_norm_width(const NormArgs& a, uint32_t group, const RowsIn& in, cudaS
   constexpr auto kKernel = norm_pipe_kernel<T, BYTES, UNITS, WIDTH>;
   const int rc = allow_shared<kKernel>();
   if (rc != HKV_OK) return rc;
-  kKernel<<<pipe_blocks(a.n, group, kResident<T, BYTES, UNITS>), pipe_threads(group), Queue::bytes(group, 1), stream>>>(a, group, in);
+  kKernel<<<pipe_blocks(a.n, group, kResident<T, BYTES, UNITS>), pipe_threads(group),
+            Queue::bytes(group, 1), stream>>>(a, group, in);
   return HKV_OK;
 }
 template <typename T, int BYTES, int UNITS>
@@ -254,8 +261,13 @@ int launch_norm_type(const NormArgs& a, cudaStream_t stream) {
   // group of as many threads as the row has units (a few units each in long rows)
   // takes one
   if (a.n <= uint64_t(sm_count()) * (kPipeBlock / group) * 2) {
-    if (units <= 16 && BYTES == 16) launch_norm_few<T, BYTES, 1, 0>(a, group_for(units, 1, BYTES), in, stream);
-    else if (units <= 1024) launch_norm_few<T, BYTES, 1, 32>(a, uint32_t((units + 31) / 32 * 32), in, stream);
+    if constexpr (BYTES == 16) {
+      if (units <= 16) {
+        launch_norm_few<T, BYTES, 1, 0>(a, group_for(units, 1, BYTES), in, stream);
+        return HKV_OK;
+      }
+    }
+    if (units <= 1024) launch_norm_few<T, BYTES, 1, 32>(a, uint32_t((units + 31) / 32 * 32), in, stream);
     else if (units <= 2048) launch_norm_few<T, BYTES, 2, 32>(a, group_for(units, 2, BYTES), in, stream);
     if (units <= 2048) return HKV_OK;
   }
@@ -295,13 +307,12 @@ int check_norm(uint64_t n, uint64_t dim, uint32_t value_kind, uint32_t param_kin
   return HKV_OK;
 }
 
-int launch_norm(const NormArgs& args, uint32_t value_kind, cudaStream_t stream) {
+int launch_norm(NormArgs args, uint32_t value_kind, cudaStream_t stream) {
   const uint32_t size = row_kind_size(value_kind);
   uint64_t bits = args.dim * size | address_bits(args.y) | args.y_stride;
-  // the pointer form's addresses are on the device: table rows start at
-  // multiples of the widest access their length allows
   if (args.row_ptrs == nullptr) bits |= address_bits(args.x) | args.x_stride;
   const uint32_t unit = unit_bytes(bits, size);
+  args.row_mask = unit_bytes(args.dim * size, size) - 1u;
   HKV_ROWS_CHECK(unit != 0, "a row does not start at a multiple of its element size");
   int rc = HKV_OK;
 #define HKV_CALL(T, BYTES) rc = launch_norm_type<T, BYTES>(args, stream)

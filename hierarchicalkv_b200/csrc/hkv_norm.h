@@ -13,6 +13,7 @@ struct NormArgs {
   const void* x = nullptr;                 // rows by base and stride ...
   uint64_t x_stride = 0;
   const void* const* row_ptrs = nullptr;   // ... or one address each; null: leave the output row
+  uint32_t row_mask = 0;                   // as for null where an address has one of these bits
   const void* weight = nullptr;            // null: ones
   const void* bias = nullptr;              // null: zeros
   bool params_f32 = false;                 // weight and bias are float, else the rows' type
@@ -45,6 +46,6 @@ struct NormBackwardArgs {
 };
 
 // HKV_OK or the error; value_kind is one of the row kinds.
-int launch_norm(const NormArgs& args, uint32_t value_kind, cudaStream_t stream);
+int launch_norm(NormArgs args, uint32_t value_kind, cudaStream_t stream);
 
 }  // namespace hkv

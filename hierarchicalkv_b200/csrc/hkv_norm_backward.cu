@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kPipeBlock, 1)
     x_queue.arrive();
     float xhat[UNITS][kElems], g[UNITS][kElems];
     float sum[2] = {0.f, 0.f};
-if (r < n) {
+    if (r < n) {
       const uint32_t x_from = x_queue.place(stage, x_row(r), map);
       const uint32_t dy_from = dy_queue.place(stage, dy_row(r), map);
       map.template each<kRun<BYTES, UNITS>>([&](int c, bool mine) {

@@ -62,6 +62,8 @@ def _run_there(fn, t: torch.Tensor, stream, *args):
             return fn(*args)
         if isinstance(stream, int):
             stream = torch.cuda.ExternalStream(stream, t.device) if stream else torch.cuda.default_stream(t.device)
+        elif stream.device != t.device:
+            raise ValueError(f"stream must be one of {t.device}, where the tensors are")
         with torch.cuda.stream(stream):
             return fn(*args)
 
@@ -133,6 +135,13 @@ def _statistic(t: Optional[torch.Tensor], name: str, n: int, like: torch.Tensor)
     if t.dtype is not _F32 or t.numel() < n or not t.is_contiguous() or t.get_device() != like.get_device():
         raise ValueError(f"{name} must be contiguous, on the device of the rows and hold {n} float32 elements")
     return t.data_ptr()
+
+
+def _weights(t: Optional[torch.Tensor], order: ExpertOrder, like: torch.Tensor):
+    """Address of the weights of an order's assignments."""
+    if t is not None and t.shape != order[1].shape:
+        raise ValueError("weights must have the shape of order.position, [tokens, top_k]")
+    return _vector(t, "weights", order[1].numel(), like)
 
 
 def _order(order: ExpertOrder, like: torch.Tensor):
@@ -211,7 +220,7 @@ def _combine(rows, weights, order, out):
     tokens, top_k, _, _, position = _order(order, rows)
     if n != tokens * top_k:
         raise ValueError("rows must have a row for every assignment of the order")
-    w = _vector(weights, "weights", n, rows)
+    w = _weights(weights, order, rows)
     out, out_stride = _out(out, tokens, dim, rows)
     lib = load_library()
     rc = lib.hkv_expert_combine(
@@ -254,7 +263,7 @@ def expert_combine_backward(d_out: torch.Tensor, rows: torch.Tensor, weights: to
     if n != tokens:
         raise ValueError("d_out must have a row for every token of the order")
     stride = _more_rows(rows, "rows", tokens * top_k, dim, d_out)
-    w = _vector(weights, "weights", tokens * top_k, rows)
+    w = _weights(weights, order, rows)
     new = out is None
     out, out_stride = _out(out, tokens * top_k, dim, rows)
     d_weights = weights.new_empty((tokens, top_k))
@@ -311,7 +320,9 @@ def layer_norm_ptr(n: int, row_ptrs: torch.Tensor, out: torch.Tensor,
     fills them, rows of the type and length of ``out``'s.  The rows are read where
     the table keeps them and must not change meanwhile (HashTable.find_layer_norm
     holds the table's lock over both steps).  Null addresses leave their row of
-    ``out`` (and of ``mean`` and ``rstd``, float32, optional) as it is."""
+    ``out`` (and of ``mean`` and ``rstd``, float32, optional) as it is, and so do
+    addresses where no table row of this length starts: those that are no multiple
+    of 16 bytes where the row's length is one, else of 4, else of the element."""
     if _elsewhere(out, stream):
         return _run_there(layer_norm_ptr, out, stream, n, row_ptrs, out, weight, bias, eps, mean, rstd)
     rows, dim, stride, kind = _float_rows(out, "out")

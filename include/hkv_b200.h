@@ -587,9 +587,10 @@ HKV_API int hkv_layer_norm(uint64_t n, uint64_t dim, uint32_t value_kind, const 
                            float* rstd, hkv_stream stream);
 /* The same on rows by address, as find* returns them
  * (include/merlin_hashtable.cuh:2729-2787): the rows are read where the table keeps
- * them and must stay valid and unchanged until the call has run.  Each address
- * is null or a multiple of the widest of 16, 8, 4, 2 bytes that divides the row's
- * length.  Null addresses (misses) leave y, mean and rstd of their row as they are. */
+ * them and must stay valid and unchanged until the call has run.  Null addresses
+ * (misses) leave y, mean and rstd of their row as they are, and so does an address
+ * at which a row of this length does not start: it has to be a multiple of 16
+ * bytes if the row's length is, else of 4 if that is, else of the element size. */
 HKV_API int hkv_layer_norm_ptr(uint64_t n, uint64_t dim, uint32_t value_kind,
                                const void* const* row_ptrs, const void* weight, const void* bias,
                                uint32_t param_kind, float eps, void* y, uint64_t y_stride,

@@ -9,6 +9,7 @@ exchanges in the warp and 32 warps follow.  Results are rounded once, by at most
 half a step of their type (finfo.eps / 2 of the value, or half the smallest
 subnormal)."""
 import os
+import subprocess
 import sys
 
 import numpy as np
@@ -485,6 +486,25 @@ def test_layer_norm_of_rows_by_address(n, dim, dtype):
     assert (mean[miss] == 5).all() and (rstd[miss] == 5).all()
 
 
+@SIZED
+@pytest.mark.parametrize("n,dim", [(7, 64), (7, 66), (7, 1025), (5000, 64), (5000, 66), (3, 20000)])
+def test_addresses_where_no_row_starts_leave_their_row(n, dim, dtype):
+    """An address that a row of this length cannot have counts as null: nothing is
+    read there."""
+    size = torch.finfo(dtype).bits // 8
+    align = 16 if dim * size % 16 == 0 else 4 if dim * size % 4 == 0 else size
+    table = norm_rows(n + 1, dim, 9, dtype)
+    ptrs = table.data_ptr() + torch.arange(n, device="cuda") * (dim * size)
+    odd = torch.arange(n, device="cuda") % 3 == 1
+    ptrs[odd] += torch.arange(n, device="cuda")[odd] % (align - 1) + 1
+    out = torch.full((n, dim), 5, dtype=dtype, device="cuda")
+    mean, rstd = torch.full((n,), 5.0, device="cuda"), torch.full((n,), 5.0, device="cuda")
+    hkv.layer_norm_ptr(n, ptrs, out, mean=mean, rstd=rstd)
+    want, m, r = hkv.layer_norm(table[:n])
+    assert torch.equal(out[~odd], want[~odd]) and torch.equal(mean[~odd], m[~odd]) and torch.equal(rstd[~odd], r[~odd])
+    assert (out[odd] == 5).all() and (mean[odd] == 5).all() and (rstd[odd] == 5).all()
+
+
 def make_table(dim, dtype=torch.float32, capacity=128 * 64, hbm=1 << 30, **options):
     t = hkv.HashTable(hkv.EvictStrategy.kLru, value_dtype=dtype)
     t.init(hkv.HashTableOptions(init_capacity=capacity, max_capacity=capacity, max_hbm_for_vectors=hbm, dim=dim,
@@ -601,6 +621,66 @@ def test_streams_by_object_and_by_handle():
         got = norm_pass(x, w, w, dy)
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_calls_that_do_not_fit_are_refused():
+    x, ids = randn((6, 8), 1), make_ids(6, 2, 3)
+    order = hkv.expert_sort(ids, 3)
+    rows, w = hkv.expert_dispatch(x, order), randn((6, 2), 2)
+
+    class Elsewhere:                                       # a stream of another GPU, without one
+        device = torch.device("cuda", torch.cuda.device_count())
+
+    with pytest.raises(ValueError, match="stream"):
+        hkv.layer_norm(x, stream=Elsewhere())
+    for bad in (w.t().contiguous(), w[:5], w.view(-1)):
+        with pytest.raises(ValueError, match="shape of order.position"):
+            hkv.expert_combine(rows, bad, order)
+        with pytest.raises(ValueError, match="shape of order.position"):
+            hkv.expert_combine_backward(x, rows, bad, order)
+    for bad in (x[:5], x[:, :7], x.half(), torch.zeros((12, 8))):
+        with pytest.raises(ValueError):
+            hkv.expert_combine_backward(x, bad, w, order)
+        with pytest.raises(ValueError):
+            hkv.expert_dispatch(x, order, out=bad)
+        with pytest.raises(ValueError):
+            hkv.layer_norm(x, out=bad)
+        with pytest.raises(ValueError):
+            hkv.layer_norm_backward(bad, x, None, w[:, 0].contiguous(), w[:, 1].contiguous())
+    with pytest.raises(ValueError, match="overlap"):
+        hkv.layer_norm(x, out=x[:1].expand(6, 8))
+    with pytest.raises(ValueError, match="top_k"):
+        hkv.expert_dispatch(x, hkv.ExpertOrder(order.offsets, torch.zeros((6, 65), dtype=torch.int32, device="cuda"), None))
+
+
+FIRST_CALLS = """
+import torch
+import hierarchicalkv_b200 as hkv
+hkv.load_library()
+x = torch.randn((5000, 64), device="cuda")
+w, ids = torch.ones(64, device="cuda"), torch.randint(0, 6, (5000, 2), device="cuda")
+wt = torch.ones((5000, 2), device="cuda")
+def calls():
+    y, mean, rstd = hkv.layer_norm(x, w, w)
+    order = hkv.expert_sort(ids, 6)
+    rows = hkv.expert_dispatch(y, order)
+    out = hkv.expert_combine(rows, wt, order)
+    d_rows, d_wt = hkv.expert_combine_backward(out, rows, wt, order)
+    dy = hkv.expert_dispatch_backward(d_rows, order)
+    return [y, mean, rstd, *order, rows, out, d_rows, d_wt, dy, *hkv.layer_norm_backward(dy, x, w, mean, rstd)]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = calls()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, calls()))
+print("same")
+"""
+
+
+def test_a_process_s_first_calls_may_be_captured():
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
 
 
 def test_captured_calls_replay_on_new_inputs_and_graphs_do_not_share_scratch():
