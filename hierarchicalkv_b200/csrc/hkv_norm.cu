@@ -26,8 +26,7 @@ namespace {
 
 constexpr int kNormBlock = 256;   // of a batch of few rows; more where a row needs more
 
-__device__ __forceinline__ const uint8_t* row_address(const NormArgs& a, uint64_t r) {
-  const void* row = a.row_ptrs[r];
+__device__ __forceinline__ const uint8_t* valid_row(const NormArgs& a, const void* row) {
   return (reinterpret_cast<uintptr_t>(row) & a.row_mask) != 0 ? nullptr : static_cast<const uint8_t*>(row);
 }
 
@@ -45,21 +44,25 @@ __device__ __forceinline__ void norm_row(const NormArgs& a, uint32_t r, const ui
   float total[1] = {sum};
   group_sum(total);
   const float mean = total[0] * a.inv_dim;
-  float sq[1] = {0.f};
+  Partial squares;
   if (row != nullptr) {
     map.template each<kRun<BYTES, UNITS>>([&](int c, bool mine) {
 #pragma unroll
       for (int e = 0; e < U::kElems; ++e) {
         x[c][e] -= mean;
-        if (mine) sq[0] = fmaf(x[c][e], x[c][e], sq[0]);
+        if (mine) {
+          float& sq = squares.part[(c * U::kElems + e) % 4];
+          sq = fmaf(x[c][e], x[c][e], sq);
+        }
       }
     });
   }
+  float sq[1] = {squares.sum()};
   group_sum(sq);
   const float rstd = rsqrtf(fmaf(sq[0], a.inv_dim, a.eps));
   if (row == nullptr) return;
-  auto* to = reinterpret_cast<typename U::Raw*>(static_cast<uint8_t*>(a.y) + r * a.y_stride) +
-             (map.part + map.lane);
+  auto* to = keep(reinterpret_cast<typename U::Raw*>(static_cast<uint8_t*>(a.y) + r * a.y_stride) +
+                  (map.part + map.lane));
   map.template each<kRun<BYTES, UNITS>>([&](int c, bool mine) {
 #pragma unroll
     for (int e = 0; e < U::kElems; ++e) x[c][e] = fmaf(x[c][e] * rstd, w[c][e], b[c][e]);
@@ -68,19 +71,6 @@ __device__ __forceinline__ void norm_row(const NormArgs& a, uint32_t r, const ui
   if (map.part + map.lane == 0) {
     if (a.mean != nullptr) a.mean[r] = mean;
     if (a.rstd != nullptr) a.rstd[r] = rstd;
-  }
-}
-
-template <typename T, int BYTES, int UNITS, int WIDTH>
-__device__ __forceinline__ void load_norm_params(const NormArgs& a, const UnitMap<UNITS, WIDTH>& map,
-                                                 float (&w)[UNITS][Unit<T, BYTES>::kElems],
-                                                 float (&b)[UNITS][Unit<T, BYTES>::kElems]) {
-  const uint32_t dim = uint32_t(a.dim);
-#pragma unroll
-  for (int c = 0; c < UNITS; ++c) {
-    const uint32_t column = (map.part + map(c)) * Unit<T, BYTES>::kElems;
-    load_params<T>(a.weight, a.params_f32, a.params_vec, column, dim, 1.f, w[c]);
-    load_params<T>(a.bias, a.params_f32, a.params_vec, column, dim, 0.f, b[c]);
   }
 }
 
@@ -95,7 +85,7 @@ __global__ void __launch_bounds__(1024)
   const UnitMap<UNITS, WIDTH> map(group, uint32_t(a.dim) / U::kElems);
   const uint8_t* row = nullptr;
   if (r < a.n) {
-    row = a.row_ptrs != nullptr ? row_address(a, r) : in.first + r * in.stride;
+    row = a.row_ptrs != nullptr ? valid_row(a, a.row_ptrs[r]) : in.first + r * in.stride;
   }
   typename U::Raw raw[UNITS];
 #pragma unroll
@@ -105,8 +95,8 @@ __global__ void __launch_bounds__(1024)
       raw[c] = __ldg(reinterpret_cast<const typename U::Raw*>(row) + map.part + map(c));
     }
   }
-  float x[UNITS][U::kElems], w[UNITS][U::kElems], b[UNITS][U::kElems], sum = 0.f;
-  load_norm_params<T, BYTES, UNITS, WIDTH>(a, map, w, b);
+  float x[UNITS][U::kElems], params[2][UNITS][U::kElems], sum = 0.f;
+  load_params<T, BYTES>({a.weight, a.bias}, a.params_f32, a.params_vec, map, uint32_t(a.dim), {1.f, 0.f}, params);
 #pragma unroll
   for (int c = 0; c < UNITS; ++c) {
     U::unpack(raw[c], x[c]);
@@ -114,7 +104,7 @@ __global__ void __launch_bounds__(1024)
     for (int e = 0; e < U::kElems; ++e) sum += x[c][e];
   }
   GroupSum<1, WIDTH> group_sum(group, scratch);
-  norm_row<T, BYTES, UNITS, WIDTH>(a, r, row, sum, map, group_sum, x, w, b);
+  norm_row<T, BYTES, UNITS, WIDTH>(a, r, row, sum, map, group_sum, x, params[0], params[1]);
 }
 
 // Many rows: the blocks stay on the device, their threads keep the weights of
@@ -132,15 +122,17 @@ __global__ void __launch_bounds__(kPipeBlock, (kResident<T, BYTES, UNITS>))
   const RowDeal deal(group);
   const uint32_t n = uint32_t(a.n), row_bytes = uint32_t(a.dim * sizeof(T));
   const RowQueue<T, BYTES, UNITS, WIDTH> queue(slots, 0, 1, map, row_bytes);
-  float w[UNITS][U::kElems], b[UNITS][U::kElems];
-  load_norm_params<T, BYTES, UNITS, WIDTH>(a, map, w, b);
+  float params[2][UNITS][U::kElems];
+  load_params<T, BYTES>({a.weight, a.bias}, a.params_f32, a.params_vec, map, uint32_t(a.dim), {1.f, 0.f}, params);
   uint32_t r = deal.row;
   auto address = [&](uint32_t row) -> const uint8_t* {
     if (row >= n) return nullptr;
-    return a.row_ptrs != nullptr ? row_address(a, row) : in.first + row * in.stride;
+    return a.row_ptrs != nullptr ? static_cast<const uint8_t*>(a.row_ptrs[row]) : in.first + row * in.stride;
   };
-  auto fill = [&](uint32_t stage, const uint8_t* row) {
+  // row: in, as it was read; out, null where no row can start
+  auto fill = [&](uint32_t stage, const uint8_t*& row) {
     const bool by_address = a.row_ptrs != nullptr;
+    if (by_address) row = valid_row(a, row);
     queue.fill(stage, row, map, by_address ? row : in.first, by_address ? row + row_bytes : in.last);
     copies_commit();
   };
@@ -160,17 +152,18 @@ __global__ void __launch_bounds__(kPipeBlock, (kResident<T, BYTES, UNITS>))
     rows[kStages] = address(r + kStages * deal.step);
     copies_wait<kStages - 1>();
     queue.arrive();
-    float x[UNITS][U::kElems], sum = 0.f;
+    float x[UNITS][U::kElems];
+    Partial sum;
     if (rows[0] != nullptr) {
       const uint32_t from = queue.place(stage, rows[0], map);
       map.template each<kRun<BYTES, UNITS>>([&](int c, bool mine) {
         queue.take(from, c, mine, map, x[c]);
 #pragma unroll
-        for (int e = 0; e < U::kElems; ++e) sum += x[c][e];
+        for (int e = 0; e < U::kElems; ++e) sum.part[(c * U::kElems + e) % 4] += x[c][e];
       });
     }
     queue.arrive();
-    norm_row<T, BYTES, UNITS, WIDTH>(a, r, rows[0], sum, map, group_sum, x, w, b);
+    norm_row<T, BYTES, UNITS, WIDTH>(a, r, rows[0], sum.sum(), map, group_sum, x, params[0], params[1]);
     stage = stage + 1 == kStages ? 0 : stage + 1;
   }
   copies_wait<0>();
@@ -182,11 +175,11 @@ template <typename T>
 __global__ void __launch_bounds__(1024)
     norm_long_kernel(const NormArgs a) {
   __shared__ float scratch[32][2][1];
-  GroupSum<1, 32> group_sum(blockDim.x, scratch);
+  GroupSum<1, kWarps> group_sum(blockDim.x, scratch);
   const uint32_t dim = uint32_t(a.dim);
   for (uint64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
     const T* row = reinterpret_cast<const T*>(
-        a.row_ptrs != nullptr ? row_address(a, r) : static_cast<const uint8_t*>(a.x) + r * a.x_stride);
+        a.row_ptrs != nullptr ? valid_row(a, a.row_ptrs[r]) : static_cast<const uint8_t*>(a.x) + r * a.x_stride);
     if (row == nullptr) continue;
     float sum[1] = {0.f};
     for (uint32_t i = threadIdx.x; i < dim; i += blockDim.x) sum[0] += to_float(row[i]);
@@ -201,10 +194,9 @@ __global__ void __launch_bounds__(1024)
     const float rstd = rsqrtf(fmaf(sq[0], a.inv_dim, a.eps));
     T* out = reinterpret_cast<T*>(static_cast<uint8_t*>(a.y) + r * a.y_stride);
     for (uint32_t i = threadIdx.x; i < dim; i += blockDim.x) {
-      float w[1], b[1];
-      load_params<T>(a.weight, a.params_f32, false, i, dim, 1.f, w);
-      load_params<T>(a.bias, a.params_f32, false, i, dim, 0.f, b);
-      out[i] = from_float<T>(fmaf((to_float(row[i]) - mean) * rstd, w[0], b[0]));
+      const float w = load_param<T>(a.weight, a.params_f32, i, 1.f);
+      const float b = load_param<T>(a.bias, a.params_f32, i, 0.f);
+      out[i] = from_float<T>(fmaf((to_float(row[i]) - mean) * rstd, w, b));
     }
     if (threadIdx.x == 0) {
       if (a.mean != nullptr) a.mean[r] = mean;
@@ -233,7 +225,8 @@ int launch_norm_width(const NormArgs& a, uint32_t group, const RowsIn& in, cudaS
 }
 template <typename T, int BYTES, int UNITS>
 int launch_norm_pipe(const NormArgs& a, uint32_t group, const RowsIn& in, cudaStream_t stream) {
-  if (group >= 32) return launch_norm_width<T, BYTES, UNITS, 32>(a, group, in, stream);
+  if (group > 32) return launch_norm_width<T, BYTES, UNITS, kWarps>(a, group, in, stream);
+  if (group == 32) return launch_norm_width<T, BYTES, UNITS, 32>(a, group, in, stream);
   if constexpr (BYTES == 16) return launch_norm_width<T, BYTES, UNITS, 0>(a, group, in, stream);
   else if (group == 16) return launch_norm_width<T, BYTES, UNITS, 16>(a, group, in, stream);
   else return launch_norm_width<T, BYTES, UNITS, 8>(a, group, in, stream);
@@ -267,8 +260,8 @@ int launch_norm_type(const NormArgs& a, cudaStream_t stream) {
         return HKV_OK;
       }
     }
-    if (units <= 1024) launch_norm_few<T, BYTES, 1, 32>(a, uint32_t((units + 31) / 32 * 32), in, stream);
-    else if (units <= 2048) launch_norm_few<T, BYTES, 2, 32>(a, group_for(units, 2, BYTES), in, stream);
+    if (units <= 1024) launch_norm_few<T, BYTES, 1, kWarps>(a, uint32_t((units + 31) / 32 * 32), in, stream);
+    else if (units <= 2048) launch_norm_few<T, BYTES, 2, kWarps>(a, group_for(units, 2, BYTES), in, stream);
     if (units <= 2048) return HKV_OK;
   }
 #define HKV_CALL(N) return launch_norm_pipe<T, BYTES, N>(a, group, in, stream)

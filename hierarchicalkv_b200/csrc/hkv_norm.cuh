@@ -11,13 +11,23 @@ constexpr uint32_t kFull = 0xFFFFFFFFu;
 constexpr int kPipeBlock = 512;   // threads of the kernels that stay on the device
 constexpr int kStages = 3;        // rows of a warp's queue: one in use, two on their way
 
-// Sum over the `group` threads of a row: WIDTH of them where that is below 32 (0:
-// a power of two known at run time), else whole warps; every thread gets it.  scratch: two floats of each
-// value per warp, used in turn, so that one barrier of the group's own (named
-// 1 + its number in the block) is enough.
+// WIDTH, of a kernel: how many lanes have a row.  8, 16 or 32; 0: a power of two
+// below 32 known at run time; kWarps: several whole warps.
+constexpr int kWarps = 64;
+
+// A thread's sum in four parts: one would be a chain of additions that wait for
+// one another.
+struct Partial {
+  float part[4] = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ float sum() const { return (part[0] + part[1]) + (part[2] + part[3]); }
+};
+
+// Sum over the `group` threads of a row; every thread gets it.  scratch: two floats
+// of each value per warp, used in turn, so that one barrier of the group's own
+// (named 1 + its number in the block) is enough.
 template <int N, int WIDTH>
 struct GroupSum {
-  static constexpr bool WIDE = WIDTH == 32;
+  static constexpr bool WIDE = WIDTH == kWarps;
   uint32_t group, warps, span, from, barrier;   // warps: of the group; span: the next power of two
   float (*scratch)[2][N];                       // [warps of the block]
   uint32_t turn = 0;
@@ -37,7 +47,7 @@ struct GroupSum {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(kFull, v[i], d);
       }
-      if (warps == 1) return;
+      if (warps == 1) return;   // few rows, on one warp each
       if ((threadIdx.x & 31u) == 0) {
 #pragma unroll
         for (int i = 0; i < N; ++i) scratch[threadIdx.x >> 5][turn][i] = v[i];
@@ -61,34 +71,59 @@ struct GroupSum {
   }
 };
 
+// Keeps an address as it is: the compiler would work it out again, from the thread's
+// number on, for every unit (831 instructions per row of 1001 bf16, 679 with it kept).
+template <typename P>
+__device__ __forceinline__ P* keep(P* p) {   // of global memory
+  asm volatile("" : "+l"(p));
+  __builtin_assume(__isGlobal(p));
+  return p;
+}
+__device__ __forceinline__ uint32_t keep(uint32_t shared) {
+  asm volatile("" : "+r"(shared));
+  return shared;
+}
+
 // Where a thread's units lie in its row: unit c of the thread is first + c * width
 // of the row.  A warp of a group of several owns a part of consecutive units, which
 // begins at unit `part` and has `count`; the lanes of a group below a warp own all.
 template <int UNITS, int WIDTH>
 struct UnitMap {
+  static constexpr uint32_t kWidth = WIDTH == kWarps ? 32 : WIDTH;
   uint32_t part, count, lane, width;   // lane: within the width
 
   __device__ __forceinline__ UnitMap(uint32_t group, uint32_t units) {
-    width = WIDTH ? uint32_t(WIDTH) : group;
+    width = WIDTH == 0 ? group : kWidth;
     lane = threadIdx.x & (width - 1u);
-    part = WIDTH == 32 ? (threadIdx.x % group >> 5) * 32u * UNITS : 0u;
+    part = WIDTH == kWarps ? (threadIdx.x % group >> 5) * 32u * UNITS : 0u;
     count = units > part ? min(units - part, width * UNITS) : 0u;
   }
   // The unit's number within the part.
   __device__ __forceinline__ uint32_t operator()(int c) const {
-    return lane + uint32_t(c) * (WIDTH ? uint32_t(WIDTH) : width);
+    return lane + uint32_t(c) * (WIDTH == 0 ? width : kWidth);
   }
   // f(c, mine) for the thread's units c, in runs of RUN: `mine` is a constant where
-  // all lanes have the whole run, and runs that none has are left out.
+  // all lanes have the whole run, and runs that none has are left out.  One test
+  // serves rows that reach into the last run (65536 x 1001 bf16: 56 us, with a test
+  // per run 64).  A single run is not tested, only its units, on a row of one warp or
+  // less (65536 x 1024 bf16: 45 us, with a test 49); on several warps, whose
+  // last may have none, it is (16384 x 8192 bf16: 102 us, without 113).
   template <int RUN, typename F>
   __device__ __forceinline__ void each(F&& f) const {
     static_assert(UNITS % RUN == 0, "whole runs");
+    if ((WIDTH != kWarps || RUN < UNITS) && (UNITS - RUN) * (WIDTH == 0 ? width : kWidth) <= count) {
+#pragma unroll
+      for (int c = 0; c < UNITS - RUN; ++c) f(c, true);
+#pragma unroll
+      for (int c = UNITS - RUN; c < UNITS; ++c) f(c, (*this)(c) < count);
+      return;
+    }
 #pragma unroll
     for (int b = 0; b < UNITS; b += RUN) {
-      if ((b + RUN) * width <= count) {
+      if ((b + RUN) * (WIDTH == 0 ? width : kWidth) <= count) {
 #pragma unroll
         for (int i = 0; i < RUN; ++i) f(b + i, true);
-      } else if (b * width < count) {
+      } else if (b * (WIDTH == 0 ? width : kWidth) < count) {
 #pragma unroll
         for (int i = 0; i < RUN; ++i) f(b + i, (*this)(b + i) < count);
       }
@@ -106,7 +141,7 @@ constexpr int kRun = BYTES == 16 || UNITS % 4 != 0 ? UNITS : 4;
 // the aligned 16 bytes around it together and take their units at any alignment.
 template <typename T, int BYTES, int UNITS, int WIDTH>
 struct RowQueue {
-  static constexpr bool WIDE = WIDTH == 32;
+  static constexpr bool WIDE = WIDTH >= 32;
   using Map = UnitMap<UNITS, WIDTH>;
   using Raw = typename Unit<T, BYTES>::Raw;
   uint32_t mine;         // shared address of this lane's slot 0 (16-byte units) or of its row's first
@@ -190,49 +225,118 @@ struct RowQueue {
 
   // Where the lane's first unit of the row in a stage is.
   __device__ __forceinline__ uint32_t place(uint32_t stage, const uint8_t* row, const Map& map) const {
-    return mine + stage * stage_bytes + (BYTES == 16 ? 0u : shift(row, map) + map.lane * BYTES);
+    return keep(mine + stage * stage_bytes + (BYTES == 16 ? 0u : shift(row, map) + map.lane * BYTES));
   }
   // Unit c of the lane, `from` place(), as floats; zeros where it has none.
   static __device__ __forceinline__ void take(uint32_t from, int c, bool mine, const Map& map,
                                               float (&f)[Unit<T, BYTES>::kElems]) {
     // inside the queue's slots even where the lane has no such unit
-    const Raw v = load_shared<BYTES>(from + (BYTES == 16 ? c * 512u : (map(c) - map.lane) * BYTES));
+    const auto v = load_shared<BYTES>(from + (BYTES == 16 ? c * 512u : (map(c) - map.lane) * BYTES));
     Unit<T, BYTES>::unpack(v, f);
 #pragma unroll
     for (int e = 0; e < Unit<T, BYTES>::kElems; ++e) f[e] = mine ? f[e] : 0.f;
   }
 };
 
-// Weights or biases of the N columns from `column` on; `none` where there is no
-// pointer or no such column.  vec: the address is a multiple of 16.
-template <typename T, int N>
-__device__ __forceinline__ void load_params(const void* p, bool f32, bool vec, uint32_t column,
-                                            uint32_t dim, float none, float (&out)[N]) {
+// One weight or bias; `none` where there are none.
+template <typename T>
+__device__ __forceinline__ float load_param(const void* p, bool f32, uint32_t column, float none) {
+  if (p == nullptr) return none;
+  return f32 ? __ldg(static_cast<const float*>(p) + column) : to_float(static_cast<const T*>(p)[column]);
+}
+
+// A thread's weights, or weights and biases (the P vectors p): those of the columns of
+// its units, none[i] where p[i] is null.  The choice between the types is made once
+// for all of them and no load is behind a condition, so that all are in flight
+// together: columns past the row's end read its last unit again.  (With the
+// choice made unit by unit each load waited for the one before: 65536 x 1001 bf16
+// took 86 us instead of 64.)  vec: the addresses are multiples of 16.
+template <typename T, int BYTES, int UNITS, int WIDTH, int P>
+__device__ __forceinline__ void load_params(const void* const (&p)[P], bool f32, bool vec,
+                                            const UnitMap<UNITS, WIDTH>& map, uint32_t dim,
+                                            const float (&none)[P],
+                                            float (&out)[P][UNITS][Unit<T, BYTES>::kElems]) {
+  constexpr int N = Unit<T, BYTES>::kElems;
+  const void* any = p[0] != nullptr ? p[0] : p[P - 1];
+  if (any == nullptr) {
 #pragma unroll
-  for (int e = 0; e < N; ++e) out[e] = none;
-  if (p == nullptr || column >= dim) return;   // units are whole: one column in, all in
-  if constexpr (N * sizeof(T) == 16) {
-    if (vec) {
-      if (f32) {
-        const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + column);
+    for (int i = 0; i < P; ++i) {
 #pragma unroll
-        for (int e = 0; e < N; e += 4) {
-          const float4 v = __ldg(s + e / 4);
-          out[e] = v.x;
-          out[e + 1] = v.y;
-          out[e + 2] = v.z;
-          out[e + 3] = v.w;
-        }
-      } else {
-        Unit<T, 16>::unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p) + column)), out);
+      for (int c = 0; c < UNITS; ++c) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) out[i][c][e] = none[i];
       }
-      return;
+    }
+    return;
+  }
+  auto column = [&](int c) { return min((map.part + map(c)) * N, dim - N); };   // rows are whole units
+  auto from = [&](int i, auto* type) {
+    return static_cast<decltype(type)>(p[i] != nullptr ? p[i] : any);
+  };
+  if (f32) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const float* at = from(i, static_cast<const float*>(nullptr));
+#pragma unroll
+      for (int c = 0; c < UNITS; ++c) {
+        if (N % 4 == 0 && vec) {
+#pragma unroll
+          for (int e = 0; e + 3 < N; e += 4) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(at + column(c) + e));
+            out[i][c][e] = v.x;
+            out[i][c][e + 1] = v.y;
+            out[i][c][e + 2] = v.z;
+            out[i][c][e + 3] = v.w;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) out[i][c][e] = __ldg(at + column(c) + e);
+        }
+      }
+    }
+  } else if (BYTES == 16 && vec) {
+    typename Unit<T, BYTES>::Raw raw[P][UNITS];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const T* at = from(i, static_cast<const T*>(nullptr));
+#pragma unroll
+      for (int c = 0; c < UNITS; ++c) {
+        raw[i][c] = __ldg(reinterpret_cast<const typename Unit<T, BYTES>::Raw*>(at + column(c)));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+#pragma unroll
+      for (int c = 0; c < UNITS; ++c) Unit<T, BYTES>::unpack(raw[i][c], out[i][c]);
+    }
+  } else {
+    T raw[P][UNITS][N];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const T* at = from(i, static_cast<const T*>(nullptr));
+#pragma unroll
+      for (int c = 0; c < UNITS; ++c) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) raw[i][c][e] = at[column(c) + e];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+#pragma unroll
+      for (int c = 0; c < UNITS; ++c) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) out[i][c][e] = to_float(raw[i][c][e]);
+      }
     }
   }
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    out[e] = f32 ? static_cast<const float*>(p)[column + e]
-                 : to_float(static_cast<const T*>(p)[column + e]);
+  for (int i = 0; i < P; ++i) {
+    if (p[i] != nullptr) continue;
+#pragma unroll
+    for (int c = 0; c < UNITS; ++c) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) out[i][c][e] = none[i];
+    }
   }
 }
 

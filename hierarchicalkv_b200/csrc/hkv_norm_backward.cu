@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(kPipeBlock, 1)
                          const RowsIn dy_in, float* __restrict__ sums) {
   using U = Unit<T, BYTES>;
   constexpr int kElems = U::kElems;
-  constexpr bool WIDE = WIDTH == 32;
+  constexpr bool WIDE = WIDTH >= 32;
   extern __shared__ uint4 slots[];
   float* columns = reinterpret_cast<float*>(slots);   // [copies][dim], after the last row
   __shared__ float scratch[kPipeBlock / 32][2][2];
@@ -45,12 +45,12 @@ __global__ void __launch_bounds__(kPipeBlock, 1)
   const uint32_t row_bytes = dim * uint32_t(sizeof(T));
   const RowQueue<T, BYTES, UNITS, WIDTH> x_queue(slots, 0, 2, map, row_bytes);
   const RowQueue<T, BYTES, UNITS, WIDTH> dy_queue(slots, 1, 2, map, row_bytes);
-  float w[UNITS][kElems], dw[UNITS][kElems], db[UNITS][kElems];
+  float w[1][UNITS][kElems], dw[UNITS][kElems], db[UNITS][kElems];
+  load_params<T, BYTES>({a.weight}, a.params_f32, a.params_vec, map, dim, {1.f}, w);
 #pragma unroll
   for (int c = 0; c < UNITS; ++c) {
 #pragma unroll
     for (int e = 0; e < kElems; ++e) dw[c][e] = db[c][e] = 0.f;
-    load_params<T>(a.weight, a.params_f32, a.params_vec, (map.part + map(c)) * kElems, dim, 1.f, w[c]);
   }
   const uint32_t step = deal.step;
   uint32_t r = deal.row;
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kPipeBlock, 1)
     copies_wait<kStages - 1>();
     x_queue.arrive();
     float xhat[UNITS][kElems], g[UNITS][kElems];
-    float sum[2] = {0.f, 0.f};
+    Partial gs, products;
     if (r < n) {
       const uint32_t x_from = x_queue.place(stage, x_row(r), map);
       const uint32_t dy_from = dy_queue.place(stage, dy_row(r), map);
@@ -97,21 +97,23 @@ __global__ void __launch_bounds__(kPipeBlock, 1)
 #pragma unroll
         for (int e = 0; e < kElems; ++e) {
           xhat[c][e] = (x[e] - mean) * rstd;
-          g[c][e] = dy[e] * w[c][e];
-          sum[0] += g[c][e];
-          sum[1] = fmaf(g[c][e], xhat[c][e], sum[1]);
+          g[c][e] = dy[e] * w[0][c][e];
+          gs.part[(c * kElems + e) % 4] += g[c][e];
+          float& product = products.part[(c * kElems + e) % 4];
+          product = fmaf(g[c][e], xhat[c][e], product);
           dw[c][e] = fmaf(dy[e], xhat[c][e], dw[c][e]);
           db[c][e] += dy[e];
         }
       });
     }
     x_queue.arrive();
+    float sum[2] = {gs.sum(), products.sum()};
     group_sum(sum);
     // dx = rstd * (g - m0 - xhat * m1)
     const float r0 = rstd * (sum[0] * a.inv_dim), m1 = sum[1] * a.inv_dim;
     if (r < n) {
-      auto* to = reinterpret_cast<typename U::Raw*>(static_cast<uint8_t*>(a.dx) + r * a.dx_stride) +
-                 (map.part + map.lane);
+      auto* to = keep(reinterpret_cast<typename U::Raw*>(static_cast<uint8_t*>(a.dx) + r * a.dx_stride) +
+                      (map.part + map.lane));
       map.template each<kRun<BYTES, UNITS>>([&](int c, bool mine) {
         float f[kElems];
 #pragma unroll
@@ -167,7 +169,7 @@ template <typename T>
 __global__ void __launch_bounds__(512)
     norm_backward_long_kernel(const NormBackwardArgs a) {
   __shared__ float scratch[16][2][2];
-  GroupSum<2, 32> group_sum(blockDim.x, scratch);
+  GroupSum<2, kWarps> group_sum(blockDim.x, scratch);
   const uint32_t dim = uint32_t(a.dim);
   for (uint64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
     const T* x = reinterpret_cast<const T*>(static_cast<const uint8_t*>(a.x) + r * a.x_stride);
@@ -176,19 +178,17 @@ __global__ void __launch_bounds__(512)
     const float mean = a.mean[r], rstd = a.rstd[r];
     float sum[2] = {0.f, 0.f};
     for (uint32_t i = threadIdx.x; i < dim; i += blockDim.x) {
-      float w[1];
-      load_params<T>(a.weight, a.params_f32, false, i, dim, 1.f, w);
-      const float g = to_float(dy[i]) * w[0];
+      const float w = load_param<T>(a.weight, a.params_f32, i, 1.f);
+      const float g = to_float(dy[i]) * w;
       sum[0] += g;
       sum[1] = fmaf(g, (to_float(x[i]) - mean) * rstd, sum[1]);
     }
     group_sum(sum);
     const float m0 = sum[0] * a.inv_dim, m1 = sum[1] * a.inv_dim;
     for (uint32_t i = threadIdx.x; i < dim; i += blockDim.x) {
-      float w[1];
-      load_params<T>(a.weight, a.params_f32, false, i, dim, 1.f, w);
+      const float w = load_param<T>(a.weight, a.params_f32, i, 1.f);
       const float xhat = (to_float(x[i]) - mean) * rstd;
-      dx[i] = from_float<T>(rstd * (fmaf(-m1, xhat, to_float(dy[i]) * w[0]) - m0));
+      dx[i] = from_float<T>(rstd * (fmaf(-m1, xhat, to_float(dy[i]) * w) - m0));
     }
   }
 }
@@ -269,7 +269,7 @@ template <typename T, int BYTES, int UNITS, int WIDTH>
 int launch_backward_pipe(const NormBackwardArgs& a, const NormBackwardPlan& p, float* sums,
                          cudaStream_t stream) {
   const uint64_t row_bytes = a.dim * sizeof(T);
-  const size_t copies = WIDTH == 32 ? kPipeBlock / p.group : kPipeBlock / 32;   // of the column sums
+  const size_t copies = WIDTH >= 32 ? kPipeBlock / p.group : kPipeBlock / 32;   // of the column sums
   const size_t queue = RowQueue<T, BYTES, UNITS, WIDTH>::bytes(p.group, 2);
   const size_t columns = copies * a.dim * sizeof(float);
   const size_t shared = queue > columns ? queue : columns;
@@ -285,7 +285,8 @@ int launch_backward_pipe(const NormBackwardArgs& a, const NormBackwardPlan& p, f
 template <typename T, int BYTES, int UNITS>
 int launch_backward_units(const NormBackwardArgs& a, const NormBackwardPlan& p, float* sums,
                           cudaStream_t stream) {
-  if (p.group >= 32) return launch_backward_pipe<T, BYTES, UNITS, 32>(a, p, sums, stream);
+  if (p.group > 32) return launch_backward_pipe<T, BYTES, UNITS, kWarps>(a, p, sums, stream);
+  if (p.group == 32) return launch_backward_pipe<T, BYTES, UNITS, 32>(a, p, sums, stream);
   if constexpr (BYTES == 16) return launch_backward_pipe<T, BYTES, UNITS, 0>(a, p, sums, stream);
   else if (p.group == 16) return launch_backward_pipe<T, BYTES, UNITS, 16>(a, p, sums, stream);
   else return launch_backward_pipe<T, BYTES, UNITS, 8>(a, p, sums, stream);

@@ -10,6 +10,7 @@
 
 #include <atomic>
 #include <string>
+#include <type_traits>
 
 #include "../../include/hkv_b200.h"
 #include "hkv_device.cuh"
@@ -25,6 +26,12 @@ inline uint32_t row_kind_size(uint32_t kind) { return kind == kValueF32 ? 4u : 2
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float low_to_float(uint32_t v, const __half*) {
+  return __half2float(__ushort_as_half(static_cast<uint16_t>(v)));
+}
+__device__ __forceinline__ float low_to_float(uint32_t v, const __nv_bfloat16*) {
+  return __uint_as_float(v << 16);   // a bfloat16 is the upper half of its float
+}
 
 // The one rounding of a result, to nearest even.
 template <typename T>
@@ -46,7 +53,7 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
 // as a thread's work per unit is the load, the arithmetic and the store and
 // nothing else.  (Cutting 16-byte chunks out of the aligned ones around them
 // instead, with their masks and shifts, took 1043 instructions per row of 1001
-// bfloat16 in layer norm, where the units take half of that.)
+// bfloat16 in layer norm, where the units take 617.)
 
 // A 32-bit word's elements as floats, and back.
 __device__ __forceinline__ void unpack_word(uint32_t w, float* f, const float*) {
@@ -58,7 +65,7 @@ __device__ __forceinline__ void unpack_word(uint32_t w, float* f, const __half*)
   f[1] = two.y;
 }
 __device__ __forceinline__ void unpack_word(uint32_t w, float* f, const __nv_bfloat16*) {
-  f[0] = __uint_as_float(w << 16);   // a bfloat16 is the upper half of its float
+  f[0] = __uint_as_float(w << 16);
   f[1] = __uint_as_float(w & 0xFFFF0000u);
 }
 __device__ __forceinline__ uint32_t pack_word(const float* f, const float*) {
@@ -77,8 +84,9 @@ template <typename T, int BYTES>
 struct Unit {
   static constexpr int kElems = BYTES / int(sizeof(T));
   using Raw = typename VecType<BYTES>::type;
+  using Loaded = std::conditional_t<BYTES == 2, uint32_t, Raw>;   // 16 bits, in a register's lower half
 
-  static __device__ __forceinline__ void unpack(const Raw& v, float (&f)[kElems]) {
+  static __device__ __forceinline__ void unpack(const Loaded& v, float (&f)[kElems]) {
     if constexpr (BYTES == 16) {
       constexpr int kPer = 4 / int(sizeof(T));
       unpack_word(v.x, f, static_cast<const T*>(nullptr));
@@ -88,9 +96,7 @@ struct Unit {
     } else if constexpr (BYTES == 4) {
       unpack_word(v, f, static_cast<const T*>(nullptr));
     } else {
-      T one;
-      *reinterpret_cast<Raw*>(&one) = v;
-      f[0] = to_float(one);
+      f[0] = low_to_float(v, static_cast<const T*>(nullptr));
     }
   }
   static __device__ __forceinline__ Raw pack(const float (&f)[kElems]) {
@@ -165,22 +171,26 @@ __device__ __forceinline__ void copies_wait() {
 template <int ELEMENT>
 __device__ __forceinline__ void copy_elements(uint32_t shared, const uint8_t* at, const uint8_t* from,
                                               const uint8_t* to) {
-#pragma unroll 1
-  for (uint32_t b = 0; b < 16u; b += ELEMENT) {
+  using Raw = typename VecType<ELEMENT>::type;
+  Raw v[16 / ELEMENT];   // all on their way before the first is stored
+#pragma unroll
+  for (int b = 0; b < 16; b += ELEMENT) {
+    if (at + b >= from && at + b < to) v[b / ELEMENT] = __ldg(reinterpret_cast<const Raw*>(at + b));
+  }
+#pragma unroll
+  for (int b = 0; b < 16; b += ELEMENT) {
     if (at + b < from || at + b >= to) continue;
     if constexpr (ELEMENT == 4) {
-      const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(at + b));
-      asm volatile("st.shared.u32 [%0], %1;" ::"r"(shared + b), "r"(v) : "memory");
+      asm volatile("st.shared.u32 [%0], %1;" ::"r"(shared + b), "r"(v[b / ELEMENT]) : "memory");
     } else {
-      const uint16_t v = __ldg(reinterpret_cast<const uint16_t*>(at + b));
-      asm volatile("st.shared.u16 [%0], %1;" ::"r"(shared + b), "h"(v) : "memory");
+      asm volatile("st.shared.u16 [%0], %1;" ::"r"(shared + b), "h"(v[b / ELEMENT]) : "memory");
     }
   }
 }
 
 template <int BYTES>
-__device__ __forceinline__ typename VecType<BYTES>::type load_shared(uint32_t at) {
-  typename VecType<BYTES>::type v;
+__device__ __forceinline__ auto load_shared(uint32_t at) {
+  std::conditional_t<BYTES == 16, uint4, uint32_t> v;
   if constexpr (BYTES == 16) {
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
@@ -189,7 +199,7 @@ __device__ __forceinline__ typename VecType<BYTES>::type load_shared(uint32_t at
   } else if constexpr (BYTES == 4) {
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
   } else {
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared.u16 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
   }
   return v;
 }
