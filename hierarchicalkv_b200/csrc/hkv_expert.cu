@@ -895,7 +895,7 @@ int hkv_expert_dispatch(uint64_t tokens, uint32_t top_k, uint64_t row_bytes, con
   unsigned grid = 0;
   rc = grid_of(tokens * parts.parts * lanes, kMoveBlock, &grid);
   if (rc != HKV_OK) return rc;
-  const RowsIn in = rows_in(x, tokens, x_stride, row_bytes);
+  const RowsIn in = rows_in(x, x_stride);
   const int32_t* kept = zero_rows_behind ? offsets + experts : nullptr;
 #define HKV_RUN(BYTES, LANES)                                                            \
   dispatch_kernel<BYTES, LANES, dispatch_shape(BYTES).units>                             \
@@ -941,7 +941,7 @@ int hkv_expert_combine(uint64_t tokens, uint32_t top_k, uint64_t dim, uint32_t v
   rc = grid_of(tokens * parts.parts * lanes, kMoveBlock, &grid);
   if (rc != HKV_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const RowsIn in = rows_in(rows, tokens * top_k, rows_stride, row_bytes);
+  const RowsIn in = rows_in(rows, rows_stride);
 #define HKV_LANES(LANES)                                                                  \
   combine_kernel<RowT, kUnit, LANES, combine_shape(kUnit).units,                          \
                  combine_shape(kUnit).assigned><<<grid, kMoveBlock, 0, s>>>(              \
@@ -996,8 +996,8 @@ int hkv_expert_combine_backward(uint64_t tokens, uint32_t top_k, uint64_t dim, u
   rc = grid_of(tokens * (lanes == 32 ? warps * 32 : lanes), 256, &grid);
   if (rc != HKV_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const RowsIn d_in = rows_in(d_out, tokens, d_out_stride, row_bytes);
-  const RowsIn in = rows_in(rows, tokens * top_k, rows_stride, row_bytes);
+  const RowsIn d_in = rows_in(d_out, d_out_stride);
+  const RowsIn in = rows_in(rows, rows_stride);
   const int32_t* kept = zero_rows_behind ? offsets + experts : nullptr;
 #define HKV_RUN(T, BYTES, LANES, FEW)                                                               \
   combine_backward_kernel<T, BYTES, LANES, backward_shape(BYTES, FEW).units,                        \

@@ -71,14 +71,7 @@ struct GroupSum {
   }
 };
 
-// Keeps an address as it is: the compiler would work it out again, from the thread's
-// number on, for every unit (831 instructions per row of 1001 bf16, 679 with it kept).
-template <typename P>
-__device__ __forceinline__ P* keep(P* p) {   // of global memory
-  asm volatile("" : "+l"(p));
-  __builtin_assume(__isGlobal(p));
-  return p;
-}
+// Keeps an address as it is: the compiler would work it out again for every unit.
 __device__ __forceinline__ uint32_t keep(uint32_t shared) {
   asm volatile("" : "+r"(shared));
   return shared;
@@ -105,7 +98,7 @@ struct UnitMap {
   // f(c, mine) for the thread's units c, in runs of RUN: `mine` is a constant where
   // all lanes have the whole run, and runs that none has are left out.  One test
   // serves rows that reach into the last run (65536 x 1001 bf16: 56 us, with a test
-  // per run 64).  A single run is not tested, only its units, on a row of one warp or
+  // per run 64, before other steps).  A single run is not tested, only its units, on a row of one warp or
   // less (65536 x 1024 bf16: 45 us, with a test 49); on several warps, whose
   // last may have none, it is (16384 x 8192 bf16: 102 us, without 113).
   template <int RUN, typename F>
@@ -139,16 +132,16 @@ constexpr int kRun = BYTES == 16 || UNITS % 4 != 0 ? UNITS : 4;
 // to the warp alone, so no barrier of the block is needed.  Rows in 16-byte units:
 // a lane copies the units it will take.  Narrower units: the lanes of a row copy
 // the aligned 16 bytes around it together and take their units at any alignment.
+// Nothing behind a row's end is read; the up to 14 bytes before its first element
+// are, which lie in the row's allocation, since no allocation starts inside aligned
+// 16 bytes.
 template <typename T, int BYTES, int UNITS, int WIDTH>
 struct RowQueue {
-  static constexpr bool WIDE = WIDTH >= 32;
   using Map = UnitMap<UNITS, WIDTH>;
-  using Raw = typename Unit<T, BYTES>::Raw;
   uint32_t mine;         // shared address of this lane's slot 0 (16-byte units) or of its row's first
   uint32_t stage_bytes;  // distance of a warp's stages
-  uint32_t row_bytes;
 
-  static __host__ __device__ __forceinline__ uint32_t slots_per_row(uint32_t width) {
+  static constexpr __host__ __device__ __forceinline__ uint32_t slots_per_row(uint32_t width) {
     return BYTES == 16 ? width * UNITS : (width * UNITS * BYTES + 15u) / 16u + 1u;
   }
   static __host__ __device__ __forceinline__ uint32_t slots_per_warp(uint32_t width) {
@@ -161,8 +154,7 @@ struct RowQueue {
 
   // operand: which of the row's matrices this queue holds
   __device__ __forceinline__ RowQueue(const uint4* shared, uint32_t operand, uint32_t operands,
-                                      const Map& map, uint32_t row_bytes_)
-      : row_bytes(row_bytes_) {
+                                      const Map& map) {
     const uint32_t warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31u;
     const uint32_t slots = slots_per_warp(map.width);
     stage_bytes = operands * warps * slots * 16u;
@@ -171,10 +163,8 @@ struct RowQueue {
            (BYTES == 16 ? lane : lane / map.width * slots_per_row(map.width)) * 16u;
   }
 
-  // Puts a row of the matrix [first, last) into a stage (null: none).
-  __device__ __forceinline__ void fill(uint32_t stage, const uint8_t* row, const Map& map,
-                                       const uint8_t* first, const uint8_t* last) const {
-    if (row == nullptr) return;
+  // Puts a row into a stage.
+  __device__ __forceinline__ void fill(uint32_t stage, const uint8_t* row, const Map& map) const {
     const uint32_t to = mine + stage * stage_bytes;
     if constexpr (BYTES == 16) {
       const uint8_t* from = row + (map.part + map.lane) * 16u;
@@ -183,39 +173,22 @@ struct RowQueue {
         if (map(c) < map.count) copy_async(to + c * 512u, from + (map(c) - map.lane) * 16u);
       }
     } else {
-      const int begin = int(map.part * BYTES), length = int(map.count * BYTES);
-      if (length == 0) return;
-      const int ahead = int(shift(row, map));
-      const uint8_t* from = row + begin - ahead;   // aligned
-      const int slots = (ahead + length + 15) >> 4;
-      const bool inside = from >= first && from + slots * 16 <= last;
-      constexpr int kRounds = WIDE ? (32 * UNITS * BYTES / 16 + 1 + 31) / 32 : 1;
-      if (inside) {
-        if constexpr (WIDE) {
+      const uint32_t ahead = shift(uint32_t(reinterpret_cast<uintptr_t>(row)), map);
+      const uint8_t* from = row + map.part * BYTES - ahead;   // aligned
+      const int end = map.count != 0 ? int(ahead + map.count * BYTES) : 0;
+      constexpr int kSlots = int(slots_per_row(Map::kWidth));
 #pragma unroll
-          for (int i = 0; i < kRounds; ++i) {
-            const int slot = i * 32 + int(map.lane);
-            if (slot < slots) copy_async(to + slot * 16, from + slot * 16);
-          }
-        } else {
-          for (int slot = int(map.lane); slot < slots; slot += int(map.width)) {
-            copy_async(to + slot * 16, from + slot * 16);
-          }
-        }
-      } else {
-        // at an end of the matrix nothing outside the row's own bytes is read
-        for (int slot = int(map.lane); slot < slots; slot += int(map.width)) {
-          const uint8_t* at = from + slot * 16;
-          if (at >= row && at + 16 <= row + row_bytes) copy_async(to + slot * 16, at);
-          else copy_elements<sizeof(T)>(to + slot * 16, at, row, row + row_bytes);
-        }
+      for (int i = 0; i < kSlots; i += int(Map::kWidth)) {
+        const int at = (i + int(map.lane)) * 16;
+        if (at < end) copy_async(to + at, from + at, uint32_t(min(16, end - at)));
       }
     }
   }
 
-  // Where the warp's part of the row begins in its first slot.
-  __device__ __forceinline__ uint32_t shift(const uint8_t* row, const Map& map) const {
-    return BYTES == 16 ? 0u : (uint32_t(reinterpret_cast<uintptr_t>(row)) + map.part * BYTES) & 15u;
+  // Where the warp's part of a row begins in its first slot; `row`: the address's
+  // lower half.
+  __device__ __forceinline__ uint32_t shift(uint32_t row, const Map& map) const {
+    return BYTES == 16 ? 0u : (row + map.part * BYTES) & 15u;
   }
 
   // Before the first take() from a stage and after the last.
@@ -224,7 +197,7 @@ struct RowQueue {
   }
 
   // Where the lane's first unit of the row in a stage is.
-  __device__ __forceinline__ uint32_t place(uint32_t stage, const uint8_t* row, const Map& map) const {
+  __device__ __forceinline__ uint32_t place(uint32_t stage, uint32_t row, const Map& map) const {
     return keep(mine + stage * stage_bytes + (BYTES == 16 ? 0u : shift(row, map) + map.lane * BYTES));
   }
   // Unit c of the lane, `from` place(), as floats; zeros where it has none.

@@ -42,9 +42,8 @@ __global__ void __launch_bounds__(kPipeBlock, 1)
   const uint32_t n = uint32_t(a.n), dim = uint32_t(a.dim);
   const UnitMap<UNITS, WIDTH> map(group, dim / kElems);
   const RowDeal deal(group);
-  const uint32_t row_bytes = dim * uint32_t(sizeof(T));
-  const RowQueue<T, BYTES, UNITS, WIDTH> x_queue(slots, 0, 2, map, row_bytes);
-  const RowQueue<T, BYTES, UNITS, WIDTH> dy_queue(slots, 1, 2, map, row_bytes);
+  const RowQueue<T, BYTES, UNITS, WIDTH> x_queue(slots, 0, 2, map);
+  const RowQueue<T, BYTES, UNITS, WIDTH> dy_queue(slots, 1, 2, map);
   float w[1][UNITS][kElems], dw[UNITS][kElems], db[UNITS][kElems];
   load_params<T, BYTES>({a.weight}, a.params_f32, a.params_vec, map, dim, {1.f}, w);
 #pragma unroll
@@ -54,11 +53,20 @@ __global__ void __launch_bounds__(kPipeBlock, 1)
   }
   const uint32_t step = deal.step;
   uint32_t r = deal.row;
-  auto x_row = [&](uint32_t row) { return row < n ? x_in.first + row * x_in.stride : nullptr; };
-  auto dy_row = [&](uint32_t row) { return row < n ? dy_in.first + row * dy_in.stride : nullptr; };
+  // the rows that are fetched next, the lower halves of the current ones' addresses,
+  // and the thread's place in the row that is written, moved on from row to row
+  const uint8_t *x_next = x_in.first + r * x_in.stride, *dy_next = dy_in.first + r * dy_in.stride;
+  uint32_t x_current = uint32_t(reinterpret_cast<uintptr_t>(x_next));
+  uint32_t dy_current = uint32_t(reinterpret_cast<uintptr_t>(dy_next));
+  uint8_t* out = static_cast<uint8_t*>(a.dx) + r * a.dx_stride + (map.part + map.lane) * BYTES;
+  const uint64_t x_step = step * x_in.stride, dy_step = step * dy_in.stride, out_step = step * a.dx_stride;
   auto fill = [&](uint32_t stage, uint32_t row) {
-    x_queue.fill(stage, x_row(row), map, x_in.first, x_in.last);
-    dy_queue.fill(stage, dy_row(row), map, dy_in.first, dy_in.last);
+    if (row < n) {
+      x_queue.fill(stage, x_next, map);
+      dy_queue.fill(stage, dy_next, map);
+    }
+    x_next += x_step;
+    dy_next += dy_step;
     copies_commit();
   };
 #pragma unroll
@@ -72,7 +80,7 @@ __global__ void __launch_bounds__(kPipeBlock, 1)
   }
   uint32_t stage = 0;
   // the lanes of a warp leave together
-  for (uint32_t warp_row = deal.warp_row; warp_row < n; warp_row += step, r += step) {
+  for (uint32_t warp_row = deal.warp_row; warp_row < n; warp_row += step) {
     fill(stage == 0 ? kStages - 1 : stage - 1, r + (kStages - 1) * step);
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) {
@@ -88,8 +96,8 @@ __global__ void __launch_bounds__(kPipeBlock, 1)
     float xhat[UNITS][kElems], g[UNITS][kElems];
     Partial gs, products;
     if (r < n) {
-      const uint32_t x_from = x_queue.place(stage, x_row(r), map);
-      const uint32_t dy_from = dy_queue.place(stage, dy_row(r), map);
+      const uint32_t x_from = x_queue.place(stage, x_current, map);
+      const uint32_t dy_from = dy_queue.place(stage, dy_current, map);
       map.template each<kRun<BYTES, UNITS>>([&](int c, bool mine) {
         float x[kElems], dy[kElems];
         x_queue.take(x_from, c, mine, map, x);
@@ -112,8 +120,7 @@ __global__ void __launch_bounds__(kPipeBlock, 1)
     // dx = rstd * (g - m0 - xhat * m1)
     const float r0 = rstd * (sum[0] * a.inv_dim), m1 = sum[1] * a.inv_dim;
     if (r < n) {
-      auto* to = keep(reinterpret_cast<typename U::Raw*>(static_cast<uint8_t*>(a.dx) + r * a.dx_stride) +
-                      (map.part + map.lane));
+      auto* to = reinterpret_cast<typename U::Raw*>(out);
       map.template each<kRun<BYTES, UNITS>>([&](int c, bool mine) {
         float f[kElems];
 #pragma unroll
@@ -122,6 +129,10 @@ __global__ void __launch_bounds__(kPipeBlock, 1)
       });
     }
     stage = stage + 1 == kStages ? 0 : stage + 1;
+    r += step;
+    x_current += uint32_t(x_step);
+    dy_current += uint32_t(dy_step);
+    out += out_step;
   }
   copies_wait<0>();
   // the sums of the block's groups: those of one warp by exchange, the others
@@ -268,7 +279,6 @@ NormBackwardPlan plan_backward(uint64_t n, uint64_t dim, uint32_t size, uint32_t
 template <typename T, int BYTES, int UNITS, int WIDTH>
 int launch_backward_pipe(const NormBackwardArgs& a, const NormBackwardPlan& p, float* sums,
                          cudaStream_t stream) {
-  const uint64_t row_bytes = a.dim * sizeof(T);
   const size_t copies = WIDTH >= 32 ? kPipeBlock / p.group : kPipeBlock / 32;   // of the column sums
   const size_t queue = RowQueue<T, BYTES, UNITS, WIDTH>::bytes(p.group, 2);
   const size_t columns = copies * a.dim * sizeof(float);
@@ -277,8 +287,7 @@ int launch_backward_pipe(const NormBackwardArgs& a, const NormBackwardPlan& p, f
   const int rc = allow_shared<kKernel>();
   if (rc != HKV_OK) return rc;
   kKernel<<<p.blocks, pipe_threads(p.group), shared, stream>>>(
-      a, p.group, rows_in(a.x, a.n, a.x_stride, row_bytes), rows_in(a.dy, a.n, a.dy_stride, row_bytes),
-      sums);
+      a, p.group, rows_in(a.x, a.x_stride), rows_in(a.dy, a.dy_stride), sums);
   return HKV_OK;
 }
 

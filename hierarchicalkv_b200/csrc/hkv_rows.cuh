@@ -145,15 +145,13 @@ inline uint32_t unit_bytes(uint64_t bits, uint32_t element) {
     else { CALL(__nv_bfloat16, 2); }                        \
   }
 
-// A matrix of rows that is read: every row lies in [first, last).
+// A matrix of rows that is read.
 struct RowsIn {
   const uint8_t* first;
-  const uint8_t* last;
   uint64_t stride;
 };
-inline RowsIn rows_in(const void* base, uint64_t n, uint64_t stride, uint64_t row_bytes) {
-  const uint8_t* p = static_cast<const uint8_t*>(base);
-  return RowsIn{p, p + (n - 1) * stride + row_bytes, stride};
+inline RowsIn rows_in(const void* base, uint64_t stride) {
+  return RowsIn{static_cast<const uint8_t*>(base), stride};
 }
 
 int rows_fail(int code, const char* message) noexcept;
@@ -161,31 +159,15 @@ int rows_fail(int code, const char* message) noexcept;
 __device__ __forceinline__ void copy_async(uint32_t shared, const uint8_t* global) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared), "l"(global) : "memory");
 }
+// Its first `bytes` bytes (1 ... 16), and zeros: nothing behind them is read.
+__device__ __forceinline__ void copy_async(uint32_t shared, const uint8_t* global, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared), "l"(global), "r"(bytes)
+               : "memory");
+}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-// Those of the 16 bytes at `at` that lie in [from, to), element by element.
-template <int ELEMENT>
-__device__ __forceinline__ void copy_elements(uint32_t shared, const uint8_t* at, const uint8_t* from,
-                                              const uint8_t* to) {
-  using Raw = typename VecType<ELEMENT>::type;
-  Raw v[16 / ELEMENT];   // all on their way before the first is stored
-#pragma unroll
-  for (int b = 0; b < 16; b += ELEMENT) {
-    if (at + b >= from && at + b < to) v[b / ELEMENT] = __ldg(reinterpret_cast<const Raw*>(at + b));
-  }
-#pragma unroll
-  for (int b = 0; b < 16; b += ELEMENT) {
-    if (at + b < from || at + b >= to) continue;
-    if constexpr (ELEMENT == 4) {
-      asm volatile("st.shared.u32 [%0], %1;" ::"r"(shared + b), "r"(v[b / ELEMENT]) : "memory");
-    } else {
-      asm volatile("st.shared.u16 [%0], %1;" ::"r"(shared + b), "h"(v[b / ELEMENT]) : "memory");
-    }
-  }
 }
 
 template <int BYTES>
