@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(1024)
 // elements, weights and biases, 32 of each at most.
 template <typename T, int BYTES>
 const uint32_t* unit_choices() {
-  static const uint32_t whole[] = {2, 3, 4, 0}, pairs[] = {4, 8, 16, 0}, ones[] = {8, 12, 16, 32, 0};
+  static const uint32_t whole[] = {1, 2, 3, 4, 0}, pairs[] = {4, 8, 16, 0}, ones[] = {8, 12, 16, 32, 0};
   return BYTES == 16 ? whole : Unit<T, BYTES>::kElems == 2 ? pairs : ones;
 }
 
@@ -266,7 +266,14 @@ template <typename T, int BYTES>
 int launch_norm_type(const NormArgs& a, cudaStream_t stream) {
   const uint64_t units = a.dim / Unit<T, BYTES>::kElems;
   const RowsIn in = rows_in(a.x, a.x_stride);
-  const uint32_t per_thread = fitting_units(units, BYTES, unit_choices<T, BYTES>());
+  uint32_t per_thread = fitting_units(units, BYTES, unit_choices<T, BYTES>());
+  // rows of floats by address: two units, for two blocks per multiprocessor, whose
+  // warps wait for addresses and rows in turn (us, with two units and with four:
+  // 1048576 x 64 80 and 84, 262144 x 128 41 and 43, 65536 x 1024 76 and 76; but
+  // rows by base and stride 1048576 x 64 100 and 96)
+  if (BYTES == 16 && sizeof(T) == 4 && a.row_ptrs != nullptr && per_thread > 2 && units <= 2 * kPipeBlock) {
+    per_thread = 2;
+  }
   if (per_thread == 0) {
     const uint64_t cap = uint64_t(sm_count()) * 2;
     norm_long_kernel<T><<<unsigned(a.n < cap ? a.n : cap), 1024, 0, stream>>>(a);
@@ -290,6 +297,7 @@ int launch_norm_type(const NormArgs& a, cudaStream_t stream) {
 #define HKV_CALL(N) return launch_norm_pipe<T, BYTES, N>(a, group, in, stream)
   if constexpr (BYTES == 16) {
     switch (per_thread) {
+      case 1: HKV_CALL(1);
       case 2: HKV_CALL(2);
       case 3: HKV_CALL(3);
       default: HKV_CALL(4);
