@@ -473,8 +473,8 @@ constexpr int kMoveBlock = 256;
 //     units of 2        8 x 1: 64   8 x 2: 66   4 x 1: 94   4 x 2: 71   8 x 4: 82   12 x 1: 116
 //     units of 4        8 x 1: 30, 36   8 x 2: 29, 35   4 x 2: 28, 36   4 x 1: 29, 44   4 x 4: 26, 42
 //   gradient of combine 2 x 4: 93    2 x 2: 97, 29    1 x 4: 101    4 x 2: 97, 28
-//     units of 2        4 x 2: 149   4 x 1: 150   8 x 2: 164   8 x 1: 191   2 x 2: 208   8 x 4: 221
-//     units of 4        4 x 2: 45, 73   2 x 2: 47, 85   4 x 1: 50, 80   6 x 1: 50, 81   4 x 3: 50, 77
+//     units of 2        8 x 2: 129   4 x 3: 134   4 x 2: 142   8 x 1: 145
+//     units of 4        4 x 2: 45, 73   8 x 2: 48, 73   4 x 3: 57, 77   8 x 1: 64, 84
 struct Shape {
   int units, assigned;
 };
@@ -483,7 +483,7 @@ constexpr Shape dispatch_shape(int unit) {
 }
 constexpr Shape combine_shape(int unit) { return unit == 16 ? Shape{2, 2} : Shape{8, 1}; }
 constexpr Shape backward_shape(int unit, bool few) {
-  return unit != 16 || few ? Shape{4, 2} : Shape{2, 4};
+  return unit == 2 ? Shape{8, 2} : unit == 4 || few ? Shape{4, 2} : Shape{2, 4};
 }
 
 // The part of a token's row that a group of LANES lanes takes: V units per lane.
@@ -683,21 +683,27 @@ __device__ __forceinline__ void combine_backward_step(
     const typename Unit<T, BYTES>::Raw* const (&from)[J], typename Unit<T, BYTES>::Raw* const (&to)[J],
     float (&dot)[J]) {
   using U = Unit<T, BYTES>;
-  typename U::Raw d[V], row[J][V];
+  using Raw = typename U::Raw;
+  Raw d[V], row[J][V];
+  // from here on constants tell the units apart, which cost no instructions
+  const Raw* d_at = d_from + first;
+  const Raw* at[J];
+#pragma unroll
+  for (int u = 0; u < J; ++u) at[u] = from[u] + first;
   float part[J];   // the step's share of the dot products, added to them at once
 #pragma unroll
   for (int u = 0; u < J; ++u) part[u] = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    d[v] = no_unit<typename U::Raw>();
-    if (FULL || first + v * LANES < units) d[v] = __ldg(d_from + first + v * LANES);
+    d[v] = no_unit<Raw>();
+    if (FULL || first + v * LANES < units) d[v] = __ldg(d_at + v * LANES);
   }
 #pragma unroll
   for (int u = 0; u < J; ++u) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      row[u][v] = no_unit<typename U::Raw>();
-      if (FULL || first + v * LANES < units) row[u][v] = __ldg(from[u] + first + v * LANES);
+      row[u][v] = no_unit<Raw>();
+      if (FULL || first + v * LANES < units) row[u][v] = __ldg(at[u] + v * LANES);
     }
   }
 #pragma unroll
@@ -713,7 +719,7 @@ __device__ __forceinline__ void combine_backward_step(
         part[u] = fmaf(f[e], y[e], part[u]);
         y[e] = a.w[u] * f[e];
       }
-      if (a.ok[u] && (FULL || first + v * LANES < units)) to[u][first + v * LANES] = U::pack(y);
+      if (a.ok[u] && (FULL || first + v * LANES < units)) (to[u] + first)[v * LANES] = U::pack(y);
     }
   }
 #pragma unroll
