@@ -110,6 +110,8 @@ __global__ void __launch_bounds__(1024)
 
 // Many rows: the blocks stay on the device, their threads keep the weights of
 // their columns, and their groups take rows in turn out of the warps' queues.
+// Two blocks per multiprocessor where the registers allow (us, with two and with one:
+// 65537 x 333 half 23.2 and 24.5, 300000 x 100 half 36 and 42, 1048576 x 8 f32 12.5 and 15.0).
 template <typename T, int BYTES, int UNITS>
 constexpr int kResident = UNITS * Unit<T, BYTES>::kElems <= 12 ? 2 : 1;   // blocks, by their registers
 template <typename T, int BYTES, int UNITS, int WIDTH, bool BY_ADDRESS>
@@ -280,19 +282,23 @@ int launch_norm_type(const NormArgs& a, cudaStream_t stream) {
     return HKV_OK;
   }
   const uint32_t group = group_for(units, per_thread, BYTES);
-  // up to two rows for every group that the device holds are not worth a queue: a
-  // group of as many threads as the row has units (a few units each in long rows)
-  // takes one
-  if (a.n <= uint64_t(sm_count()) * (kPipeBlock / group) * 2) {
-    if constexpr (BYTES == 16) {
-      if (units <= 16) {
-        launch_norm_few<T, BYTES, 1, 0>(a, group_for(units, 1, BYTES), in, stream);
-        return HKV_OK;
-      }
+  // Few rows are not worth a queue: a group of as many threads as the row has units
+  // (two units each in long rows) takes one, as long as all of them run at once, in
+  // the 1024 threads per multiprocessor that their registers allow.  us, one row per
+  // group and queues: 5000 x 64 f32 2.4 and 3.7, 16 x 8192 bf16 3.5 and 3.7, 1000 x 1000
+  // bf16 3.2 and 3.7, 300 x 333 half 2.8 and 3.1; beyond it 20000 x 64 by
+  // address 4.6 and 4.2, 220 x 8192 6.1 and 4.2, 1700 x 1000 4.6 and 3.8, 500 x 333 3.5 and 3.1.
+  if (units <= 2048) {
+    const bool two = units > 1024, narrow_warp = BYTES == 16 && units <= 16;
+    const uint32_t threads = two           ? group_for(units, 2, BYTES)
+                             : narrow_warp ? group_for(units, 1, BYTES)
+                                           : uint32_t((units + 31) / 32 * 32);
+    if (a.n * threads <= uint64_t(sm_count()) * 1024) {
+      if (two) launch_norm_few<T, BYTES, 2, kWarps>(a, threads, in, stream);
+      else if (!narrow_warp) launch_norm_few<T, BYTES, 1, kWarps>(a, threads, in, stream);
+      else if constexpr (BYTES == 16) launch_norm_few<T, BYTES, 1, 0>(a, threads, in, stream);
+      return HKV_OK;
     }
-    if (units <= 1024) launch_norm_few<T, BYTES, 1, kWarps>(a, uint32_t((units + 31) / 32 * 32), in, stream);
-    else if (units <= 2048) launch_norm_few<T, BYTES, 2, kWarps>(a, group_for(units, 2, BYTES), in, stream);
-    if (units <= 2048) return HKV_OK;
   }
 #define HKV_CALL(N) return launch_norm_pipe<T, BYTES, N>(a, group, in, stream)
   if constexpr (BYTES == 16) {

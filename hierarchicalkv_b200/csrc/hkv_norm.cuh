@@ -97,10 +97,10 @@ struct UnitMap {
   }
   // f(c, mine) for the thread's units c, in runs of RUN: `mine` is a constant where
   // all lanes have the whole run, and runs that none has are left out.  One test
-  // serves rows that reach into the last run (65536 x 1001 bf16: 56 us, with a test
-  // per run 64, before other steps).  A single run is not tested, only its units, on a row of one warp or
-  // less (65536 x 1024 bf16: 45 us, with a test 49); on several warps, whose
-  // last may have none, it is (16384 x 8192 bf16: 102 us, without 113).
+  // serves rows that reach into the last run (65536 x 1001 bf16: 50 us, with a test
+  // per run 58).  A single run is not tested, only its units, on a row of one warp or
+  // less (262144 x 128 bf16: 22.2 us, with a test 23.6); on several warps, whose
+  // last may have none, it is (16384 x 8192 bf16: 91 us, without 110).
   template <int RUN, typename F>
   __device__ __forceinline__ void each(F&& f) const {
     static_assert(UNITS % RUN == 0, "whole runs");
@@ -343,10 +343,10 @@ inline uint32_t group_for(uint64_t units, uint32_t per_thread, uint32_t unit) {
 // Of the numbers of units per thread (ascending, 0 ends them) the one that leaves
 // the fewest places of the group empty; 0: the row is too long for a block.  A row
 // shared by warps counts one and a half times: its sums need barriers (65536 x
-// 1001 bf16: 126 us on four warps of 8 units per lane, 97 us on one of 32).  Of
+// 1001 bf16: 92 us on four warps of 8 units per lane, 50 us on one of 32).  Of
 // equals the most units per thread, for the fewest threads; but narrow units that fit
-// a warp the fewest, for the registers (1 Mi x 33 half, gradient: 131 us with 8
-// units on eight lanes, 149 us with 16).
+// a warp the fewest, for the registers (1 Mi x 33 half, gradient: 96 us with 8
+// units on eight lanes, 110 us with 16).
 inline uint32_t fitting_units(uint64_t units, uint32_t unit, const uint32_t* choices) {
   uint32_t best = 0;
   uint64_t least = 0;
