@@ -533,7 +533,9 @@ HKV_API int hkv_accum_or_assign_unique(hkv_table* table, uint64_t n, const uint6
  * Sums are in 32-bit floats, results are rounded once and do not depend on the
  * order in which blocks run.  The calls enqueue on `stream` (of the current
  * device), allocate nothing and keep nothing: they may be captured, and calls
- * that run at the same time need workspaces of their own. */
+ * that run at the same time need workspaces of their own.  Sizes that are refused
+ * (HKV_ERR_INVALID_ARG, nothing launched): 2^31 rows or assignments and more, rows to
+ * dispatch of 2^30 bytes, to combine of 2^28 elements, to normalise of 2^24. */
 
 /* Sorts the tokens * top_k assignments of tokens to experts by expert (buffers as
  * in include/merlin_hashtable.cuh:216-221).  expert_ids[tokens][top_k], int32 or
