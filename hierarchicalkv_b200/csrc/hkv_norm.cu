@@ -254,8 +254,13 @@ int launch_norm_width(const NormArgs& a, uint32_t group, const RowsIn& in, cudaS
 }
 template <typename T, int BYTES, int UNITS>
 int launch_norm_pipe(const NormArgs& a, uint32_t group, const RowsIn& in, cudaStream_t stream) {
-  if (group > 32) return launch_norm_width<T, BYTES, UNITS, kWarps>(a, group, in, stream);
-  if (group == 32) return launch_norm_width<T, BYTES, UNITS, 32>(a, group, in, stream);
+  // the widths that fitting_units() gives rows of so many units per thread
+  if constexpr (BYTES != 16 || UNITS != 1) {
+    if constexpr (BYTES == 16 || UNITS * Unit<T, BYTES>::kElems == 32) {
+      if (group > 32) return launch_norm_width<T, BYTES, UNITS, kWarps>(a, group, in, stream);
+    }
+    if (group == 32) return launch_norm_width<T, BYTES, UNITS, 32>(a, group, in, stream);
+  }
   if constexpr (BYTES == 16) return launch_norm_width<T, BYTES, UNITS, 0>(a, group, in, stream);
   else if (group == 16) return launch_norm_width<T, BYTES, UNITS, 16>(a, group, in, stream);
   else return launch_norm_width<T, BYTES, UNITS, 8>(a, group, in, stream);

@@ -347,12 +347,17 @@ inline uint32_t group_for(uint64_t units, uint32_t per_thread, uint32_t unit) {
 // equals the most units per thread, for the fewest threads; but narrow units that fit
 // a warp the fewest, for the registers (1 Mi x 33 half, gradient: 96 us with 8
 // units on eight lanes, 110 us with 16).
+// Not among them: one unit of 16 bytes where a warp or more has the row (60000 x 516
+// f32: 78 us with one, 46 with three; gradient 20000 x 2240 bf16 99 and 61 with two; but
+// 1048576 x 8 f32 12.5 with one, 14.4 with two), and narrow units on several warps unless
+// they are the most per thread.
 inline uint32_t fitting_units(uint64_t units, uint32_t unit, const uint32_t* choices) {
   uint32_t best = 0;
   uint64_t least = 0;
   for (; *choices != 0; ++choices) {
     const uint64_t group = group_for(units, *choices, unit);
     if (group > uint32_t(kPipeBlock)) continue;
+    if (unit == 16 ? *choices == 1 && group > 16 : choices[1] != 0 && group > 32) continue;
     // narrow units: runs of four that no lane of the group has are left out
     const uint64_t run = unit == 16 ? *choices : 4;
     const uint64_t width = group < 32 ? group : 32, warps = group / width;

@@ -295,8 +295,13 @@ int launch_backward_pipe(const NormBackwardArgs& a, const NormBackwardPlan& p, f
 template <typename T, int BYTES, int UNITS>
 int launch_backward_units(const NormBackwardArgs& a, const NormBackwardPlan& p, float* sums,
                           cudaStream_t stream) {
-  if (p.group > 32) return launch_backward_pipe<T, BYTES, UNITS, kWarps>(a, p, sums, stream);
-  if (p.group == 32) return launch_backward_pipe<T, BYTES, UNITS, 32>(a, p, sums, stream);
+  // the widths that fitting_units() gives rows of so many units per thread
+  if constexpr (BYTES != 16 || UNITS != 1) {
+    if constexpr (BYTES == 16 || UNITS * Unit<T, BYTES>::kElems == 16) {
+      if (p.group > 32) return launch_backward_pipe<T, BYTES, UNITS, kWarps>(a, p, sums, stream);
+    }
+    if (p.group == 32) return launch_backward_pipe<T, BYTES, UNITS, 32>(a, p, sums, stream);
+  }
   if constexpr (BYTES == 16) return launch_backward_pipe<T, BYTES, UNITS, 0>(a, p, sums, stream);
   else if (p.group == 16) return launch_backward_pipe<T, BYTES, UNITS, 16>(a, p, sums, stream);
   else return launch_backward_pipe<T, BYTES, UNITS, 8>(a, p, sums, stream);

@@ -386,6 +386,33 @@ def test_layer_norm_backward(n, dim, dtype, wide_params):
 
 
 @SIZED
+@pytest.mark.parametrize("dim", [1, 2, 7, 8, 16, 24, 33, 40, 64, 66, 100, 130, 161, 200, 256, 258, 333, 390, 449, 511, 516,
+                                 520, 776, 1001, 1032, 1160, 2049, 2240, 4104, 9000])
+def test_more_rows_than_run_at_once(dim, dtype):
+    """Batches that wait in queues, on every number of threads per row: whole, by
+    address with misses, strided, and the gradient."""
+    n = max(310000 // max(2, dim * torch.finfo(dtype).bits // 128), 3 * 148) + 3
+    x = norm_rows(n, dim, dim, dtype)
+    w, b = 1 + 0.2 * randn((dim,), 7), randn((dim,), 8)
+    y, mean, rstd = hkv.layer_norm(x, w, b)
+    check_norm(y, x, w, b, 1e-5, (mean, rstd))
+    wide = apart(x, 1)
+    padded, m, r = hkv.layer_norm(wide, w, b)
+    check_norm(padded, x, w, b, 1e-5, (m, r))
+    ptrs = x.data_ptr() + torch.arange(n, device="cuda") * (dim * x.element_size())
+    miss = torch.arange(n, device="cuda") % 5 == 2
+    ptrs[miss] = 0
+    out = torch.full_like(x, 5)
+    hkv.layer_norm_ptr(n, ptrs, out, w, b)
+    check_norm(out[~miss], x[~miss], w, b, 1e-5)
+    assert (out[miss] == 5).all()
+    dy = randn((n, dim), 5, dtype)
+    got = hkv.layer_norm_backward(dy, x, w, mean, rstd)
+    check_norm_grad(got, dy, x, w, mean, rstd)
+    check_norm_grad(hkv.layer_norm_backward(apart(dy, 1), wide, w, mean, rstd), dy, x, w, mean, rstd)
+
+
+@SIZED
 def test_layer_norm_backward_without_weight_or_bias_and_strided(dtype):
     n, dim = 77, 96
     x, dy = norm_rows(n, dim, 1, dtype), randn((n, dim), 5, dtype)
