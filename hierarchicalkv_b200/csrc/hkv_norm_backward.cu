@@ -13,9 +13,10 @@
 // into the warps' queues meanwhile, and their mean and rstd into registers (asked
 // for one row ahead instead of two they cost 59 us more at 16384 x 8192 bf16).  That
 // size takes 146 us, 82 % of what its bytes need, bound by the instructions that a
-// row costs its 16 warps beside the arithmetic; 1048576 x 64 f32 130 us, 97 %.  At the end each block writes one row of column sums (its groups
-// added in a fixed order), and norm_reduce_kernel adds the blocks' rows in a
-// fixed order: no atomics, the same bits every time.
+// row costs its 16 warps beside the arithmetic; 1048576 x 64 f32 130 us, 97 %.  At the
+// end each block writes one row of column sums (its groups added in a fixed order),
+// and norm_reduce_kernel adds the blocks' rows in a fixed order: no atomics, the same
+// bits every time.
 #include "hkv_norm.cuh"
 
 namespace hkv {
