@@ -463,6 +463,22 @@ void refuse_in_memory_mode(const hkv_table* t, const char* what) {
   }
 }
 
+// For calls that work in the table's scratch: a graph would keep the address of memory
+// that a later, larger call gives back, and its replays would take neither the scratch
+// nor the table's lock.  The legacy stream answers with an error while a blocking
+// stream is captured, and takes part in no capture then.
+void refuse_capture(cudaStream_t stream, const char* what) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  const cudaError_t e = cudaStreamIsCapturing(stream, &status);
+  if (e != cudaSuccess) cudaGetLastError();
+  if (e != cudaSuccess && e != cudaErrorStreamCaptureImplicit) {
+    throw HkvError{HKV_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e)};
+  }
+  if (e != cudaSuccess || status != cudaStreamCaptureStatusNone) {
+    throw HkvError{HKV_ERR_MERLIN, std::string(what) + "() is not for use inside a stream capture."};
+  }
+}
+
 // accum_or_assign adds elements of V (include/merlin/core_kernels/accum_or_assign.cuh:139-172):
 // the element type must be known and a row chunk must hold whole elements.
 void check_accum_type(const hkv_table* t, const void* batch) {
@@ -1271,6 +1287,7 @@ int hkv_find_layer_norm(hkv_table* t, uint64_t n, const uint64_t* keys, const vo
     }
     DeviceGuard dg(t->device);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    refuse_capture(s, "find_layer_norm");
     WorkspaceLease work(t, 0, n * sizeof(void*), s);   // the rows' addresses
     if (work.get() == nullptr) {
       throw HkvError{HKV_ERR_CUDA, "find_layer_norm: out of device memory for the row addresses"};

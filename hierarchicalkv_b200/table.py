@@ -459,7 +459,8 @@ class HashTable:
         ``weight`` / ``bias`` (dim elements of the value type or float32, both of
         one type; None: ones / zeros), ``mean`` / ``rstd`` (float32, optional):
         what layer_norm_backward needs.  Values must be float32, float16 or
-        bfloat16."""
+        bfloat16.  Not for use inside a stream capture: the call works in the
+        table's scratch, and a capture is refused."""
         dim = self._opts.dim if self._opts is not None else 0
         kind = None
         for name, p in (("weight", weight), ("bias", bias)):

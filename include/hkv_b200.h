@@ -533,7 +533,8 @@ HKV_API int hkv_accum_or_assign_unique(hkv_table* table, uint64_t n, const uint6
  * Sums are in 32-bit floats, results are rounded once and do not depend on the
  * order in which blocks run.  The calls enqueue on `stream` (of the current
  * device), allocate nothing and keep nothing: they may be captured, and calls
- * that run at the same time need workspaces of their own.  Sizes that are refused
+ * that run at the same time need workspaces of their own.  hkv_find_layer_norm
+ * is a call of its table in all of this (see there).  Sizes that are refused
  * (HKV_ERR_INVALID_ARG, nothing launched): 2^31 rows or assignments and more, rows to
  * dispatch of 2^30 bytes, to combine of 2^28 elements, to normalise of 2^24. */
 
@@ -600,7 +601,11 @@ HKV_API int hkv_layer_norm_ptr(uint64_t n, uint64_t dim, uint32_t value_kind,
 /* HashTable::find (include/merlin_hashtable.cuh:2464-2577) whose rows go through
  * layer norm on their way out: find* and hkv_layer_norm_ptr under one reader lock.
  * values[n][dim] has the table's element type (float, half or bfloat16); rows of
- * misses are left as they are, founds[n] tells which. */
+ * misses are left as they are, founds[n] tells which.  The addresses wait in the
+ * table's own scratch, which grows with the largest n: the call may allocate, and
+ * inside a stream capture it is refused (HKV_ERR_MERLIN, nothing launched; a graph
+ * would keep the address of scratch that a larger call replaces, and replay without
+ * the lock). */
 HKV_API int hkv_find_layer_norm(hkv_table* table, uint64_t n, const uint64_t* keys,
                                 const void* weight, const void* bias, uint32_t param_kind,
                                 float eps, void* values, bool* founds, float* mean, float* rstd,

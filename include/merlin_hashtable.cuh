@@ -629,7 +629,8 @@ class HashTable : public HashTableBase<K, V, S> {
    * (not in the reference): they are normalised straight from the table.  V is
    * float, __half or __nv_bfloat16; `weight` and `bias` (dim elements of V or
    * float, null: ones / zeros) and `mean` / `rstd` (n floats, null: not kept)
-   * are device pointers.  Rows of misses are left as they are.
+   * are device pointers.  Rows of misses are left as they are.  Not for use
+   * inside a stream capture.
    */
   template <class P = V>
   void find_layer_norm(const size_type n, const key_type* keys, const P* weight, const P* bias,
