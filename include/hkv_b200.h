@@ -583,7 +583,9 @@ HKV_API int hkv_expert_combine_backward(uint64_t tokens, uint32_t top_k, uint64_
 /* y = (x - mean) * rstd * weight + bias over rows of dim elements (those find
  * returns, include/merlin_hashtable.cuh:2464-2577), rstd = 1 / sqrt(var + eps) with the
  * variance over dim.  weight / bias null: ones / zeros.  mean and rstd (n floats
- * each, may be null) are what the gradient needs. */
+ * each, may be null) are what the gradient needs.  Rows far from zero keep the
+ * precision of their deviations in y; the mean kept for the gradient is rounded to a
+ * float, which is all the gradient then knows of it. */
 HKV_API int hkv_layer_norm(uint64_t n, uint64_t dim, uint32_t value_kind, const void* x,
                            uint64_t x_stride, const void* weight, const void* bias,
                            uint32_t param_kind, float eps, void* y, uint64_t y_stride, float* mean,

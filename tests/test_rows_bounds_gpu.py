@@ -54,3 +54,85 @@ def test_find_layer_norm_is_refused_inside_a_capture(warm):
     t.find_layer_norm(n, keys, out, found)
     assert found.all() and torch.equal(out, want)
     t.close()
+
+
+# ---- layer norm of rows far from zero --------------------------------------------------
+
+U = 2.0 ** -24
+
+
+def rounded(value, dtype):
+    """How far rounding `value` to dtype may move it."""
+    f = torch.finfo(dtype)
+    return value.abs() * (f.eps / 2) + f.smallest_normal * f.eps / 2
+
+
+def check(got, want, bound, what=""):
+    off = (got.double() - want).abs()
+    bad = ~(off <= bound)     # a NaN is bad
+    assert not bad.any(), (what, int(bad.sum()), float(off[bad].max()), float((off / bound.clamp(min=1e-300)).max()))
+
+
+def check_centred(x, w, b, eps, y, mean, rstd):
+    """Layer norm of rows whose mean is corrected by the mean of the distances from it.
+
+    L u bounds the relative error of a sum of the row (its terms pass at most L additions)
+    with the division; the first mean is off by first = (L + 3) u mean|x|.  A distance from
+    it is at most |x - m| + first and rounded to u of that, so the correction, itself at
+    most first, is off by second = (L + 4) u (mean|x - m| + first).  Behind it a distance
+    is off by 2 u (|x - m| + first) + second: the size of x counts in second order only.
+    The variance, of corrected distances: (L + 5) u (var + second^2) + second^2; rsqrtf
+    adds 4 u, the products and the last sum 4 u."""
+    x = x.double()
+    m = x.mean(1, keepdim=True)
+    d = x - m
+    var = (d * d).mean(1, keepdim=True)
+    want_rstd = (var + eps) ** -0.5
+    terms = (max(64, x.shape[1] // 256) + 48 + 3) * U
+    first = terms * x.abs().mean(1, keepdim=True)
+    second = (terms + U) * (d.abs().mean(1, keepdim=True) + first)
+    centred = 2 * U * (d.abs() + first) + second
+    rel = ((terms + 2 * U) * (var + second ** 2) + second ** 2) / (var + eps) + 4 * U
+    w, b = w.double(), b.double()
+    want = d * want_rstd * w + b
+    off = w.abs() * want_rstd * centred * (1 + rel) + (w * d * want_rstd).abs() * (rel + 4 * U) + 2 * U * want.abs()
+    check(y, want, off + rounded(want, y.dtype), "y")
+    check(mean, m[:, 0], (second + 2 * U * first)[:, 0] + U * m[:, 0].abs(), "mean")
+    check(rstd, want_rstd[:, 0], ((rel + U) * want_rstd)[:, 0], "rstd")
+
+
+@pytest.mark.parametrize("n,dim", [(3, 7), (5, 333), (4, 1000), (3, 5000), (2, 12001), (2, 50000), (9000, 333),
+                                   (4000, 1000), (3000, 1001), (500, 5000), (200, 12001), (20000, 100), (100000, 12)])
+@pytest.mark.parametrize("spread", [0.0, 1.0])
+@pytest.mark.parametrize("far", [1.0e3, 3.0e4, -7.0e6])
+def test_layer_norm_of_rows_far_from_zero(n, dim, spread, far):
+    """No length here is a power of two, so 1 / dim is rounded: constant rows come out as
+    the bias, and rows that vary by 1 about a large value lose no more than the type does."""
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    x = far + spread * torch.randn((n, dim), generator=g, device="cuda")
+    w, b = 1 + 0.2 * torch.randn(dim, generator=g, device="cuda"), torch.randn(dim, generator=g, device="cuda")
+    y, mean, rstd = hkv.layer_norm(x, w, b)
+    check_centred(x, w, b, 1e-5, y, mean, rstd)
+    out = torch.zeros_like(x)
+    ptrs = x.data_ptr() + torch.arange(n, device="cuda") * (dim * 4)
+    hkv.layer_norm_ptr(n, ptrs, out, w, b, 1e-5, mean, rstd)
+    check_centred(x, w, b, 1e-5, out, mean, rstd)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("n,dim", [(4, 1000), (4000, 1000), (20, 333), (9000, 333), (2, 40002)])
+def test_layer_norm_of_short_types_far_from_zero(n, dim, dtype):
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    x = (2.0e4 + 100 * torch.randn((n, dim), generator=g, device="cuda")).to(dtype)
+    x[0] = 3.0e4
+    w, b = 1 + 0.2 * torch.randn(dim, generator=g, device="cuda"), torch.randn(dim, generator=g, device="cuda")
+    check_centred(x, w, b, 1e-5, *hkv.layer_norm(x, w, b))
+
+
+def test_layer_norm_of_huge_rows_stays_finite():
+    """Where a rounding error's square overflows, rstd is 0 and the bias is left."""
+    for dim in (1000, 333, 20000):
+        x = torch.full((2, dim), 1.0e31, device="cuda")
+        x[1] = -3.0e33
+        b = torch.randn(dim, device="cuda")
+        assert torch.equal(hkv.layer_norm(x, None, b, stats=False), b.expand(2, dim))
