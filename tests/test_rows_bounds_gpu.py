@@ -136,3 +136,34 @@ def test_layer_norm_of_huge_rows_stays_finite():
         x[1] = -3.0e33
         b = torch.randn(dim, device="cuda")
         assert torch.equal(hkv.layer_norm(x, None, b, stats=False), b.expand(2, dim))
+
+
+# ---- expert sort of batches with large tiles ---------------------------------------------
+
+
+def check_order(order, ids, experts):
+    flat = ids.cpu().numpy().reshape(-1).astype(np.int64)
+    kept = np.flatnonzero((flat >= 0) & (flat < experts))
+    taken = kept[np.argsort(flat[kept], kind="stable")]
+    position = np.full(flat.size, -1, np.int32)
+    position[taken] = np.arange(taken.size)
+    source = np.full(flat.size, -1, np.int32)
+    source[:taken.size] = taken
+    offsets = np.concatenate([[0], np.cumsum(np.bincount(flat[kept], minlength=experts))])
+    np.testing.assert_array_equal(order.offsets.cpu().numpy(), offsets)
+    np.testing.assert_array_equal(order.position.cpu().numpy().reshape(-1), position)
+    np.testing.assert_array_equal(order.source.cpu().numpy(), source)
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64], ids=["i32", "i64"])
+@pytest.mark.parametrize("tokens,top_k,experts", [((1 << 21) + 1, 1, 64), (625001, 8, 8), (1100000, 1, 1024),
+                                                  (1100009, 2, 1), (1400001, 3, 512)])
+def test_sort_of_sixteen_ids_per_lane(tokens, top_k, experts, dtype):
+    """Above 512 tiles of four ids per lane a tile has sixteen: uneven experts, a tenth
+    dropped, and one expert for all, which brings the counters to their largest sums."""
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    ids = (torch.rand((tokens, top_k), generator=g, device="cuda") ** 2 * experts * 1.06).long() - 1
+    ids = ids.to(dtype)
+    check_order(hkv.expert_sort(ids, experts), ids, experts)
+    ids.fill_(experts - 1)
+    check_order(hkv.expert_sort(ids, experts), ids, experts)
