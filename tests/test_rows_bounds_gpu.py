@@ -167,3 +167,82 @@ def test_sort_of_sixteen_ids_per_lane(tokens, top_k, experts, dtype):
     check_order(hkv.expert_sort(ids, experts), ids, experts)
     ids.fill_(experts - 1)
     check_order(hkv.expert_sort(ids, experts), ids, experts)
+
+
+# ---- offsets past 32 bits --------------------------------------------------------------
+
+
+def far_apart(rows, stride):
+    """The same rows, `stride` elements apart, 4 GiB and more in all."""
+    assert rows.shape[0] * stride * rows.element_size() > 2 ** 32
+    wide = torch.empty(rows.shape[0] * stride, dtype=rows.dtype, device="cuda")
+    out = wide.as_strided(rows.shape, (stride, 1))
+    out.copy_(rows)
+    return out
+
+
+WIDE = [(600, 1001, torch.bfloat16, 8000001), (600, 1024, torch.bfloat16, 8000000), (600, 2050, torch.float16, 8000002),
+        (800, 333, torch.float32, 2000001), (40, 1001, torch.bfloat16, 80000001), (6, 40000, torch.float32, 200000000)]
+BY_WIDTH = pytest.mark.parametrize("n,dim,dtype,stride", WIDE, ids=[f"{n}x{d}" for n, d, _, _ in WIDE])
+
+
+@BY_WIDTH
+def test_layer_norm_past_32_bit_offsets(n, dim, dtype, stride):
+    """Rows far apart give the bits of the same rows side by side (which the other tests
+    hold to the formula): the units, and with them the sums' order, are the same."""
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    x = torch.randn((n, dim), generator=g, device="cuda").to(dtype)
+    dy = torch.randn((n, dim), generator=g, device="cuda").to(dtype)
+    w, b = 1 + 0.2 * torch.randn(dim, generator=g, device="cuda"), torch.randn(dim, generator=g, device="cuda")
+    want = hkv.layer_norm(x, w, b)
+    wide_x, out = far_apart(x, stride), far_apart(torch.zeros_like(x), stride)
+    got = hkv.layer_norm(wide_x, w, b, out=out)
+    assert got[0] is out and all(torch.equal(p, q) for p, q in zip(got, want))
+    ptrs = wide_x.data_ptr() + torch.arange(n, device="cuda") * (stride * x.element_size())
+    near = x.data_ptr() + torch.arange(n, device="cuda") * (dim * x.element_size())
+    out.zero_()
+    assert torch.equal(hkv.layer_norm_ptr(n, ptrs, out, w, b), hkv.layer_norm_ptr(n, near, torch.zeros_like(x), w, b))
+    want = hkv.layer_norm_backward(dy, x, w, *want[1:])
+    got = hkv.layer_norm_backward(far_apart(dy, stride), wide_x, w, *got[1:], out=out)
+    assert got[0] is out and all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@BY_WIDTH
+def test_experts_past_32_bit_offsets(n, dim, dtype, stride):
+    top_k, experts = 2, 5
+    tokens = n // top_k
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    order = hkv.expert_sort(torch.randint(-1, experts, (tokens, top_k), generator=g, device="cuda"), experts)
+    m = int(order.offsets[-1])
+    y = torch.randn((n, dim), generator=g, device="cuda").to(dtype)
+    x = torch.randn((tokens, dim), generator=g, device="cuda").to(dtype)
+    wt = torch.randn((tokens, top_k), generator=g, device="cuda")
+    wide_y, wide_x = far_apart(y, stride), far_apart(x, stride * top_k)
+    rows, out = far_apart(torch.zeros_like(y), stride), far_apart(torch.zeros_like(x), stride * top_k)
+    assert torch.equal(hkv.expert_dispatch(wide_x, order, out=rows)[:m], hkv.expert_dispatch(x, order)[:m])
+    assert torch.equal(hkv.expert_combine(wide_y, wt, order, out=out), hkv.expert_combine(y, wt, order))
+    assert torch.equal(hkv.expert_dispatch_backward(wide_y, order, out=out), hkv.expert_dispatch_backward(y, order))
+    d_rows, d_wt = hkv.expert_combine_backward(wide_x, wide_y, wt, order, out=rows)
+    want_rows, want_wt = hkv.expert_combine_backward(x, y, wt, order)
+    assert torch.equal(d_rows[:m], want_rows[:m]) and torch.equal(d_wt, want_wt)
+
+
+def test_experts_of_a_batch_above_four_gigabytes():
+    """Every row without a gap: whole numbers, whose sums are exact in any order."""
+    tokens, top_k, dim = 70000, 2, 16384
+    g = torch.Generator(device="cuda").manual_seed(1)
+    order = hkv.expert_sort(torch.randint(0, 4, (tokens, top_k), generator=g, device="cuda"), 4)
+    t = torch.arange(tokens, device="cuda")
+    x = ((t % 5)[:, None] + (torch.arange(dim, device="cuda") % 2)).to(torch.bfloat16)
+    rows = hkv.expert_dispatch(x, order)
+    assert rows.numel() * 2 > 2 ** 32
+    token = order.source.long() // top_k
+    assert all(torch.equal(rows[i:i + 20000], x[token[i:i + 20000]]) for i in range(0, tokens * top_k, 20000))
+    wt = torch.tensor([0.5, 2.0], device="cuda").expand(tokens, top_k).contiguous()
+    assert torch.equal(hkv.expert_combine(rows, wt, order), x * 2.5)
+    d_rows, d_wt = hkv.expert_combine_backward(x, rows, wt, order)
+    factor = wt.view(-1)[order.source.long()].to(torch.bfloat16)[:, None]
+    for i in range(0, tokens * top_k, 20000):
+        assert torch.equal(d_rows[i:i + 20000], x[token[i:i + 20000]] * factor[i:i + 20000])
+    dots = dim // 2 * ((t % 5) ** 2 + (t % 5 + 1) ** 2)
+    assert torch.equal(d_wt, dots.float()[:, None].expand(tokens, top_k))
