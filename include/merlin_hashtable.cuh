@@ -639,6 +639,28 @@ class HashTable : public HashTableBase<K, V, S> {
     detail::rethrow(hkv_find_layer_norm(table_, n, u(keys), weight, bias, detail::value_kind_of<P>(),
                                         eps, values, founds, mean, rstd, stream));
   }
+  // A null pointer constant has no type to deduce P from: the other parameter's, or V.
+  template <class P>
+  void find_layer_norm(const size_type n, const key_type* keys, const P* weight, std::nullptr_t,
+                       const float eps, value_type* values, bool* founds, float* mean = nullptr,
+                       float* rstd = nullptr, cudaStream_t stream = 0) const {
+    find_layer_norm<P>(n, keys, weight, static_cast<const P*>(nullptr), eps, values, founds, mean,
+                       rstd, stream);
+  }
+  template <class P>
+  void find_layer_norm(const size_type n, const key_type* keys, std::nullptr_t, const P* bias,
+                       const float eps, value_type* values, bool* founds, float* mean = nullptr,
+                       float* rstd = nullptr, cudaStream_t stream = 0) const {
+    find_layer_norm<P>(n, keys, static_cast<const P*>(nullptr), bias, eps, values, founds, mean,
+                       rstd, stream);
+  }
+  template <class P = V>
+  void find_layer_norm(const size_type n, const key_type* keys, std::nullptr_t, std::nullptr_t,
+                       const float eps, value_type* values, bool* founds, float* mean = nullptr,
+                       float* rstd = nullptr, cudaStream_t stream = 0) const {
+    const P* none = nullptr;
+    find_layer_norm<P>(n, keys, none, none, eps, values, founds, mean, rstd, stream);
+  }
 
   void find(const size_type n, const key_type* keys, value_type* values, key_type* missed_keys,
             int* missed_indices, int* missed_size, score_type* scores = nullptr,
