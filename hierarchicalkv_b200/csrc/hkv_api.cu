@@ -1270,6 +1270,7 @@ int hkv_find_layer_norm(hkv_table* t, uint64_t n, const uint64_t* keys, const vo
                         const void* bias, uint32_t param_kind, float eps, void* values,
                         bool* founds, float* mean, float* rstd, hkv_stream stream) {
   return guarded([&] {
+    if (t == nullptr) throw HkvError{HKV_ERR_INVALID_ARG, "find_layer_norm: there is no table"};
     refuse_in_memory_mode(t, "find_layer_norm");
     uint32_t kind = t->view.value_kind;
     if (kind == hkv::kValueOpaque && t->opt.value_size == 4) kind = hkv::kValueF32;

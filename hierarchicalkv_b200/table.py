@@ -473,11 +473,24 @@ class HashTable:
             kind = p.dtype
         if values.dtype != self.value_dtype or values.numel() < n * dim:
             raise ValueError("values must hold n rows of the table's value type")
-        if keys.numel() < n or founds.numel() < n:
-            raise ValueError("keys and founds must hold n elements")
+        if keys.numel() < n or keys.element_size() != 8 or keys.is_floating_point():
+            raise ValueError("keys must hold n 64-bit integers")
+        if founds.numel() < n or founds.element_size() != 1:
+            raise ValueError("founds must hold n elements of one byte")
         for name, s in (("mean", mean), ("rstd", rstd)):
             if s is not None and (s.dtype != torch.float32 or s.numel() < n):
                 raise ValueError(f"{name} must hold n float32 elements")
+        device = values.get_device()
+        for name, p in (("keys", keys), ("values", values), ("founds", founds), ("weight", weight),
+                        ("bias", bias), ("mean", mean), ("rstd", rstd)):
+            if p is None:
+                continue
+            if not p.is_cuda:
+                reached = p.is_pinned()
+            else:
+                reached = p.get_device() == device or not values.is_cuda
+            if not reached:
+                raise ValueError(f"{name} must be on the GPU of values, or in pinned host memory")
         self._call("hkv_find_layer_norm", n, _ptr(keys), _ptr(weight), _ptr(bias),
                    _VALUE_KINDS.get(kind or self.value_dtype, 0), eps, _ptr(values), _ptr(founds),
                    _ptr(mean), _ptr(rstd), _stream(stream))

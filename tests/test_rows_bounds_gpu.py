@@ -246,3 +246,19 @@ def test_experts_of_a_batch_above_four_gigabytes():
         assert torch.equal(d_rows[i:i + 20000], x[token[i:i + 20000]] * factor[i:i + 20000])
     dots = dim // 2 * ((t % 5) ** 2 + (t % 5 + 1) ** 2)
     assert torch.equal(d_wt, dots.float()[:, None].expand(tokens, top_k))
+
+
+def test_find_layer_norm_with_pinned_buffers():
+    """What a kernel can reach it may use, as find may: pinned host memory."""
+    dim, n = 16, 500
+    t = make_table(dim)
+    keys, rows = to_dev(unique_keys(n, seed=2)), torch.randn((n, dim), device="cuda")
+    t.insert_or_assign(n, keys, rows)
+    out, found = torch.zeros((n, dim)).pin_memory(), torch.zeros(n, dtype=torch.bool).pin_memory()
+    w = (1 + torch.rand(dim)).pin_memory()
+    t.find_layer_norm(n, keys.cpu().pin_memory(), out, found, w)
+    torch.cuda.synchronize()
+    assert found.all() and torch.equal(out, hkv.layer_norm(rows, w.cuda(), stats=False).cpu())
+    with pytest.raises(ValueError, match="founds must be on the GPU"):
+        t.find_layer_norm(n, keys, rows, torch.zeros(n, dtype=torch.bool))
+    t.close()
