@@ -877,6 +877,8 @@ int hkv_expert_sort(uint64_t tokens, uint32_t top_k, const void* expert_ids, uin
   HKV_ROWS_CHECK(work_bytes >= hkv_expert_sort_workspace_bytes(tokens, top_k, experts) &&
                      (work_bytes == 0 || work != nullptr),
                  "workspace smaller than hkv_expert_sort_workspace_bytes");
+  HKV_ROWS_CHECK(all_aligned(id_bytes, expert_ids) && all_aligned(4, offsets, position, source, work),
+                 "a buffer does not start at a multiple of its element size, or work of 4");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return id_bytes == 4
              ? launch_sort(n, static_cast<const int32_t*>(expert_ids), experts, offsets, position,
@@ -896,6 +898,8 @@ int hkv_expert_dispatch(uint64_t tokens, uint32_t top_k, uint64_t row_bytes, con
   if (tokens == 0) return HKV_OK;
   HKV_ROWS_CHECK(x != nullptr && position != nullptr && rows != nullptr && offsets != nullptr,
                  "x, offsets, position and rows must not be null");
+  HKV_ROWS_CHECK(all_aligned(4, offsets, position),
+                 "offsets and position must start at a multiple of their element size");
   const uint64_t bits = row_bytes | address_bits(x) | x_stride | address_bits(rows) | rows_stride;
   uint32_t unit = 16;
   while (bits % unit != 0) unit >>= 1;
@@ -940,6 +944,8 @@ int hkv_expert_combine(uint64_t tokens, uint32_t top_k, uint64_t dim, uint32_t v
   if (tokens == 0) return HKV_OK;
   HKV_ROWS_CHECK(rows != nullptr && position != nullptr && out != nullptr,
                  "rows, position and out must not be null");
+  HKV_ROWS_CHECK(all_aligned(4, position) && all_aligned(row_kind_size(weight_kind), weights),
+                 "position and weights must start at a multiple of their element size");
   const uint64_t row_bytes = dim * size;
   const uint32_t unit =
       unit_bytes(row_bytes | address_bits(rows) | rows_stride | address_bits(out) | out_stride, size);
@@ -985,6 +991,9 @@ int hkv_expert_combine_backward(uint64_t tokens, uint32_t top_k, uint64_t dim, u
   HKV_ROWS_CHECK(d_out != nullptr && rows != nullptr && weights != nullptr && offsets != nullptr &&
                      position != nullptr && d_rows != nullptr && d_weights != nullptr,
                  "no argument may be null");
+  HKV_ROWS_CHECK(all_aligned(4, offsets, position) &&
+                     all_aligned(row_kind_size(weight_kind), weights, d_weights),
+                 "offsets, position and weights must start at a multiple of their element size");
   const uint64_t row_bytes = dim * size;
   const uint32_t unit = unit_bytes(row_bytes | address_bits(d_out) | d_out_stride | address_bits(rows) |
                                        rows_stride | address_bits(d_rows) | d_rows_stride,

@@ -419,6 +419,8 @@ int hkv_layer_norm(uint64_t n, uint64_t dim, uint32_t value_kind, const void* x,
   HKV_ROWS_CHECK(y_stride >= dim * row_kind_size(value_kind), "the output rows overlap");
   if (n == 0) return HKV_OK;
   HKV_ROWS_CHECK(x != nullptr && y != nullptr, "x and y must not be null");
+  HKV_ROWS_CHECK(all_aligned(row_kind_size(param_kind), weight, bias) && all_aligned(4, mean, rstd),
+                 "weight, bias, mean and rstd must start at a multiple of their element size");
   NormArgs a{};
   a.n = n;
   a.dim = dim;
@@ -445,6 +447,9 @@ int hkv_layer_norm_ptr(uint64_t n, uint64_t dim, uint32_t value_kind, const void
   HKV_ROWS_CHECK(y_stride >= dim * row_kind_size(value_kind), "the output rows overlap");
   if (n == 0) return HKV_OK;
   HKV_ROWS_CHECK(row_ptrs != nullptr && y != nullptr, "row_ptrs and y must not be null");
+  HKV_ROWS_CHECK(all_aligned(row_kind_size(param_kind), weight, bias) && all_aligned(4, mean, rstd) &&
+                     all_aligned(8, row_ptrs),
+                 "weight, bias, mean, rstd and row_ptrs must start at a multiple of their element size");
   NormArgs a{};
   a.n = n;
   a.dim = dim;

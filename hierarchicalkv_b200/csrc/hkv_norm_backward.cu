@@ -399,6 +399,9 @@ int hkv_layer_norm_backward(uint64_t n, uint64_t dim, uint32_t value_kind, const
                      (work != nullptr &&
                       work_bytes >= hkv_layer_norm_backward_workspace_bytes(n, dim, value_kind)),
                  "workspace smaller than hkv_layer_norm_backward_workspace_bytes");
+  HKV_ROWS_CHECK(all_aligned(row_kind_size(param_kind), weight, d_weight, d_bias) &&
+                     all_aligned(4, mean, rstd, work),
+                 "a buffer does not start at a multiple of its element size, or work of 4");
   NormBackwardArgs a{};
   a.n = n;
   a.dim = dim;

@@ -122,6 +122,12 @@ __device__ __forceinline__ Raw no_unit() {
 
 inline uint64_t address_bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
+// Whether every address is a multiple of `bytes` (null is).
+template <typename... P>
+inline bool all_aligned(uint32_t bytes, const P*... p) {
+  return ((address_bits(p) | ...) & (bytes - 1u)) == 0;
+}
+
 // Unit for rows whose addresses, strides and lengths in bytes have these bits (or
 // of all of them) set: 16, 4 or one element; 0 where an element would be split.
 inline uint32_t unit_bytes(uint64_t bits, uint32_t element) {

@@ -525,8 +525,8 @@ HKV_API int hkv_accum_or_assign_unique(hkv_table* table, uint64_t n, const uint6
 /* ---- row operators of a model ------------------------------------------------
  * What a model does with the rows of a table next: layer norm, and the routing
  * of token rows to experts and back.  No counterpart in the reference.  Buffers
- * must be GPU-accessible and start at a multiple of their element size, as
- * everywhere (include/merlin_hashtable.cuh:216-221); strides are in bytes;
+ * must be GPU-accessible and start at a multiple of their element size (`work` of
+ * 4 bytes), as everywhere (include/merlin_hashtable.cuh:216-221); strides are in bytes;
  * rows may lie apart, a row itself is contiguous; outputs must not overlap inputs.
  * value_kind (HKV_VALUE_F32 / F16 / BF16) names the rows' element type; weights,
  * biases and their gradients have that type or float (weight_kind / param_kind).
