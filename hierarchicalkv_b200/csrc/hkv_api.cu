@@ -12,6 +12,7 @@
 #include <condition_variable>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <stdexcept>
@@ -1285,6 +1286,18 @@ int hkv_find_layer_norm(hkv_table* t, uint64_t n, const uint64_t* keys, const vo
     if (n >= (1ull << 31) || keys == nullptr || values == nullptr || founds == nullptr) {
       throw HkvError{HKV_ERR_INVALID_ARG,
                      "find_layer_norm: keys, values and founds must not be null, n below 2^31"};
+    }
+    const auto starts_at = [](uint32_t size, std::initializer_list<const void*> buffers) {
+      for (const void* p : buffers) {
+        if (reinterpret_cast<uintptr_t>(p) % size != 0) return false;
+      }
+      return true;
+    };
+    const uint32_t value_size = uint32_t(t->opt.value_size);
+    if (!starts_at(8, {keys}) || !starts_at(value_size, {values}) || !starts_at(4, {mean, rstd}) ||
+        !starts_at(param_kind == hkv::kValueF32 ? 4u : value_size, {weight, bias})) {
+      throw HkvError{HKV_ERR_INVALID_ARG,
+                     "find_layer_norm: a buffer does not start at a multiple of its element size"};
     }
     DeviceGuard dg(t->device);
     cudaStream_t s = static_cast<cudaStream_t>(stream);

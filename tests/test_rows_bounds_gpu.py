@@ -262,3 +262,24 @@ def test_find_layer_norm_with_pinned_buffers():
     with pytest.raises(ValueError, match="founds must be on the GPU"):
         t.find_layer_norm(n, keys, rows, torch.zeros(n, dtype=torch.bool))
     t.close()
+
+
+def test_find_layer_norm_refuses_misaligned_buffers_before_the_lookup():
+    """At the C entry (tensors start at a multiple of their element): nothing has run."""
+    dim, n = 8, 100
+    t = make_table(dim)
+    keys, rows = to_dev(unique_keys(n, seed=2)), torch.randn((n, dim), device="cuda")
+    t.insert_or_assign(n, keys, rows)
+    out, found = torch.full((n, dim), 5.0, device="cuda"), torch.zeros(n, dtype=torch.bool, device="cuda")
+    spare = torch.full((n,), 5.0, device="cuda")
+    fine = dict(keys=keys.data_ptr(), weight=spare.data_ptr(), bias=spare.data_ptr(), values=out.data_ptr(),
+                mean=spare.data_ptr(), rstd=spare.data_ptr())
+    stream = torch.cuda.current_stream().cuda_stream
+    for name in fine:
+        p = {**fine, name: fine[name] + (4 if name == "keys" else 2)}
+        rc = t._lib.hkv_find_layer_norm(t._h, n, p["keys"], p["weight"], p["bias"], 1, 1e-5, p["values"],
+                                        found.data_ptr(), p["mean"], p["rstd"], stream)
+        assert rc == 4 and b"element size" in t._lib.hkv_last_error(), name
+    torch.cuda.synchronize()
+    assert not found.any() and (out == 5).all() and (spare == 5).all()
+    t.close()
