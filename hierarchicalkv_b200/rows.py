@@ -258,6 +258,8 @@ def expert_combine_backward(d_out: torch.Tensor, rows: torch.Tensor, weights: to
     ``out``; the weights of dropped assignments get 0."""
     if _elsewhere(d_out, stream):
         return _run_there(expert_combine_backward, d_out, stream, d_out, rows, weights, order, out)
+    if weights is None:
+        raise ValueError("weights must be those of expert_combine")
     n, dim, d_stride, kind = _float_rows(d_out, "d_out")
     tokens, top_k, experts, offsets, position = _order(order, d_out)
     if n != tokens:
