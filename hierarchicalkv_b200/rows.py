@@ -78,6 +78,8 @@ def _rows(t: torch.Tensor, name: str):
     stride, step = t.stride()
     if step != 1 and dim > 1:
         raise ValueError(f"the rows of {name} must be contiguous")
+    if dim == 1 and t.is_neg():    # such views are two elements apart: longer rows are refused above
+        raise ValueError(f"{name} is a negative view: resolve_neg it first")
     # of a single row, what the stride says is of no account
     return n, dim, (stride if n > 1 else dim) * t.element_size()
 
@@ -112,6 +114,8 @@ def _out(out: Optional[torch.Tensor], n: int, dim: int, like: torch.Tensor):
     stride = _more_rows(out, "out", n, dim, like)
     if stride < dim * out.element_size():
         raise ValueError("the rows of out overlap")
+    if out.is_conj():
+        raise ValueError("out is a conjugate view: resolve_conj it first")
     return out, stride
 
 
@@ -199,6 +203,8 @@ def expert_dispatch(x: torch.Tensor, order: ExpertOrder, out: Optional[torch.Ten
     if _elsewhere(x, stream):
         return _run_there(expert_dispatch, x, stream, x, order, out)
     n, dim, x_stride = _rows(x, "x")
+    if x.is_conj():
+        raise ValueError("x is a conjugate view: resolve_conj it first")
     if not x.is_cuda:
         raise ValueError("x must be on a GPU")
     tokens, top_k, experts, offsets, position = _order(order, x)
