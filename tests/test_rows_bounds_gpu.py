@@ -283,3 +283,25 @@ def test_find_layer_norm_refuses_misaligned_buffers_before_the_lookup():
     torch.cuda.synchronize()
     assert not found.any() and (out == 5).all() and (spare == 5).all()
     t.close()
+
+
+# ---- sums over many rows ---------------------------------------------------------------
+
+
+def test_column_sums_of_many_long_rows():
+    """One row of x and dy for 262,144 rows: every column adds a constant, whose rounding
+    errors do not cancel.  A term passes 64 additions of a run, 64 runs, and 6 + 5 in the
+    kernel that adds the 64 row splits; each product adds 3 roundings."""
+    n, dim = 1 << 18, 8196
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, dy = torch.randn((1, dim), generator=g, device="cuda"), torch.randn((1, dim), generator=g, device="cuda")
+    dy[0, :100] = 0.1
+    _, mean, rstd = hkv.layer_norm(x)
+    out = torch.empty((n, dim), device="cuda")
+    _, dw, db = hkv.layer_norm_backward(dy.expand(n, dim), x.expand(n, dim), torch.ones(dim, device="cuda"),
+                                        mean.expand(n).contiguous(), rstd.expand(n).contiguous(), out=out)
+    xhat = (x[0].double() - mean.double()) * rstd.double()
+    want_w, want_b = n * dy[0].double() * xhat, n * dy[0].double()
+    chain = (64 + 64 + 11) * U
+    check(dw, want_w, (chain + 3 * U) * want_w.abs() + rounded(want_w, dw.dtype), "d_weight")
+    check(db, want_b, chain * want_b.abs() + rounded(want_b, db.dtype), "d_bias")
