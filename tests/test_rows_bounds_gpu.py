@@ -2,6 +2,7 @@
 rows far from zero, batches and offsets past the sizes of the other tests."""
 import os
 import sys
+import threading
 
 import numpy as np
 import pytest
@@ -53,6 +54,53 @@ def test_find_layer_norm_is_refused_inside_a_capture(warm):
     assert torch.equal(y, want) and (out == 5).all() and not found.any()
     t.find_layer_norm(n, keys, out, found)
     assert found.all() and torch.equal(out, want)
+    t.close()
+
+
+def test_find_layer_norm_on_several_streams_and_threads_at_once():
+    """Readers share the table: the first takes the table's scratch, the others bring
+    their own, and a batch that is larger than any before replaces the scratch while
+    calls are under way.  Keys may come twice, and n may be one.  The bits are those of
+    the same call alone (the order of a row's sums goes by the batch's size), and the
+    rows those of the keys: their values are off by far less than 2^-12 of 1."""
+    dim, stored = 48, 30000
+    t = make_table(dim, capacity=1 << 16)
+    keys, rows = to_dev(unique_keys(stored, seed=5)), torch.randn((stored, dim), device="cuda")
+    t.insert_or_assign(stored, keys, rows)
+    want = hkv.layer_norm(rows, stats=False)
+    torch.cuda.synchronize()
+    failed, results = [], []
+
+    def ask(seed):
+        try:
+            g = torch.Generator(device="cuda").manual_seed(seed)
+            stream = torch.cuda.Stream()
+            kept = []
+            with torch.cuda.stream(stream):
+                for turn in range(12):
+                    n = 1 if turn == 3 else 500 * (turn + 1) * (seed % 3 + 1)
+                    at = torch.randint(0, stored, (n,), generator=g, device="cuda")
+                    out = torch.zeros((n, dim), device="cuda")
+                    found = torch.zeros(n, dtype=torch.bool, device="cuda")
+                    t.find_layer_norm(n, keys[at], out, found)
+                    kept.append((at, out, found))
+                stream.synchronize()
+                results.extend(kept)
+        except BaseException as e:      # noqa: BLE001 - reported by the main thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=ask, args=(seed,)) for seed in range(6)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not failed, failed
+    assert len(results) == 6 * 12
+    for at, out, found in results:
+        alone, again = torch.zeros_like(out), torch.zeros_like(found)
+        t.find_layer_norm(at.numel(), keys[at], alone, again)
+        assert found.all() and torch.equal(out, alone)
+        assert (out - want[at]).abs().max() < 2.0 ** -12
     t.close()
 
 
