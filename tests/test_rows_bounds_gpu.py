@@ -353,3 +353,57 @@ def test_column_sums_of_many_long_rows():
     chain = (64 + 64 + 11) * U
     check(dw, want_w, (chain + 3 * U) * want_w.abs() + rounded(want_w, dw.dtype), "d_weight")
     check(db, want_b, chain * want_b.abs() + rounded(want_b, db.dtype), "d_bias")
+
+
+# ---- calls that no other test makes ------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n,dim", [(6, 64), (5000, 64), (700, 333), (4, 20000)])
+def test_one_row_for_all(n, dim, dtype):
+    """Inputs whose rows are one row (a distance of zero) give the bits of their copies."""
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    x = torch.randn((1, dim), generator=g, device="cuda").to(dtype).expand(n, dim)
+    w = 1 + 0.2 * torch.randn(dim, generator=g, device="cuda")
+    want = hkv.layer_norm(x.contiguous(), w, w)
+    got = hkv.layer_norm(x, w, w)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    want = hkv.layer_norm_backward(x.contiguous(), x.contiguous(), w, *want[1:])
+    got = hkv.layer_norm_backward(x, x, w, *got[1:])
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    tokens, experts = n // 2, 3
+    order = hkv.expert_sort(torch.randint(-1, experts, (tokens, 2), generator=g, device="cuda"), experts)
+    m = int(order.offsets[-1])
+    one, wt = x[:tokens], torch.randn((tokens, 2), generator=g, device="cuda")
+    assert torch.equal(hkv.expert_dispatch(one, order)[:m], one[:1].expand(m, dim))
+    y = x[:1].expand(tokens * 2, dim)
+    assert torch.equal(hkv.expert_combine(y, wt, order), hkv.expert_combine(y.contiguous(), wt, order))
+    got = hkv.expert_combine_backward(one, y, wt, order)
+    want = hkv.expert_combine_backward(one.contiguous(), y.contiguous(), wt, order)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("n", [300, 20000])
+def test_layer_norm_by_address_captured_and_replayed(n):
+    """The addresses are read when the graph runs: rows may move between replays, become
+    misses and come back."""
+    dim = 48
+    g = torch.Generator(device="cuda").manual_seed(n)
+    table = torch.randn((2 * n, dim), generator=g, device="cuda")
+    want, mean, rstd = hkv.layer_norm(table)
+    ptrs, out = torch.zeros(n, dtype=torch.int64, device="cuda"), torch.zeros((n, dim), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        hkv.layer_norm_ptr(n, ptrs, out)
+    for turn in range(3):
+        at = torch.randint(0, 2 * n, (n,), generator=g, device="cuda")
+        miss = torch.rand(n, generator=g, device="cuda") < 0.3
+        ptrs.copy_(torch.where(miss, 0, table.data_ptr() + at * (dim * 4)))
+        out.fill_(5)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = hkv.layer_norm_ptr(n, ptrs, torch.full_like(out, 5))
+        assert torch.equal(out, eager) and (out[miss] == 5).all()
+        assert (out[~miss] - want[at[~miss]]).abs().max() < 2.0 ** -12
