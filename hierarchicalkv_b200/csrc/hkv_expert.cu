@@ -16,7 +16,7 @@
 // Sums and products are in 32-bit floats and every result is rounded once.
 // No floats are added with atomics: results do not depend on the order in which
 // blocks run.  Measured, us, and the share of the bandwidth of a copy: 16384 tokens of
-// 8 rows of 4096 bf16, sort 12 and dispatch 189, 93 % together; combine 65536 of 2 of
+// 8 rows of 4096 bf16, sort 12 and dispatch 187, 94 % together; combine 65536 of 2 of
 // 128 f32 15, 95 %; its gradient 8192 of 8 of 2048 bf16 93, 95 %; rows of 1001 half,
 // moved in 2-byte units and bound by the latency of so many small loads, combine 85,
 // 69 % (30011 of 6), gradient 130, 59 % (20000 of 6).
@@ -479,6 +479,11 @@ constexpr int kMoveBlock = 256;
 //   gradient of combine 2 x 4: 93    2 x 2: 97, 29    1 x 4: 101    4 x 2: 97, 28
 //     units of 2        8 x 2: 129   4 x 3: 134   4 x 2: 142   8 x 1: 145
 //     units of 4        4 x 2: 45, 73   8 x 2: 48, 73   4 x 3: 57, 77   8 x 1: 64, 84
+// The gradient of combine takes 2 x 4 where a token has more than two experts.  With one or
+// two half or more of the four places would stay empty, so there it takes 4 x 2 (4 x 2 and
+// 2 x 4, one expert: 65536 x 128 f32 18 and 28, 16384 x 2048 bf16 34 and 50, 8192 x 4096 f32
+// 69 and 91, 300000 x 64 bf16 30 and 67; two: 28 and 33, 52 and 62, 107 and 118, 41 and 72;
+// only 100 x 4096 bf16 goes the other way, 3.4 and 3.2).
 struct Shape {
   int units, assigned;
 };

@@ -16,9 +16,11 @@
 // bf16 91 us without either, 94 and 104; 300000 x 100 half 37, 38 and 42; with far rows
 // only, 135 us at 16384 x 8192 bf16).
 // Measured, us, and the share of the bandwidth of a copy: 1048576 x 64 f32 98, 87 %
-// (by address with a tenth missing 80, 94 %); 16384 x 8192 bf16 91, 91 %; rows in
-// narrow units, which are bound by their instructions: 65536 x 1001 bf16 49, 83 %,
-// 65537 x 333 half 23, 59 %.
+// (by address with a tenth missing 80, 95 %); 16384 x 8192 bf16 94, 89 %; rows in
+// narrow units, which are bound by their instructions: 65536 x 1001 bf16 50, 82 %,
+// 65537 x 333 half 25, 55 %; rows past the registers, in scalar loads: 4096 x 12288 f32
+// 191, 33 %.  (The comparisons beside the code below were taken before the means of far
+// rows were corrected, but for that of rows by address.)
 //
 // Rows are given by base and stride, or (the pointer form) by one address per
 // row, as find* returns them: rows are then normalised straight from where the
@@ -324,9 +326,11 @@ int launch_norm_type(const NormArgs& a, cudaStream_t stream) {
   const RowsIn in = rows_in(a.x, a.x_stride);
   uint32_t per_thread = fitting_units(units, BYTES, unit_choices<T, BYTES>());
   // rows of floats by address: two units, for two blocks per multiprocessor, whose
-  // warps wait for addresses and rows in turn (us, with two units and with four:
-  // 1048576 x 64 80 and 84, 262144 x 128 41 and 43, 65536 x 1024 76 and 76; but
-  // rows by base and stride 1048576 x 64 100 and 96)
+  // warps wait for addresses and rows in turn (us, with two units and without the
+  // rule, a tenth missing: 1048576 x 48 76 and 78, x 64 81 and 85, 524288 x 128 77 and 83,
+  // 300000 x 200 75 and 80, 131072 x 512 76 and 81, 65536 x 1024 77 and 76; it loses at
+  // 262144 x 256, 84 and 76, and 100000 x 600, 90 and 82; by base and stride 1048576 x
+  // 64 takes 100 with two units and 96 with four)
   if (BYTES == 16 && sizeof(T) == 4 && a.row_ptrs != nullptr && per_thread > 2 && units <= 2 * kPipeBlock) {
     per_thread = 2;
   }

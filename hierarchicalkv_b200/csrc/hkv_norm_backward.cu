@@ -12,8 +12,10 @@
 // up in its registers beside the row's own work.  The next rows are on their way
 // into the warps' queues meanwhile, and their mean and rstd into registers (asked
 // for one row ahead instead of two they cost 59 us more at 16384 x 8192 bf16).  That
-// size takes 146 us, 82 % of what its bytes need, bound by the instructions that a
-// row costs its 16 warps beside the arithmetic; 1048576 x 64 f32 130 us, 97 %.  At the
+// size takes 151 us, 83 % of the bandwidth of a copy (norm_reduce_kernel is 6 of them),
+// bound by the instructions that a row costs its 16 warps beside the arithmetic;
+// 1048576 x 64 f32 134 us, 94 %; rows past the registers, 4096 x 12288 bf16, 302 us,
+// 16 %: scalar loads, and x and dy read twice.  At the
 // end each block writes one row of column sums (its groups added in a fixed order),
 // and norm_reduce_kernel adds the blocks' rows in a fixed order: no atomics, the same
 // bits every time.  A thread's column sum is one chain over the rows of its group, n /

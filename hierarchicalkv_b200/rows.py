@@ -10,9 +10,13 @@ distance apart.  Rows are float32, float16 or bfloat16; weights and biases have
 the rows' type or float32, and so have their gradients.  The calls run on the
 current stream of the tensors' device, or on ``stream``, and do not synchronise.
 ``out`` arguments receive the result (they must not overlap an input); without
-them it is a new tensor.  The functions are outside autograd: the gradients are
-the functions whose names end in ``_backward``, to be called by the training
-step, as accum_or_assign is.
+them it is a new tensor.  Inputs that were made on another stream than the one of
+the call must be complete there, and stay allocated until it has run.
+
+The functions are outside autograd: a tensor that requires gradients is taken for
+its values, and the results carry no graph, whether gradients are enabled or not.
+The gradients are the functions whose names end in ``_backward``, to be called by
+the training step, as accum_or_assign is.
 """
 from __future__ import annotations
 
@@ -199,7 +203,8 @@ def expert_dispatch(x: torch.Tensor, order: ExpertOrder, out: Optional[torch.Ten
                     stream=None) -> torch.Tensor:
     """Copies of the token rows in the order of the experts: [tokens * top_k, dim]
     with row ``order.position[t, j]`` = x[t].  Rows behind the last expert's are
-    zeros in a new tensor and left as they are in ``out``.  Any element type."""
+    zeros in a new tensor and left as they are in ``out``.  Any element type.
+    Records no graph: the gradient is expert_dispatch_backward."""
     if _elsewhere(x, stream):
         return _run_there(expert_dispatch, x, stream, x, order, out)
     n, dim, x_stride = _rows(x, "x")
@@ -251,7 +256,8 @@ def expert_combine(rows: torch.Tensor, weights: torch.Tensor, order: ExpertOrder
                    out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """The experts' rows back in token order: out[t] is the sum over j of
     weights[t, j] * rows[order.position[t, j]].  Dropped assignments add nothing,
-    whatever their weight; a token without any gets zeros."""
+    whatever their weight; a token without any gets zeros.  Records no graph: the
+    gradients are expert_combine_backward."""
     if _elsewhere(rows, stream):
         return _run_there(_combine, rows, stream, rows, weights, order, out)
     return _combine(rows, weights, order, out)
@@ -301,7 +307,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                out: Optional[torch.Tensor] = None, stream=None):
     """Layer norm of every row of x [n, dim].  Returns (y, mean, rstd), the
     statistics (float32 [n]) being what layer_norm_backward needs, or y alone
-    with ``stats=False``."""
+    with ``stats=False``.  Records no graph: the gradients are layer_norm_backward."""
     if _elsewhere(x, stream):
         return _run_there(layer_norm, x, stream, x, weight, bias, eps, stats, out)
     n, dim, stride, kind = _float_rows(x, "x")
